@@ -15,7 +15,8 @@
  * (src/ggml-xdna.cpp:316-470) as plain C calls, because without ggml the
  * compat ABI has no way to place weights in a device buffer.  Section 3 is the
  * thin launcher layer over the CUDA kernels (device pointers, explicit stream).
- * Section 4 is the N-row sharded multi-GPU path.
+ * Section 4 is the N-row sharded multi-GPU path.  Section 5 holds the paged
+ * KV cache operators of a decode step.
  *
  * Error behaviour: bool-returning calls return false and print
  * "[b200 error] ..." to stderr, as the reference does; int-returning calls
@@ -238,6 +239,138 @@ int ggml_backend_xdna_nccl_unique_id(uint8_t out[128]);
 ggml_backend_t ggml_backend_xdna_init_sharded(size_t dev_num, int world, int rank, const uint8_t id[128]);
 /* Rows of an N-row weight owned by `rank`; N must be divisible by world. */
 int ggml_backend_xdna_shard_rows(int64_t n, int world, int rank, int64_t *row0, int64_t *nrows);
+
+/* ============== 5. paged KV cache: step plan, query/key norm + rotation, attention ==============
+ * The operators between the q/k/v matmuls and the output matmul of a decode
+ * step, on device pointers and an explicit stream as in section 3: every
+ * `stream` is a cudaStream_t of the current device.  No reference counterpart
+ * (the reference leaves these ops to ggml's CPU backend).
+ *
+ * Calls return 0, -1 for a refused argument (nothing is launched), or another
+ * negative code for a CUDA error.  They allocate nothing, keep nothing from one call to the
+ * next, never synchronise, and may be captured into CUDA graphs.  Lengths,
+ * tables and slots are read on the device, so a captured call serves other
+ * lengths on replay.  What the device data may hold is bounded there: a block
+ * id outside [0, num_blocks) is never dereferenced (its keys and values read as
+ * zeros), there are no keys behind a table row, and a slot outside the cache is
+ * not written. */
+
+/* K and V of one layer, in blocks of block_size tokens.  Element (block, head,
+ * token, i) of k (and of v) lies at
+ * block * nb_block + head * nb_head + token * nb_token + 2 * i bytes; all three
+ * strides 0 means contiguous [num_blocks][kv_heads][block_size][head_dim]. */
+struct b200_kv_cache {
+    int32_t type;       /* GGML_TYPE_F16 or GGML_TYPE_BF16 */
+    int32_t head_dim;   /* 64, 96, 128 or 256 */
+    int32_t kv_heads;
+    int32_t block_size; /* 16, 32, 64, 128 or 256 */
+    int64_t num_blocks; /* num_blocks * block_size < 2^31 */
+    void *k, *v;        /* device, 16-byte aligned */
+    int64_t nb_token, nb_head, nb_block; /* byte strides, multiples of 16 */
+};
+
+/* The plan of one step over n_seqs requests: request b has cached_lens[b]
+ * tokens in the cache, held by the first ceil(cached / block_size) entries of
+ * its block_table row, and new_lens[b] >= 0 new tokens.  New blocks come from
+ * free_blocks[*free_head ...] in request order and are written into the table.
+ * Outputs:
+ *   cu_new[n_seqs + 1]   first new token of each request, and their total
+ *   kv_lens[n_seqs]      cached + new (may be cached_lens itself)
+ *   positions, slots     [max_tokens]: each new token's position in its request
+ *                        and its cache slot, block * block_size + offset; from
+ *                        the total on: 0 and -1
+ *   *free_head_out       *free_head + blocks taken (may be free_head itself)
+ *   *status              0, or B200_KV_* bits; then tokens without a block have
+ *                        slot -1 and the step must not be run
+ * Table entries that no new token needs are left as they are. */
+enum {
+    B200_KV_BAD_LENGTH = 1,  /* a negative length, or one whose sum passes 2^31 - 1 (taken as 0 new tokens) */
+    B200_KV_ROW_TOO_SHORT = 2, /* a request needs more than table_width blocks */
+    B200_KV_NO_FREE_BLOCK = 4, /* the free list ran out */
+    B200_KV_TOO_MANY_TOKENS = 8 /* more than max_tokens new tokens: those behind are left out, cu_new stops there */
+};
+struct b200_kv_plan_args {
+    int32_t n_seqs;      /* <= 16384 */
+    int32_t block_size;  /* 16, 32, 64, 128 or 256 */
+    const int32_t *cached_lens, *new_lens; /* [n_seqs] */
+    int32_t *block_table;                  /* [n_seqs][table_width] */
+    int64_t table_width;
+    const int32_t *free_blocks;            /* [n_free] */
+    int64_t n_free;
+    const int32_t *free_head;              /* NULL: 0 */
+    int32_t *free_head_out;                /* NULL: not written */
+    int32_t *cu_new, *kv_lens;
+    int32_t *positions;                    /* NULL: not written */
+    int64_t *slots;
+    int64_t max_tokens;
+    int32_t *status;
+};
+int b200_kv_plan(const struct b200_kv_plan_args *plan, void *stream);
+
+/* For every token t and head: RMS norm of its head_dim values (where a weight
+ * is given) and rotation by positions[t], queries into q_out, keys and values
+ * (values unchanged) into the cache at slots[t]:
+ *   y = x * rsqrt(mean(x^2) + eps) * w
+ *   a_i = positions[t] * freq_scale * freq_base^(-2i / n_rot) / freq_factors[i]
+ *   (y_u, y_v) -> (y_u cos a_i - y_v sin a_i, y_u sin a_i + y_v cos a_i), i < n_rot / 2
+ * with (u, v) = (2i, 2i + 1), or (i, i + n_rot / 2) when neox (ggml's rope
+ * modes 0 and 2).  Angles are formed in 64 bits, the rest in F32, rounded once
+ * into the output type.  q_out may be q itself (same type and stride). */
+struct b200_qk_norm_rope_args {
+    int64_t n_tokens;
+    int32_t heads;             /* query heads */
+    int32_t in_type, out_type; /* F32, F16 or BF16: of q, k, v; of q_out */
+    int32_t n_rot;             /* rotated dimensions: a multiple of 8, 0 .. head_dim */
+    const void *q, *k, *v;     /* [n_tokens][heads or kv_heads][head_dim], 16-byte aligned */
+    int64_t nb_q, nb_k, nb_v;  /* byte strides between tokens, multiples of 16; 0: contiguous */
+    void *q_out;
+    int64_t nb_q_out;
+    const float *q_norm, *k_norm; /* [head_dim], 16-byte aligned; NULL: no norm */
+    const int32_t *positions;     /* [n_tokens] */
+    const int64_t *slots;         /* [n_tokens]; a slot outside the cache (-1) is not written */
+    const float *freq_factors;    /* [n_rot / 2] or NULL */
+    float eps, freq_base, freq_scale;
+    int32_t neox;
+};
+int b200_qk_norm_rope(const struct b200_qk_norm_rope_args *p, const struct b200_kv_cache *kv, void *stream);
+
+/* Causal attention of every request's new tokens over its paged cache (which
+ * already holds their keys and values).  Row t of request b, t in
+ * [cu_new[b], cu_new[b + 1]), has position p = kv_lens[b] - cu_new[b + 1] + t
+ * and sees the keys j <= p (j > p - window with a window):
+ *   s_j = scale q.k_j;  s_j = c tanh(s_j / c) with logit_softcap c;
+ *   s_j += slope_h (j - p) with max_bias (ggml's ALiBi slopes of `heads` heads)
+ *   out = sum_j softmax(s)_j v_j, or 0 for a row that sees no key (p < 0) or
+ *   none but with a score of -inf
+ * Query head h reads KV head h / (heads / kv_heads).  Rows of q that belong to
+ * no request leave their row of out as it is.  q and out are F32 or of the
+ * cache's type.  Scores, softmax and sums are held in F32; with 16-bit q the
+ * softmax weights are rounded to the cache's type for the product with V, with
+ * F32 q both products carry F32's precision.
+ * Keys behind kv_lens[b] may hold anything, NaN included; the values of keys
+ * in front of it are finite (a request's own non-finite values may reach rows
+ * of that request that do not see them). */
+struct b200_paged_attention_args {
+    int64_t n_tokens;        /* rows of q and out */
+    int32_t n_seqs, heads;
+    int32_t q_type, out_type;
+    const void *q;           /* [n_tokens][heads][head_dim], 16-byte aligned */
+    void *out;
+    int64_t nb_q, nb_out;    /* byte strides between tokens, multiples of 16; 0: contiguous */
+    const int32_t *cu_new;   /* [n_seqs + 1], not decreasing */
+    const int32_t *kv_lens;  /* [n_seqs] */
+    const int32_t *block_table; /* [n_seqs][table_width] */
+    int64_t table_width;
+    int32_t max_new, max_kv; /* the most of any request: they choose kernels and work split, not results */
+    float scale, logit_softcap, max_bias; /* 0: no cap, no bias */
+    int32_t window;          /* 0: none */
+    void *workspace;         /* device, 16-byte aligned, not shared by calls that may overlap in time */
+    size_t workspace_bytes;
+};
+/* Bytes of workspace the call needs (0 is possible); they depend on the sizes,
+ * types and hints, not on device data. */
+size_t b200_paged_attention_workspace(const struct b200_paged_attention_args *p, const struct b200_kv_cache *kv);
+int b200_paged_attention(const struct b200_paged_attention_args *p, const struct b200_kv_cache *kv, void *stream);
 
 #ifdef __cplusplus
 }

@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -21,9 +22,10 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libggml-b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CU_SOURCES = ["gemv.cu", "gemv_mma.cu", "repack.cu", "quantize.cu"]
-CXX_SOURCES = ["backend.cpp"]
-HEADERS = ["formats.cuh", "gemv.cuh", "nccl_shim.h"]
+CU_SOURCES = ["gemv.cu", "gemv_mma.cu", "repack.cu", "quantize.cu", "kv_plan.cu", "qk_norm_rope.cu",
+              "paged_attention.cu"]
+CXX_SOURCES = ["backend.cpp", "paged_api.cpp"]
+HEADERS = ["formats.cuh", "gemv.cuh", "nccl_shim.h", "paged.cuh", "paged_attn.cuh"]
 
 
 def _stale(target: str, deps: list[str]) -> bool:
@@ -42,7 +44,7 @@ def build(verbose: bool = False) -> str:
     common = [os.path.join(CSRC, h) for h in HEADERS] + [tables, os.path.join(HERE, "..", "include", "ggml-b200.h")]
     flags = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I", BUILD, "-I", CSRC,
                     "--expt-relaxed-constexpr"]
-    objs = []
+    objs, cmds = [], []
     for src in CU_SOURCES + CXX_SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(BUILD, src + ".o")
@@ -51,7 +53,10 @@ def build(verbose: bool = False) -> str:
             cmd = [NVCC] + flags + (["-x", "cu"] if src.endswith(".cu") else []) + ["-c", s, "-o", o]
             if src.endswith(".cu"):
                 cmd += ["-Xptxas", "-v"] if verbose else []
-            subprocess.run(cmd, check=True)
+            cmds.append(cmd)
+    with ThreadPoolExecutor(max_workers=os.cpu_count()) as pool:  # the compilers run in parallel
+        for done in [pool.submit(subprocess.run, cmd, check=True) for cmd in cmds]:
+            done.result()
     if _stale(LIB, objs):
         subprocess.run([NVCC] + ARCH + ["-shared", "-o", LIB] + objs + ["-lcudart_static", "-lrt", "-ldl", "-lpthread"],
                        check=True)

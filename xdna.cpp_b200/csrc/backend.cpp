@@ -38,6 +38,7 @@ namespace xb {
 // ------------------------------------------------------------------ errors
 namespace {
 thread_local std::string g_last_error;
+}  // namespace
 
 void set_error(const char* fmt, ...) {
     char buf[1024];
@@ -49,6 +50,7 @@ void set_error(const char* fmt, ...) {
     fprintf(stderr, "[b200 error] %s\n", buf);
 }
 
+namespace {
 bool cuda_ok(cudaError_t e, const char* what) {
     if (e == cudaSuccess) return true;
     set_error("%s: %s", what, cudaGetErrorString(e));

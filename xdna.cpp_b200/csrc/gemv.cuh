@@ -6,6 +6,9 @@
 
 namespace xb {
 
+// Records the calling thread's last error and prints it (backend.cpp).
+void set_error(const char* fmt, ...);
+
 // Devices a process may use with the per-device caches of this library.
 constexpr int kMaxDevices = 64;
 

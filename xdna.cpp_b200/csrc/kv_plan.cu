@@ -1,0 +1,188 @@
+// The plan of a step over a paged KV cache: block tables, cache slots and
+// positions of every request's new tokens, from the request lengths.
+//
+// Mathematics: with owned_b = ceil(cached_b / bs) and need_b =
+// ceil((cached_b + new_b) / bs) - owned_b, the exclusive prefix sums of new
+// and need give each request its first token and its first free-list entry.
+// Token t of request b has position pos = cached_b + t - cu_b and lies in the
+// request's block pos / bs: a block the request owns (read from its table
+// row), or free[head + first_b + pos / bs - owned_b].
+//
+// The work is a few bytes per token, so the call is bound by latency: one
+// launch, in which every CTA forms the prefix sums of all requests for itself
+// (8 bytes a request, from L2) and then takes its share of the tokens.  The
+// CTAs form one cluster: its barrier stands between the last read of the
+// lengths and the head and the first write to them, so both may be updated in
+// place, and no counter in memory has to be kept.
+#include <cuda_runtime.h>
+
+#include "gemv.cuh"
+#include "paged.cuh"
+
+namespace xb {
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kCluster = 8;
+constexpr int kOneCtaTokens = 2048;  // up to here one CTA takes the tokens in two rounds
+
+struct Sum {
+    long long tokens, blocks;
+};
+
+__device__ __forceinline__ Sum warp_inclusive(Sum v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, v.tokens, d);
+        const long long n = __shfl_up_sync(0xffffffffu, v.blocks, d);
+        if (lane >= d) {
+            v.tokens += t;
+            v.blocks += n;
+        }
+    }
+    return v;
+}
+
+struct Lens {
+    int cached, fresh;
+    bool bad;
+};
+
+__device__ __forceinline__ Lens read_lens(const struct b200_kv_plan_args& p, int b) {
+    const int c = p.cached_lens[b], n = p.new_lens[b];
+    Lens l{c, n, false};
+    if (c < 0 || n < 0 || static_cast<long long>(c) + n > 0x7fffffffLL) l = Lens{c < 0 ? 0 : c, 0, true};
+    return l;
+}
+
+template <int kCtas>
+__global__ void __launch_bounds__(kThreads) kv_plan_kernel(const __grid_constant__ struct b200_kv_plan_args p, int log_bs) {
+    // Held to 32 bits: sums past max_tokens or 2^31 - 1 blocks are cut there, and
+    // no token that is written lies behind a cut (the status says so).
+    extern __shared__ int prefix[];  // [n_seqs] first token, then [n_seqs] first free-list entry
+    int* first_token = prefix;
+    int* first_block = prefix + p.n_seqs;
+    __shared__ Sum warp_sum[32];
+    __shared__ int flags;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = static_cast<int>(blockIdx.x);
+    const int B = p.n_seqs, bs = 1 << log_bs;
+    if (tid == 0) flags = 0;
+    grid_wait();
+    __syncthreads();
+
+    // prefix sums: a thread owns `per` consecutive requests
+    const int per = (B + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
+    const int head = p.free_head ? *p.free_head : 0;
+    Sum mine{0, 0};
+    int bad = 0;
+    for (int b = b0; b < b1; ++b) {
+        const Lens l = read_lens(p, b);
+        const long long owned = (static_cast<long long>(l.cached) + bs - 1) >> log_bs;
+        const long long held = (static_cast<long long>(l.cached) + l.fresh + bs - 1) >> log_bs;
+        if (l.bad) bad |= B200_KV_BAD_LENGTH;
+        if (held > p.table_width) bad |= B200_KV_ROW_TOO_SHORT;
+        mine.tokens += l.fresh;
+        mine.blocks += held - owned;
+    }
+    const Sum inc = warp_inclusive(mine);
+    if (lane == 31) warp_sum[warp] = inc;
+    if (bad) atomicOr(&flags, bad);
+    __syncthreads();
+    if (warp == 0) warp_sum[lane] = warp_inclusive(warp_sum[lane]);
+    __syncthreads();
+    const Sum before = warp ? warp_sum[warp - 1] : Sum{0, 0};
+    const Sum all = warp_sum[31];
+    Sum run{before.tokens + inc.tokens - mine.tokens, before.blocks + inc.blocks - mine.blocks};
+    for (int b = b0; b < b1; ++b) {
+        const Lens l = read_lens(p, b);
+        first_token[b] = static_cast<int>(run.tokens < p.max_tokens ? run.tokens : p.max_tokens);
+        first_block[b] = static_cast<int>(run.blocks < 0x7fffffffLL ? run.blocks : 0x7fffffffLL);
+        run.tokens += l.fresh;
+        run.blocks += ((static_cast<long long>(l.cached) + l.fresh + bs - 1) >> log_bs) -
+                      ((static_cast<long long>(l.cached) + bs - 1) >> log_bs);
+    }
+    if (tid == 0) {
+        int f = flags;
+        if (head < 0 || head + all.blocks > p.n_free) f |= B200_KV_NO_FREE_BLOCK;
+        if (all.tokens > p.max_tokens) f |= B200_KV_TOO_MANY_TOKENS;
+        if (rank == 0) *p.status = f;
+    }
+    __syncthreads();
+
+    // the tokens of this CTA (cached_lens is read here for the last time)
+    const long long total = all.tokens < p.max_tokens ? all.tokens : p.max_tokens;
+    for (long long t = static_cast<long long>(rank) * kThreads + tid; t < p.max_tokens; t += kCtas * kThreads) {
+        if (t >= total) {
+            if (p.positions) p.positions[t] = 0;
+            p.slots[t] = -1;
+            continue;
+        }
+        int lo = 0, hi = B;  // the last request whose first token is at or before t
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first_token[mid] <= t) lo = mid; else hi = mid;
+        }
+        const int cached = max(p.cached_lens[lo], 0);
+        const int pos = cached + static_cast<int>(t - first_token[lo]);
+        const long long owned = (static_cast<long long>(cached) + bs - 1) >> log_bs;
+        const int page = pos >> log_bs;
+        int block = -1;
+        if (page < p.table_width) {
+            int32_t* entry = p.block_table + static_cast<long long>(lo) * p.table_width + page;
+            if (page < owned) {
+                block = *entry;
+            } else {
+                const long long i = static_cast<long long>(head) + first_block[lo] + page - owned;
+                if (i >= 0 && i < p.n_free) {
+                    block = p.free_blocks[i];
+                    // the block's first token is new, and its thread alone writes the entry
+                    if ((pos & (bs - 1)) == 0) *entry = block;
+                }
+            }
+        }
+        if (p.positions) p.positions[t] = pos;
+        p.slots[t] = block < 0 ? -1 : static_cast<int64_t>(block) * bs + (pos & (bs - 1));
+    }
+
+    // every CTA has read the lengths and the head: now they may be overwritten
+    if (kCtas > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
+    if (rank == 0) {
+        for (int b = tid; b <= B; b += kThreads) {
+            p.cu_new[b] = b < B ? first_token[b] : static_cast<int32_t>(total);
+            if (b < B) {
+                const Lens l = read_lens(p, b);
+                p.kv_lens[b] = l.cached + l.fresh;
+            }
+        }
+        if (tid == 0 && p.free_head_out) {
+            const long long h = head + all.blocks;
+            *p.free_head_out = static_cast<int32_t>(head < 0 ? head : h < p.n_free ? h : p.n_free);
+        }
+    }
+}
+
+}  // namespace
+
+cudaError_t kv_plan_launch(const struct b200_kv_plan_args& p, cudaStream_t stream) {
+    int log_bs = 4;
+    while ((1 << log_bs) < p.block_size) ++log_bs;
+    const size_t smem = 2 * static_cast<size_t>(p.n_seqs) * sizeof(int);
+    const bool one = p.max_tokens <= kOneCtaTokens;
+    void (*kernel)(const struct b200_kv_plan_args, int) = one ? kv_plan_kernel<1> : kv_plan_kernel<kCluster>;
+    if (smem > 48 * 1024) {
+        const cudaError_t e =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+    }
+    return launch_pdl(kernel, dim3(one ? 1 : kCluster), dim3(kThreads), smem, stream, one ? 1 : kCluster, p, log_bs);
+}
+
+}  // namespace xb

@@ -1,0 +1,54 @@
+// Internal launcher interface of the paged KV cache operators.  The argument
+// records are those of the public header; the entry points (paged_api.cpp)
+// have checked them and filled in the strides.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/ggml-b200.h"
+
+namespace xb {
+
+cudaError_t kv_plan_launch(const struct b200_kv_plan_args& p, cudaStream_t stream);
+
+cudaError_t qk_norm_rope_launch(const struct b200_qk_norm_rope_args& p, const struct b200_kv_cache& kv,
+                                cudaStream_t stream);
+
+size_t paged_attention_workspace(const struct b200_paged_attention_args& p, const struct b200_kv_cache& kv);
+cudaError_t paged_attention_launch(const struct b200_paged_attention_args& p, const struct b200_kv_cache& kv,
+                                   cudaStream_t stream);
+
+// Launch with programmatic stream serialization: the kernel may start while
+// the one before it on the stream drains.  Every thread of every kernel
+// launched so executes griddepcontrol.wait before its first access to global
+// memory (and before it returns), so stream order holds as without it.
+template <typename... Params, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                       int cluster, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    if (cluster > 1) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = cluster;
+        attr[1].val.clusterDim.y = 1;
+        attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+    }
+    cfg.attrs = attr;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+#endif
+
+}  // namespace xb

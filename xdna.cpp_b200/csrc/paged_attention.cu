@@ -1,0 +1,322 @@
+// Causal attention of new tokens over a paged KV cache: the tile kernel.
+//
+// Mathematics: a row (token i, head h) at position p sees the keys j <= p (and
+// j > p - window).  One pass over the keys keeps the row's running maximum m,
+// its sum l = sum 2^(s_j - m) and o = sum 2^(s_j - m) v_j, where s_j is the
+// score times log2(e); a larger maximum scales l and o by 2^(m - m').  The
+// row's output is o / l.
+//
+// The query heads that share a KV head are rows of the same tile (row r is
+// token r / group, head r % group), so a K/V tile is read once for all of
+// them.  A CTA of 4 warps takes 64 rows, 16 per warp; K and V tiles of kKeys
+// keys come through a two-stage cp.async ring of shared memory, in rows padded
+// by 16 bytes (an odd number of 16-byte columns: ldmatrix reads 8 rows without
+// a bank conflict).  F32 queries run as NP 16-bit pieces of q and of the
+// softmax weights, whose products with the exact 16-bit K and V add up in F32.
+#include <cfloat>
+#include <cmath>
+
+#include "paged_attn.cuh"
+
+namespace xb {
+namespace {
+
+constexpr int kRows = 64;
+constexpr int kThreads = 128;
+
+template <typename T, int D, int NP>
+struct Tile {
+    static constexpr int kKeys = D > 128 ? 32 : 64;
+    static constexpr int kStride = D + 8;  // elements per row
+    static constexpr int kQ = kRows * kStride;
+    static constexpr int kK = kKeys * kStride;
+    static constexpr size_t kBytes = (NP * kQ + 4 * kK) * sizeof(uint16_t) + kRows * sizeof(float);
+};
+
+// The request and the row tile of the x-th tile of kRows rows, found by every
+// warp for itself; false behind the last one.
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, int64_t x, int& b, int& tile) {
+    const int lane = threadIdx.x & 31;
+    for (int base = 0; base < a.p.n_seqs; base += 32) {
+        int64_t n = 0;
+        if (base + lane < a.p.n_seqs) n = (my_rows(a, read_request(a, base + lane)) + kRows - 1) / kRows;
+        int64_t inc = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += o;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, x < inc);
+        if (hit) {
+            const int at = __ffs(hit) - 1;
+            b = base + at;
+            tile = static_cast<int>(x - (__shfl_sync(0xffffffffu, inc, at) - __shfl_sync(0xffffffffu, n, at)));
+            return true;
+        }
+        x -= __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return false;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+    const int bytes = on ? 16 : 0;  // 0: fills with zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+template <typename T, int D, int NP>
+__global__ void __launch_bounds__(kThreads) attn_tile_kernel(const __grid_constant__ AttnArgs a) {
+    using L = Tile<T, D, NP>;
+    constexpr int kKeys = L::kKeys, kS = L::kStride;
+    extern __shared__ __align__(16) uint16_t smem[];
+    uint16_t* qs = smem;
+    uint16_t* ks = qs + NP * L::kQ;
+    uint16_t* vs = ks + 2 * L::kK;
+    float* row_scale = reinterpret_cast<float*>(vs + 2 * L::kK);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    grid_wait();
+
+    int b, tile;
+    if (!find_tile(a, blockIdx.x, b, tile)) return;
+    const Request rq = read_request(a, b);
+    const int kvh = blockIdx.y, G = a.group;
+    const int r0 = tile * kRows, rows = min(kRows, rq.count * G - r0);
+    int lo, hi;
+    key_range(a, rq, r0 / G, (r0 + rows - 1) / G, lo, hi);
+    lo = lo / kKeys * kKeys;
+
+    auto load = [&](int j0, int stage) {
+        constexpr int kChunks = D / 8;
+        for (int i = tid; i < kKeys * kChunks; i += kThreads) {
+            const int r = i / kChunks, c = i - r * kChunks, j = j0 + r;
+            const int id = j < hi ? key_block(a, b, j >> a.log_bs) : -1;
+            const int64_t at = id < 0 ? 0
+                                      : id * a.kv.nb_block + kvh * a.kv.nb_head +
+                                            (j & (a.kv.block_size - 1)) * a.kv.nb_token + c * 16;
+            const int d = stage * L::kK + r * kS + c * 8;
+            cp_async16(smem_addr(ks + d), static_cast<const char*>(a.kv.k) + at, id >= 0);
+            cp_async16(smem_addr(vs + d), static_cast<const char*>(a.kv.v) + at, id >= 0);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (lo < hi) load(lo, 0);
+
+    // the tile's queries, as NP pieces
+    for (int r = warp; r < kRows; r += 4) {
+        const bool on = r < rows;
+        const int i = (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
+        const char* src = static_cast<const char*>(a.p.q) + (rq.first + (on ? i : 0)) * a.p.nb_q;
+        if (NP == 1) {
+            const uint32_t* s = reinterpret_cast<const uint32_t*>(src) + static_cast<int64_t>(h) * (D / 2);
+            for (int c = lane; c < D / 2; c += 32)
+                *reinterpret_cast<uint32_t*>(qs + r * kS + 2 * c) = on ? s[c] : 0u;
+        } else {
+            const float2* s = reinterpret_cast<const float2*>(src) + static_cast<int64_t>(h) * (D / 2);
+            // F16 pieces reach down to 2^-24 only: the row is scaled by a power of
+            // two to a largest value in [1, 2)
+            float big = 0.f, up = 1.f;
+            if (sizeof(T) == 2 && NP == 2) {
+                for (int c = lane; on && c < D / 2; c += 32) big = fmaxf(big, fmaxf(fabsf(s[c].x), fabsf(s[c].y)));
+#pragma unroll
+                for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+                if (big > 0.f && big <= FLT_MAX) up = ldexpf(1.f, min(ilogbf(big), 126));
+            }
+            if (lane == 0) row_scale[r] = up;
+            const float down = 1.f / up;
+            for (int c = lane; c < D / 2; c += 32) {
+                const float2 x = on ? s[c] : make_float2(0.f, 0.f);
+                uint32_t piece[NP];
+                split_pair<T, NP>(x.x * down, x.y * down, piece);
+#pragma unroll
+                for (int k = 0; k < NP; ++k) *reinterpret_cast<uint32_t*>(qs + k * L::kQ + r * kS + 2 * c) = piece[k];
+            }
+        }
+    }
+    __syncthreads();
+
+    // this thread's two rows
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope[2], mul[2];
+    int p[2], last[2], row[2];  // position, last key it sees, row of the tile
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        row[e] = warp * 16 + (lane >> 2) + 8 * e;
+        const int i = (r0 + row[e]) / G;
+        p[e] = rq.pos0() + i;
+        last[e] = min(p[e], hi - 1);
+        slope[e] = head_slope(a, kvh * G + (r0 + row[e]) - i * G);
+        mul[e] = NP == 1 ? a.pre : a.pre * row_scale[row[e]];
+    }
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+
+    int stage = 0;
+    for (int j0 = lo; j0 < hi; j0 += kKeys, stage ^= 1) {
+        if (j0 + kKeys < hi) {
+            load(j0 + kKeys, stage ^ 1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        __syncthreads();
+        const uint16_t* kt = ks + stage * L::kK;
+        const uint16_t* vt = vs + stage * L::kK;
+
+        float s[kKeys / 8][4];
+#pragma unroll
+        for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            uint32_t qf[NP][4];
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+                ldsm4(qf[i], smem_addr(qs + i * L::kQ + (warp * 16 + (lane & 15)) * kS + k * 16 + (lane >> 4) * 8));
+#pragma unroll
+            for (int n = 0; n < kKeys / 16; ++n) {
+                uint32_t kf[4];
+                ldsm4(kf, smem_addr(kt + (n * 16 + (lane & 7) + (lane >> 4) * 8) * kS + k * 16 + ((lane >> 3) & 1) * 8));
+#pragma unroll
+                for (int i = NP - 1; i >= 0; --i) {
+                    mma16816<T>(s[2 * n], qf[i], kf[0], kf[1]);
+                    mma16816<T>(s[2 * n + 1], qf[i], kf[2], kf[3]);
+                }
+            }
+        }
+
+        // scores in units of log 2, hidden keys at -inf
+        float top[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int q = e >> 1, j = j0 + n * 8 + 2 * (lane & 3) + (e & 1);
+                float x = s[n][e] * mul[q];
+                if (a.post != 0.f) x = a.post * tanhf(x);
+                if (a.bias_near) x = fmaf(slope[q], static_cast<float>(j - p[q]), x);
+                if (j > last[q] || (a.p.window > 0 && p[q] - j >= a.p.window)) x = -INFINITY;
+                s[n][e] = x;
+                top[q] = fmaxf(top[q], x);
+            }
+        float base[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 1));
+            top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 2));
+            base[q] = top[q] == -INFINITY ? 0.f : top[q];  // a row that has seen no key yet
+            const float c = exp2f(m[q] - base[q]);
+            m[q] = top[q];
+            l[q] *= c;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+                o[n][2 * q] *= c;
+                o[n][2 * q + 1] *= c;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[n][e] = exp2f(s[n][e] - base[e >> 1]);
+                l[e >> 1] += s[n][e];
+            }
+
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k) {
+            uint32_t pf[NP][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t piece[NP];
+                const float* x = &s[2 * k + (e >> 1)][2 * (e & 1)];
+                split_pair<T, NP>(x[0], x[1], piece);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) pf[i][e] = piece[i];
+            }
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) {
+                uint32_t vf[4];
+                ldsm4_t(vf, smem_addr(vt + (k * 16 + (lane & 15)) * kS + n * 16 + (lane >> 4) * 8));
+#pragma unroll
+                for (int i = NP - 1; i >= 0; --i) {
+                    mma16816<T>(o[2 * n], pf[i], vf[0], vf[1]);
+                    mma16816<T>(o[2 * n + 1], pf[i], vf[2], vf[3]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        l[q] += __shfl_xor_sync(0xffffffffu, l[q], 1);
+        l[q] += __shfl_xor_sync(0xffffffffu, l[q], 2);
+        if (row[q] >= rows) continue;
+        const bool none = m[q] == -INFINITY;  // no key, or only scores of -inf
+        const float inv = 1.f / l[q];
+        const int i = (r0 + row[q]) / G, h = kvh * G + (r0 + row[q]) - i * G;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+            store_out(a, rq.first + i, h, n * 8 + 2 * (lane & 3), none ? 0.f : o[n][2 * q] * inv,
+                      none ? 0.f : o[n][2 * q + 1] * inv);
+    }
+}
+
+template <typename T, int D, int NP>
+cudaError_t launch_tile(const AttnArgs& a, cudaStream_t stream) {
+    using L = Tile<T, D, NP>;
+    const auto kernel = attn_tile_kernel<T, D, NP>;
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L::kBytes));
+    if (e != cudaSuccess) return e;
+    // every request's last tile may be partly filled
+    const int64_t tiles = a.p.n_tokens * a.group / kRows + a.p.n_seqs;
+    return launch_pdl(kernel, dim3(static_cast<unsigned>(tiles), a.kv.kv_heads), dim3(kThreads), L::kBytes, stream, 1,
+                      a);
+}
+template <typename T, int D>
+cudaError_t launch_pieces(const AttnArgs& a, cudaStream_t stream) {
+    return a.p.q_type == GGML_TYPE_F32 ? launch_tile<T, D, Half16<T>::kPieces>(a, stream)
+                                       : launch_tile<T, D, 1>(a, stream);
+}
+template <typename T>
+cudaError_t launch_type(const AttnArgs& a, cudaStream_t stream) {
+    switch (a.kv.head_dim) {
+        case 64: return launch_pieces<T, 64>(a, stream);
+        case 96: return launch_pieces<T, 96>(a, stream);
+        case 128: return launch_pieces<T, 128>(a, stream);
+        default: return launch_pieces<T, 256>(a, stream);
+    }
+}
+
+AttnArgs make_args(const struct b200_paged_attention_args& p, const struct b200_kv_cache& kv) {
+    AttnArgs a = {};
+    a.p = p;
+    a.kv = kv;
+    a.group = p.heads / kv.kv_heads;
+    while ((1 << a.log_bs) < kv.block_size) ++a.log_bs;
+    a.pre = p.logit_softcap != 0.f ? p.scale / p.logit_softcap : p.scale * kLog2e;
+    a.post = p.logit_softcap * kLog2e;
+    if (p.max_bias != 0.f) {
+        a.bias_near = 1;
+        while (2 * a.bias_near <= p.heads) a.bias_near *= 2;
+        a.log2_m0 = -p.max_bias / a.bias_near;
+        a.log2_m1 = -p.max_bias / 2.f / a.bias_near;
+    }
+    a.min_rows = 0;
+    a.max_rows = 0x7fffffff;
+    return a;
+}
+
+}  // namespace
+
+size_t paged_attention_workspace(const struct b200_paged_attention_args&, const struct b200_kv_cache&) { return 0; }
+
+cudaError_t paged_attention_launch(const struct b200_paged_attention_args& p, const struct b200_kv_cache& kv,
+                                   cudaStream_t stream) {
+    const AttnArgs a = make_args(p, kv);
+    return kv.type == GGML_TYPE_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream);
+}
+
+}  // namespace xb

@@ -21,7 +21,7 @@ LIB_PATH = os.environ.get("XDNA_B200_LIB") or os.path.join(HERE, "libggml-b200.s
 HEADER = os.path.join(HERE, "..", "include", "ggml-b200.h")
 
 # ggml type ids
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 30
 Q4_0, Q3_K, Q4_K, Q5_K, Q6_K = 2, 11, 12, 13, 14
 IQ3_XXS, IQ3_S, IQ2_S, IQ4_XS = 18, 21, 22, 23
 CLAIMED = {"Q4_0": Q4_0, "Q3_K": Q3_K, "Q4_K": Q4_K, "Q5_K": Q5_K, "Q6_K": Q6_K,
@@ -50,6 +50,46 @@ GgmlTensorXdna._fields_ = [
     ("name", C.c_char * 64),
     ("extra", C.c_void_p),
 ]
+
+
+class _Record(C.Structure):
+    """An argument record of the paged KV cache operators: fields by keyword,
+    the others 0 / NULL; pointers are device addresses (None: NULL)."""
+
+
+class KvCache(_Record):
+    _fields_ = [("type", C.c_int32), ("head_dim", C.c_int32), ("kv_heads", C.c_int32), ("block_size", C.c_int32),
+                ("num_blocks", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("nb_token", C.c_int64),
+                ("nb_head", C.c_int64), ("nb_block", C.c_int64)]
+
+
+class KvPlan(_Record):
+    _fields_ = [("n_seqs", C.c_int32), ("block_size", C.c_int32), ("cached_lens", C.c_void_p), ("new_lens", C.c_void_p),
+                ("block_table", C.c_void_p), ("table_width", C.c_int64), ("free_blocks", C.c_void_p),
+                ("n_free", C.c_int64), ("free_head", C.c_void_p), ("free_head_out", C.c_void_p), ("cu_new", C.c_void_p),
+                ("kv_lens", C.c_void_p), ("positions", C.c_void_p), ("slots", C.c_void_p), ("max_tokens", C.c_int64),
+                ("status", C.c_void_p)]
+
+
+KV_BAD_LENGTH, KV_ROW_TOO_SHORT, KV_NO_FREE_BLOCK, KV_TOO_MANY_TOKENS = 1, 2, 4, 8
+
+
+class QkNormRope(_Record):
+    _fields_ = [("n_tokens", C.c_int64), ("heads", C.c_int32), ("in_type", C.c_int32), ("out_type", C.c_int32),
+                ("n_rot", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("nb_q", C.c_int64),
+                ("nb_k", C.c_int64), ("nb_v", C.c_int64), ("q_out", C.c_void_p), ("nb_q_out", C.c_int64),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("positions", C.c_void_p), ("slots", C.c_void_p),
+                ("freq_factors", C.c_void_p), ("eps", C.c_float), ("freq_base", C.c_float), ("freq_scale", C.c_float),
+                ("neox", C.c_int32)]
+
+
+class PagedAttention(_Record):
+    _fields_ = [("n_tokens", C.c_int64), ("n_seqs", C.c_int32), ("heads", C.c_int32), ("q_type", C.c_int32),
+                ("out_type", C.c_int32), ("q", C.c_void_p), ("out", C.c_void_p), ("nb_q", C.c_int64),
+                ("nb_out", C.c_int64), ("cu_new", C.c_void_p), ("kv_lens", C.c_void_p), ("block_table", C.c_void_p),
+                ("table_width", C.c_int64), ("max_new", C.c_int32), ("max_kv", C.c_int32), ("scale", C.c_float),
+                ("logit_softcap", C.c_float), ("max_bias", C.c_float), ("window", C.c_int32), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
 
 
 def row_bytes(t: int, K: int) -> int:
@@ -139,6 +179,10 @@ def lib() -> C.CDLL:
         "b200_unpack_host": (C.c_int, [C.c_int, vp, vp, i64, i64]),
         "b200_row_bytes": (sz, [C.c_int, i64]),
         "b200_gemv_smem_bytes": (sz, [C.c_int, i64]),
+        "b200_kv_plan": (C.c_int, [C.POINTER(KvPlan), vp]),
+        "b200_qk_norm_rope": (C.c_int, [C.POINTER(QkNormRope), C.POINTER(KvCache), vp]),
+        "b200_paged_attention_workspace": (sz, [C.POINTER(PagedAttention), C.POINTER(KvCache)]),
+        "b200_paged_attention": (C.c_int, [C.POINTER(PagedAttention), C.POINTER(KvCache), vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
