@@ -238,11 +238,18 @@ __global__ void __launch_bounds__(kThreads) attn_tile_kernel(const __grid_consta
             for (int n = 0; n < D / 16; ++n) {
                 uint32_t vf[4];
                 ldsm4_t(vf, smem_addr(vt + (k * 16 + (lane & 15)) * kS + n * 16 + (lane >> 4) * 8));
+                // The matrix unit cuts its sums off instead of rounding them, which
+                // adds up over a long axis: for F32 every 16 keys' sum starts at 0
+                // and is added by a rounded addition.
+                float t[2][4] = {};
 #pragma unroll
                 for (int i = NP - 1; i >= 0; --i) {
-                    mma16816<T>(o[2 * n], pf[i], vf[0], vf[1]);
-                    mma16816<T>(o[2 * n + 1], pf[i], vf[2], vf[3]);
+                    mma16816<T>(NP > 1 ? t[0] : o[2 * n], pf[i], vf[0], vf[1]);
+                    mma16816<T>(NP > 1 ? t[1] : o[2 * n + 1], pf[i], vf[2], vf[3]);
                 }
+                if (NP > 1)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[2 * n][e] += t[0][e], o[2 * n + 1][e] += t[1][e];
             }
         }
         __syncthreads();
@@ -253,7 +260,7 @@ __global__ void __launch_bounds__(kThreads) attn_tile_kernel(const __grid_consta
         l[q] += __shfl_xor_sync(0xffffffffu, l[q], 1);
         l[q] += __shfl_xor_sync(0xffffffffu, l[q], 2);
         if (row[q] >= rows) continue;
-        const bool none = m[q] == -INFINITY;  // no key, or only scores of -inf
+        const bool none = l[q] == 0.f;  // no key, or only scores of -inf
         const float inv = 1.f / l[q];
         const int i = (r0 + row[q]) / G, h = kvh * G + (r0 + row[q]) - i * G;
 #pragma unroll
@@ -311,11 +318,44 @@ AttnArgs make_args(const struct b200_paged_attention_args& p, const struct b200_
 
 }  // namespace
 
-size_t paged_attention_workspace(const struct b200_paged_attention_args&, const struct b200_kv_cache&) { return 0; }
+int sm_count() {
+    static int count[kMaxDevices];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return 0;
+    if (!count[dev] && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) count[dev] = n;
+    return count[dev];
+}
+
+// Requests of up to kStreamRows rows go to the stream kernel, the others to the
+// tile kernel; where the hints (or a single request) leave no doubt, one kernel
+// takes everything.
+namespace {
+struct Split {
+    bool stream, tile;
+};
+Split split(const AttnArgs& a) {
+    const bool few = static_cast<int64_t>(a.p.max_new) * a.group <= kStreamRows;
+    return Split{few || a.p.n_seqs > 1, !few};
+}
+}  // namespace
+
+size_t paged_attention_workspace(const struct b200_paged_attention_args& p, const struct b200_kv_cache& kv) {
+    const AttnArgs a = make_args(p, kv);
+    return split(a).stream ? stream_workspace(a) : 0;
+}
 
 cudaError_t paged_attention_launch(const struct b200_paged_attention_args& p, const struct b200_kv_cache& kv,
                                    cudaStream_t stream) {
-    const AttnArgs a = make_args(p, kv);
+    AttnArgs a = make_args(p, kv);
+    const Split s = split(a);
+    if (s.stream) {
+        if (s.tile) a.max_rows = kStreamRows;
+        const cudaError_t e = stream_launch(a, stream);
+        if (e != cudaSuccess) return e;
+    }
+    if (!s.tile) return cudaSuccess;
+    a.min_rows = s.stream ? kStreamRows : 0;
+    a.max_rows = 0x7fffffff;
     return kv.type == GGML_TYPE_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream);
 }
 

@@ -4,12 +4,16 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include "gemv.cuh"
 #include "paged.cuh"
 
 namespace xb {
+
+// Streaming multiprocessors of the current device (0 without one).
+int sm_count();
 
 struct AttnArgs {
     struct b200_paged_attention_args p;
@@ -24,6 +28,12 @@ struct AttnArgs {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// The stream kernel (paged_stream.cu): rows (new tokens x group) up to which a
+// request is its work, its workspace, and its launch.
+constexpr int kStreamRows = 32;
+size_t stream_workspace(const AttnArgs& a);
+cudaError_t stream_launch(const AttnArgs& a, cudaStream_t stream);
 
 #ifdef __CUDACC__
 // Slope of a query head, times log2(e).
@@ -60,6 +70,25 @@ __device__ __forceinline__ void key_range(const AttnArgs& a, const Request& r, i
     hi = min(max(0, r.pos0() + i1 + 1), table_keys(a));
     lo = a.p.window > 0 && p0 >= a.p.window ? p0 - a.p.window + 1 : 0;
 }
+// Work of one request in units of kKeys keys: `tiles` row tiles of R rows for
+// each KV head, `units` units for each of those from key lo on (one even where
+// no key is seen, so that the rows are written).
+struct Work {
+    int rows, tiles, lo, hi, units;
+};
+template <int kKeys>
+__device__ __forceinline__ Work request_work(const AttnArgs& a, const Request& r, int R) {
+    Work w;
+    w.rows = my_rows(a, r);
+    w.tiles = (w.rows + R - 1) / R;
+    w.lo = w.hi = w.units = 0;
+    if (w.rows) {
+        key_range(a, r, 0, r.count - 1, w.lo, w.hi);
+        w.lo = w.lo / kKeys * kKeys;
+        w.units = max(1, (w.hi - w.lo + kKeys - 1) / kKeys);
+    }
+    return w;
+}
 // Cache block of a key, or -1 where the table has none (its keys read as zeros).
 __device__ __forceinline__ int key_block(const AttnArgs& a, int b, int page) {
     if (page >= a.p.table_width) return -1;
@@ -75,6 +104,16 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, int64_t row, int he
         *reinterpret_cast<__half2*>(base + at * 2) = __floats2half2_rn(x, y);
     else
         *reinterpret_cast<__nv_bfloat162*>(base + at * 2) = __floats2bfloat162_rn(x, y);
+}
+__device__ __forceinline__ void store_one(const AttnArgs& a, int64_t row, int head, int col, float x) {
+    char* base = static_cast<char*>(a.p.out) + row * a.p.nb_out;
+    const int64_t at = static_cast<int64_t>(head) * a.kv.head_dim + col;
+    if (a.p.out_type == GGML_TYPE_F32)
+        *reinterpret_cast<float*>(base + at * 4) = x;
+    else if (a.p.out_type == GGML_TYPE_F16)
+        *reinterpret_cast<__half*>(base + at * 2) = __float2half_rn(x);
+    else
+        *reinterpret_cast<__nv_bfloat16*>(base + at * 2) = __float2bfloat16_rn(x);
 }
 
 // 16-bit types: packing, and the pieces whose sum is an F32 value.
@@ -115,6 +154,16 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[NP]
             y -= h.y;
         }
     }
+}
+// F16 pieces reach down to 2^-24 only, so a row of F32 queries is divided by a
+// power of two that leaves its largest value in [1, 2) (BF16 pieces have F32's
+// range).  `big` is a lane's largest value of the row; 4 lanes hold a row.
+template <int NP>
+__device__ __forceinline__ float row_power(float big) {
+    if (NP != 2) return 1.f;
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    return big > 0.f && big <= FLT_MAX ? ldexpf(1.f, min(ilogbf(big), 126)) : 1.f;
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {

@@ -1,0 +1,538 @@
+// Causal attention over a paged KV cache for requests with few rows (decode):
+// every warp streams keys and values of its own.
+//
+// Mathematics as in paged_attention.cu.  With few rows the pass is bound by
+// reading K and V once from HBM, so it is cut along the keys: a request's rows
+// of one KV head (new tokens x group, R = 8 NT at a time) are an item, 16 keys
+// of an item are a unit, and the units of all items, in order, are dealt out as
+// one equal contiguous run to every warp of the GPU (a stream), whatever the
+// lengths.  A warp keeps its own ring of units in shared memory (cp.async), so
+// no warp waits for another one.  An item that ends in another stream than it
+// began in leaves a partial (m, l, o) in the workspace for each stream;
+// combine_kernel joins them in stream order, so results do not depend on timing.
+//
+// The products run transposed, S^T = K q^T and O^T = V^T P^T, with keys (then
+// dimensions of V) as the 16 rows of mma.m16n8k16 and the item's rows as its 8
+// columns: with up to 8 query heads a KV head nothing is multiplied in vain.
+// The running maximum is moved only when a score passes it by 8 (a weight then
+// is at most 2^8), which a vote finds out; moving it takes the shuffles.
+#include <algorithm>
+
+#include "paged_attn.cuh"
+
+namespace xb {
+namespace {
+
+constexpr int kKeys = 16;      // a unit
+constexpr int kMinUnits = 4;   // units per stream below which fewer streams run
+constexpr float kSlack = 8.f;  // log2 of the largest weight
+
+template <int D>
+struct Ring {
+    static constexpr int kWarps = D > 128 ? 4 : 8;
+    static constexpr int kStages = D == 64 ? 5 : D == 96 ? 4 : 3;
+    static constexpr int kStride = D + 8;
+    static constexpr int kHalf = kKeys * kStride;  // elements of K (and of V) in a stage
+    static constexpr size_t kBytes = static_cast<size_t>(kWarps) * kStages * 2 * kHalf * sizeof(uint16_t);
+};
+
+// What a stream that begins an item, but does not end it, leaves for combine_kernel.
+struct alignas(16) Head {
+    int b, kvh, tile;
+    int parts;  // streams the item lies in; 0: none
+};
+
+__host__ __device__ __forceinline__ size_t part_floats(int R, int D) { return static_cast<size_t>(R) * (D + 2); }
+
+struct StreamArgs {
+    AttnArgs a;
+    Head* heads;   // [streams]
+    float* parts;  // [streams][2][R][D] sums, then [R] maxima and [R] l: slot 0 for an item begun elsewhere
+};
+
+// Walks the units of a stream.
+struct Cursor {
+    int b, kvh, tile, unit;
+    Request rq;
+    Work w;
+
+    template <int R>
+    __device__ __forceinline__ void enter(const AttnArgs& a) {
+        rq = read_request(a, b);
+        w = request_work<kKeys>(a, rq, R);
+    }
+    // The next unit (there is one).
+    template <int R>
+    __device__ __forceinline__ void next(const AttnArgs& a) {
+        if (++unit < w.units) return;
+        unit = 0;
+        if (++tile < w.tiles) return;
+        tile = 0;
+        if (++kvh < a.kv.kv_heads) return;
+        kvh = 0;
+        do {
+            ++b;
+            enter<R>(a);
+        } while (!w.rows);
+    }
+};
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <typename T, int D, int NP, int NT>
+__global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(const __grid_constant__ StreamArgs g) {
+    using L = Ring<D>;
+    constexpr int R = 8 * NT, kThreads = L::kWarps * 32, kS = L::kStride, kSteps = D / 16;
+    extern __shared__ __align__(16) uint16_t smem[];
+    __shared__ long long before[kThreads + 1];  // units of the requests before each thread's
+    __shared__ long long warp_units[L::kWarps];
+    const AttnArgs& a = g.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.p.n_seqs;
+    grid_wait();
+
+    // units of all requests, summed up over the threads
+    const int per = (B + kThreads - 1) / kThreads;
+    {
+        long long mine = 0;
+        for (int b = min(tid * per, B); b < min(tid * per + per, B); ++b) {
+            const Work w = request_work<kKeys>(a, read_request(a, b), R);
+            mine += static_cast<long long>(w.units) * w.tiles * a.kv.kv_heads;
+        }
+        long long inc = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += o;
+        }
+        if (lane == 31) warp_units[warp] = inc;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) inc += warp_units[w];
+        before[tid + 1] = inc;
+        if (tid == 0) before[0] = 0;
+        __syncthreads();
+    }
+    const long long all = before[kThreads];
+    const long long most = static_cast<long long>(gridDim.x) * L::kWarps;
+    const long long streams = min(most, max(1LL, all / kMinUnits));
+    // neighbouring streams lie on different SMs: a short run of units uses all of them
+    const long long me = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
+    if (lane == 0) g.heads[me].parts = 0;
+    if (me >= streams || all == 0) return;
+    const long long u0 = all * me / streams, u1 = all * (me + 1) / streams;
+    int left = static_cast<int>(u1 - u0);  // units to fetch
+    int todo = left;                       // units to work off
+
+    // the first unit
+    Cursor at;
+    long long item0;  // units before the item `at` is in
+    {
+        int lo = 0, hi = kThreads;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (before[mid] <= u0) lo = mid; else hi = mid;
+        }
+        long long u = before[lo];
+        at.b = lo * per;
+        at.enter<R>(a);
+        for (;;) {
+            const long long n = static_cast<long long>(at.w.units) * at.w.tiles * a.kv.kv_heads;
+            if (u0 < u + n) break;
+            u += n;
+            ++at.b;
+            at.enter<R>(a);
+        }
+        const long long item = (u0 - u) / at.w.units;
+        at.unit = static_cast<int>(u0 - u - item * at.w.units);
+        at.kvh = static_cast<int>(item / at.w.tiles);
+        at.tile = static_cast<int>(item - static_cast<long long>(at.kvh) * at.w.tiles);
+        item0 = u0 - at.unit;
+    }
+
+    // the ring: `fetch` runs ahead of `at`
+    uint16_t* ring = smem + static_cast<size_t>(warp) * L::kStages * 2 * L::kHalf;
+    Cursor fetch = at;
+    auto block_of = [&](const Cursor& c) {
+        const int j0 = c.w.lo + c.unit * kKeys;
+        return j0 < c.w.hi ? key_block(a, c.b, j0 >> a.log_bs) : -1;
+    };
+    int id = block_of(fetch), fill = 0;
+    auto load = [&]() {
+        if (left > 0) {
+            const int j0 = fetch.w.lo + fetch.unit * kKeys;
+            const int n = id < 0 ? 0 : fetch.w.hi - j0;  // keys of the unit that exist
+            const int64_t base = id < 0 ? 0
+                                        : id * a.kv.nb_block + fetch.kvh * a.kv.nb_head +
+                                              (j0 & (a.kv.block_size - 1)) * a.kv.nb_token;
+            uint16_t* to = ring + fill * 2 * L::kHalf;
+            constexpr int kChunks = D / 8;
+#pragma unroll
+            for (int i = 0; i < kKeys * kChunks / 32; ++i) {
+                const int x = i * 32 + lane, r = x / kChunks, c = x - r * kChunks;
+                const int bytes = r < n ? 16 : 0;  // 0: fills with zeros
+                const int64_t from = r < n ? base + r * a.kv.nb_token + c * 16 : 0;
+                const uint32_t d = smem_addr(to + r * kS + c * 8);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d),
+                             "l"(static_cast<const char*>(a.kv.k) + from), "r"(bytes)
+                             : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + L::kHalf * 2),
+                             "l"(static_cast<const char*>(a.kv.v) + from), "r"(bytes)
+                             : "memory");
+            }
+            if (--left > 0) {
+                fetch.next<R>(a);
+                id = block_of(fetch);
+            }
+            fill = fill + 1 == L::kStages ? 0 : fill + 1;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < L::kStages - 1; ++i) load();
+
+    uint32_t qf[NP][NT][kSteps][2];
+    float o[NT][kSteps][4], m[NT][2], l[NT][2], mul[NT][2], slope[NT][2];
+    int pos[NT][2];
+    int rows = 0, all_lo = 0, all_hi = 0;  // keys [all_lo, all_hi) are seen by every row
+
+    int stage = 0;
+    bool fresh = true, begun_here = at.unit == 0;
+    while (todo > 0) {
+        if (fresh) {  // a new item: its queries, and nothing seen yet
+            fresh = false;
+            const int G = a.group, r0 = at.tile * R;
+            rows = min(R, at.w.rows - r0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int r = nt * 8 + (lane >> 2);
+                const bool on = r < rows;
+                const int i = (r0 + r) / G, h = at.kvh * G + (r0 + r) - i * G;
+                const char* src = static_cast<const char*>(a.p.q) + (at.rq.first + (on ? i : 0)) * a.p.nb_q;
+                float up = 1.f;
+                if constexpr (NP == 1) {
+                    const uint32_t* s = reinterpret_cast<const uint32_t*>(src) + static_cast<int64_t>(h) * (D / 2) + (lane & 3);
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) {
+                        qf[0][nt][k][0] = on ? __ldg(s + k * 8) : 0u;
+                        qf[0][nt][k][1] = on ? __ldg(s + k * 8 + 4) : 0u;
+                    }
+                } else {
+                    const float2* s = reinterpret_cast<const float2*>(src) + static_cast<int64_t>(h) * (D / 2) + (lane & 3);
+                    float2 x[kSteps][2];
+                    float big = 0.f;
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            x[k][e] = on ? __ldg(s + k * 8 + e * 4) : make_float2(0.f, 0.f);
+                            big = fmaxf(big, fmaxf(fabsf(x[k][e].x), fabsf(x[k][e].y)));
+                        }
+                    up = row_power<NP>(big);
+                    const float down = 1.f / up;
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t piece[NP];
+                            split_pair<T, NP>(x[k][e].x * down, x[k][e].y * down, piece);
+#pragma unroll
+                            for (int c = 0; c < NP; ++c) qf[c][nt][k][e] = piece[c];
+                        }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {  // this lane's columns of S^T
+                    const int col = 2 * (lane & 3) + e, rr = r0 + nt * 8 + col, it = rr / G;
+                    mul[nt][e] = a.pre * __shfl_sync(0xffffffffu, up, col * 4);
+                    slope[nt][e] = head_slope(a, at.kvh * G + rr - it * G);
+                    pos[nt][e] = at.rq.pos0() + it;
+                    m[nt][e] = -INFINITY;
+                    l[nt][e] = 0.f;
+                }
+#pragma unroll
+                for (int n = 0; n < kSteps; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][n][e] = 0.f;
+            }
+            const int p0 = at.rq.pos0() + r0 / G, p1 = at.rq.pos0() + (r0 + rows - 1) / G;
+            all_hi = min(p0 + 1, at.w.hi);
+            all_lo = a.p.window > 0 && p1 >= a.p.window ? p1 - a.p.window + 1 : 0;
+        }
+        load();
+        asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 1) : "memory");
+        __syncwarp();
+        const uint16_t* kt = ring + stage * 2 * L::kHalf;
+        const uint16_t* vt = kt + L::kHalf;
+
+        // scores: two chains of matrix instructions, joined by an addition
+        float s[NT][2][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[nt][0][e] = s[nt][1][e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            uint32_t kf[4];
+            ldsm4(kf, smem_addr(kt + (lane & 15) * kS + k * 16 + (lane >> 4) * 8));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = NP - 1; c >= 0; --c) mma16816<T>(s[nt][k & 1], kf, qf[c][nt][k][0], qf[c][nt][k][1]);
+        }
+        const int j0 = at.w.lo + at.unit * kKeys;
+        const bool whole = j0 >= all_lo && j0 + kKeys <= all_hi;
+        bool higher = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int q = e & 1, j = j0 + (lane >> 2) + 8 * (e >> 1);
+                float x = (s[nt][0][e] + s[nt][1][e]) * mul[nt][q];
+                if (a.post != 0.f) x = a.post * tanhf(x);
+                if (a.bias_near) x = fmaf(slope[nt][q], static_cast<float>(j - pos[nt][q]), x);
+                if (!whole && (j > min(pos[nt][q], at.w.hi - 1) || (a.p.window > 0 && pos[nt][q] - j >= a.p.window)))
+                    x = -INFINITY;
+                s[nt][0][e] = x;
+                higher |= x > m[nt][q] + kSlack;
+            }
+        if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    float top = fmaxf(s[nt][0][q], s[nt][0][2 + q]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    top = fmaxf(top, m[nt][q]);
+                    const float c = top == -INFINITY ? 1.f : exp2f(m[nt][q] - top);
+                    m[nt][q] = top;
+                    l[nt][q] *= c;
+#pragma unroll
+                    for (int n = 0; n < kSteps; ++n) o[nt][n][q] *= c, o[nt][n][2 + q] *= c;
+                }
+        }
+        uint32_t pf[NP][NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float base = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
+                s[nt][0][e] = exp2f(s[nt][0][e] - base);
+                l[nt][e & 1] += s[nt][0][e];
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {  // keys 0-7, then 8-15
+                uint32_t piece[NP];
+                split_pair<T, NP>(s[nt][0][2 * e], s[nt][0][2 * e + 1], piece);
+#pragma unroll
+                for (int c = 0; c < NP; ++c) pf[c][nt][e] = transpose8x8(piece[c]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kSteps; ++n) {
+            uint32_t vf[4];
+            ldsm4_t(vf, smem_addr(vt + ((lane & 7) + ((lane >> 4) & 1) * 8) * kS + n * 16 + ((lane >> 3) & 1) * 8));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if (NP == 1) {
+                    mma16816<T>(o[nt][n], vf, pf[0][nt][0], pf[0][nt][1]);
+                } else {
+                    // the matrix unit cuts its sums off: every unit's sum starts at 0 and
+                    // is added by a rounded addition, or a long axis would show it
+                    float t[4] = {};
+#pragma unroll
+                    for (int c = NP - 1; c >= 0; --c) mma16816<T>(t, vf, pf[c][nt][0], pf[c][nt][1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][n][e] += t[e];
+                }
+            }
+        }
+        __syncwarp();  // every lane has read the stage
+        stage = stage + 1 == L::kStages ? 0 : stage + 1;
+        --todo;
+        const bool ends = at.unit + 1 == at.w.units;
+        if (!ends && todo > 0) {
+            ++at.unit;
+            continue;
+        }
+
+        // the item ends here, or goes on in the next stream
+        const bool whole_item = ends && begun_here;
+        const int part = begun_here ? 1 : 0;
+        float* to = g.parts + (static_cast<size_t>(me) * 2 + part) * part_floats(R, D);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float sum = l[nt][q];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int r = nt * 8 + 2 * (lane & 3) + q;
+                if (r >= rows) continue;
+                if (whole_item) {
+                    const int rr = at.tile * R + r, i = rr / a.group, h = at.kvh * a.group + rr - i * a.group;
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                    for (int n = 0; n < kSteps; ++n) {
+                        store_one(a, at.rq.first + i, h, n * 16 + (lane >> 2), sum == 0.f ? 0.f : o[nt][n][q] * inv);
+                        store_one(a, at.rq.first + i, h, n * 16 + 8 + (lane >> 2),
+                                  sum == 0.f ? 0.f : o[nt][n][2 + q] * inv);
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < kSteps; ++n) {
+                        to[r * D + n * 16 + (lane >> 2)] = o[nt][n][q];
+                        to[r * D + n * 16 + 8 + (lane >> 2)] = o[nt][n][2 + q];
+                    }
+                    if ((lane >> 2) == 0) {
+                        to[R * D + r] = m[nt][q];
+                        to[R * D + R + r] = sum;
+                    }
+                }
+            }
+        if (begun_here && !ends && lane == 0) {
+            // the stream that holds the item's last unit u is the largest with all * w / streams <= u
+            const long long u = item0 + at.w.units - 1;
+            const long long w1 = ((u + 1) * streams - 1) / all;
+            g.heads[me] = Head{at.b, at.kvh, at.tile, static_cast<int>(w1 - me + 1)};
+        }
+        if (todo > 0) {
+            item0 += at.w.units;
+            at.next<R>(a);
+            fresh = begun_here = true;
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Joins the partials of the item that stream blockIdx.x began: a warp per row,
+// parts in stream order.
+template <int D, int R>
+__global__ void __launch_bounds__(R < 8 ? 32 * R : 256) combine_kernel(const __grid_constant__ StreamArgs g) {
+    grid_wait();
+    const AttnArgs& a = g.a;
+    const Head head = g.heads[blockIdx.x];
+    if (!head.parts) return;
+    const Request rq = read_request(a, head.b);
+    const int rows = min(R, rq.count * a.group - head.tile * R), lane = threadIdx.x & 31;
+    const size_t slot = part_floats(R, D);
+    for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5) {
+        // lane p holds part p, p + 32, ...: the row's largest maximum, then its parts' weights
+        auto part = [&](int p) { return g.parts + (2 * (static_cast<size_t>(blockIdx.x) + p) + (p == 0)) * slot; };
+        float top = -INFINITY;
+        for (int p = lane; p < head.parts; p += 32) top = fmaxf(top, part(p)[R * D + r]);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, o[D / 32] = {};
+        for (int p0 = 0; p0 < head.parts; p0 += 32) {
+            float w = 0.f;
+            if (p0 + lane < head.parts) {
+                const float* x = part(p0 + lane);
+                w = exp2f(x[R * D + r] - base);
+                sum += w * x[R * D + R + r];
+            }
+            const int n = min(32, head.parts - p0);
+#pragma unroll 4
+            for (int p = 0; p < n; ++p) {
+                const float c = __shfl_sync(0xffffffffu, w, p);
+                const float* x = part(p0 + p) + r * D + lane * 2;
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) {
+                    const float2 v = *reinterpret_cast<const float2*>(x + i * 64);
+                    o[2 * i] = fmaf(c, v.x, o[2 * i]);
+                    o[2 * i + 1] = fmaf(c, v.y, o[2 * i + 1]);
+                }
+                if (D % 64) o[D / 32 - 1] = fmaf(c, part(p0 + p)[r * D + D / 64 * 64 + lane], o[D / 32 - 1]);
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int rr = head.tile * R + r, i = rr / a.group, h = head.kvh * a.group + rr - i * a.group;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k)
+            store_out(a, rq.first + i, h, k * 64 + lane * 2, sum == 0.f ? 0.f : o[2 * k] * inv,
+                      sum == 0.f ? 0.f : o[2 * k + 1] * inv);
+        if (D % 64)
+            store_one(a, rq.first + i, h, D / 64 * 64 + lane, sum == 0.f ? 0.f : o[D / 32 - 1] * inv);
+    }
+}
+
+template <int D>
+size_t workspace_of(int R) {
+    const size_t streams = static_cast<size_t>(sm_count()) * Ring<D>::kWarps;
+    return streams * (sizeof(Head) + 2 * part_floats(R, D) * sizeof(float));
+}
+
+template <typename T, int D, int NP, int NT>
+cudaError_t launch_rows(const AttnArgs& a, cudaStream_t stream) {
+    using L = Ring<D>;
+    const auto kernel = attn_stream_kernel<T, D, NP, NT>;
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L::kBytes));
+    if (e != cudaSuccess) return e;
+    const unsigned sms = static_cast<unsigned>(sm_count());
+    StreamArgs g{a, nullptr, nullptr};
+    g.heads = static_cast<Head*>(a.p.workspace);
+    g.parts = reinterpret_cast<float*>(g.heads + static_cast<size_t>(sms) * L::kWarps);
+    const cudaError_t f = launch_pdl(kernel, dim3(sms), dim3(L::kWarps * 32), L::kBytes, stream, 1, g);
+    if (f != cudaSuccess) return f;
+    return launch_pdl(combine_kernel<D, 8 * NT>, dim3(sms * L::kWarps), dim3(256), 0, stream, 1, g);
+}
+
+// Rows of an item: as few 8-column blocks as the hints ask for, as many as the
+// registers hold beside q's NP pieces and o (255 a thread; more would spill).
+constexpr int most_blocks(int D, bool f32) { return D > 128 ? 1 : f32 || D > 96 ? 2 : 4; }
+int row_blocks(const AttnArgs& a) {
+    const int64_t rows = static_cast<int64_t>(a.p.max_new) * a.group;
+    const int want = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    return std::min(want, most_blocks(a.kv.head_dim, a.p.q_type == GGML_TYPE_F32));
+}
+
+template <typename T, int D, int NP, int kMost>
+cudaError_t launch_blocks(const AttnArgs& a, cudaStream_t stream) {
+    const int n = row_blocks(a);
+    if constexpr (kMost >= 4)
+        if (n == 4) return launch_rows<T, D, NP, 4>(a, stream);
+    if constexpr (kMost >= 2)
+        if (n == 2) return launch_rows<T, D, NP, 2>(a, stream);
+    return launch_rows<T, D, NP, 1>(a, stream);
+}
+template <typename T, int D>
+cudaError_t launch_pieces(const AttnArgs& a, cudaStream_t stream) {
+    if (a.p.q_type == GGML_TYPE_F32)
+        return launch_blocks<T, D, Half16<T>::kPieces, most_blocks(D, true)>(a, stream);
+    return launch_blocks<T, D, 1, most_blocks(D, false)>(a, stream);
+}
+template <typename T>
+cudaError_t launch_type(const AttnArgs& a, cudaStream_t stream) {
+    switch (a.kv.head_dim) {
+        case 64: return launch_pieces<T, 64>(a, stream);
+        case 96: return launch_pieces<T, 96>(a, stream);
+        case 128: return launch_pieces<T, 128>(a, stream);
+        default: return launch_pieces<T, 256>(a, stream);
+    }
+}
+
+}  // namespace
+
+size_t stream_workspace(const AttnArgs& a) {
+    const int R = 8 * row_blocks(a);
+    switch (a.kv.head_dim) {
+        case 64: return workspace_of<64>(R);
+        case 96: return workspace_of<96>(R);
+        case 128: return workspace_of<128>(R);
+        default: return workspace_of<256>(R);
+    }
+}
+
+cudaError_t stream_launch(const AttnArgs& a, cudaStream_t stream) {
+    return a.kv.type == GGML_TYPE_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream);
+}
+
+}  // namespace xb
