@@ -248,7 +248,7 @@ int ggml_backend_xdna_shard_rows(int64_t n, int world, int rank, int64_t *row0, 
  *
  * Calls return 0, -1 for a refused argument (nothing is launched), or another
  * negative code for a CUDA error.  They allocate nothing, keep nothing from one call to the
- * next, never synchronise, and may be captured into CUDA graphs.  Lengths,
+ * next, never synchronise (b200_paged_attention_error does), and may be captured into CUDA graphs.  Lengths,
  * tables and slots are read on the device, so a captured call serves other
  * lengths on replay.  What the device data may hold is bounded there: a block
  * id outside [0, num_blocks) is never dereferenced (its keys and values read as
@@ -371,6 +371,10 @@ struct b200_paged_attention_args {
  * types and hints, not on device data. */
 size_t b200_paged_attention_workspace(const struct b200_paged_attention_args *p, const struct b200_kv_cache *kv);
 int b200_paged_attention(const struct b200_paged_attention_args *p, const struct b200_kv_cache *kv, void *stream);
+/* Status of the attention kernels' bounded waits on the current CUDA device:
+ * *status = 1 if a wait inside a kernel ran out (2 s) since the last call, whose
+ * output is then not valid, else 0; the word is cleared.  Synchronises. */
+int b200_paged_attention_error(int *status);
 
 #ifdef __cplusplus
 }

@@ -14,6 +14,14 @@ pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out(cuda, G):
+    yield
+    status = C.c_int(-1)
+    G.check(G.lib().b200_paged_attention_error(C.byref(status)), "paged_attention_error")
+    assert status.value == 0
+
+
 def gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 

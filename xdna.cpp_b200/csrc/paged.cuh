@@ -18,6 +18,9 @@ cudaError_t qk_norm_rope_launch(const struct b200_qk_norm_rope_args& p, const st
 size_t paged_attention_workspace(const struct b200_paged_attention_args& p, const struct b200_kv_cache& kv);
 cudaError_t paged_attention_launch(const struct b200_paged_attention_args& p, const struct b200_kv_cache& kv,
                                    cudaStream_t stream);
+// Reads and clears the current device's error word of the attention kernels'
+// bounded waits.
+cudaError_t paged_error_status(int* out);
 
 // Launch with programmatic stream serialization: the kernel may start while
 // the one before it on the stream drains.  Every thread of every kernel

@@ -182,4 +182,12 @@ int b200_paged_attention(const struct b200_paged_attention_args* p, const struct
     return done(paged_attention_launch(q, c, static_cast<cudaStream_t>(stream)), "b200_paged_attention");
 }
 
+int b200_paged_attention_error(int* status) {
+    if (!status) {
+        set_error("b200_paged_attention_error: null status pointer");
+        return -1;
+    }
+    return done(paged_error_status(status), "b200_paged_attention_error");
+}
+
 }  // extern "C"

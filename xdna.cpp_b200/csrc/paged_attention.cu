@@ -13,6 +13,7 @@
 // by 16 bytes (an odd number of 16-byte columns: ldmatrix reads 8 rows without
 // a bank conflict).  F32 queries run as NP 16-bit pieces of q and of the
 // softmax weights, whose products with the exact 16-bit K and V add up in F32.
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 
@@ -284,8 +285,7 @@ cudaError_t launch_tile(const AttnArgs& a, cudaStream_t stream) {
 }
 template <typename T, int D>
 cudaError_t launch_pieces(const AttnArgs& a, cudaStream_t stream) {
-    return a.p.q_type == GGML_TYPE_F32 ? launch_tile<T, D, Half16<T>::kPieces>(a, stream)
-                                       : launch_tile<T, D, 1>(a, stream);
+    return launch_tile<T, D, Half16<T>::kPieces>(a, stream);
 }
 template <typename T>
 cudaError_t launch_type(const AttnArgs& a, cudaStream_t stream) {
@@ -327,21 +327,24 @@ int sm_count() {
 }
 
 // Requests of up to kStreamRows rows go to the stream kernel, the others to the
-// tile kernel; where the hints (or a single request) leave no doubt, one kernel
-// takes everything.
+// chunk kernel (16-bit queries) or the tile kernel (F32); where the hints (or a
+// single request) leave no doubt, one kernel takes everything.  The kernels run
+// one after the other and share the workspace.
 namespace {
 struct Split {
-    bool stream, tile;
+    bool stream, chunk, tile;
 };
 Split split(const AttnArgs& a) {
     const bool few = static_cast<int64_t>(a.p.max_new) * a.group <= kStreamRows;
-    return Split{few || a.p.n_seqs > 1, !few};
+    const bool f32 = a.p.q_type == GGML_TYPE_F32;
+    return Split{few || a.p.n_seqs > 1, !few && !f32, !few && f32};
 }
 }  // namespace
 
 size_t paged_attention_workspace(const struct b200_paged_attention_args& p, const struct b200_kv_cache& kv) {
     const AttnArgs a = make_args(p, kv);
-    return split(a).stream ? stream_workspace(a) : 0;
+    const Split s = split(a);
+    return std::max(s.stream ? stream_workspace(a) : 0, s.chunk ? chunk_workspace(a) : 0);
 }
 
 cudaError_t paged_attention_launch(const struct b200_paged_attention_args& p, const struct b200_kv_cache& kv,
@@ -349,13 +352,13 @@ cudaError_t paged_attention_launch(const struct b200_paged_attention_args& p, co
     AttnArgs a = make_args(p, kv);
     const Split s = split(a);
     if (s.stream) {
-        if (s.tile) a.max_rows = kStreamRows;
+        if (s.chunk || s.tile) a.max_rows = kStreamRows;
         const cudaError_t e = stream_launch(a, stream);
-        if (e != cudaSuccess) return e;
+        if (e != cudaSuccess || !(s.chunk || s.tile)) return e;
+        a.min_rows = kStreamRows;
+        a.max_rows = 0x7fffffff;
     }
-    if (!s.tile) return cudaSuccess;
-    a.min_rows = s.stream ? kStreamRows : 0;
-    a.max_rows = 0x7fffffff;
+    if (s.chunk) return chunk_launch(a, stream);
     return kv.type == GGML_TYPE_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream);
 }
 

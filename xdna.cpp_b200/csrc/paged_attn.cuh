@@ -35,6 +35,10 @@ constexpr int kStreamRows = 32;
 size_t stream_workspace(const AttnArgs& a);
 cudaError_t stream_launch(const AttnArgs& a, cudaStream_t stream);
 
+// The chunk kernel (paged_chunk.cu), for 16-bit queries: its workspace and launch.
+size_t chunk_workspace(const AttnArgs& a);
+cudaError_t chunk_launch(const AttnArgs& a, cudaStream_t stream);
+
 #ifdef __CUDACC__
 // Slope of a query head, times log2(e).
 __device__ __forceinline__ float head_slope(const AttnArgs& a, int h) {

@@ -1,0 +1,768 @@
+// Causal attention of many new tokens over a paged KV cache on the
+// fifth-generation tensor cores.
+//
+// Mathematics as in paged_attention.cu: per row a running maximum m, l = sum
+// 2^(s - m) and o = sum 2^(s - m) v, in one pass over tiles of 128 keys.
+//
+// A CTA works on an item of up to 2 x 128 rows (query tile q: rows 128 q ..) of
+// one request and KV head.  Per tile of keys: S = Q K^T into TMEM, weights
+// P = 2^(s - m) back into TMEM over S in 16 bits, O += P V in TMEM.  Roles:
+//   4 warps per query tile   one row per thread: softmax, rescaling and output
+//   one warp                 issues the matrix instructions
+//   one warp                 TMA loads of K and V, page by page, into a ring
+// While one query tile is in its softmax the matrix unit works on the other
+// one.  O is rescaled only when a row's maximum grows by more than 8 (weights
+// stay below 2^8), which a vote of the warp finds out.  The weights are rounded
+// to 16 bits (the cache's type) because the matrix unit takes both factors in
+// one type; scores, sums and O are F32.
+//
+// The work of all items, counted in key tiles, is dealt out in equal contiguous
+// runs to one CTA per SM; items that end up cut are joined by combine_kernel.
+//
+// K is held as the K-major, V as the MN-major operand in 128-byte swizzled rows:
+// the layout a TMA box of 64 values by 16..128 tokens has in shared memory.  D is
+// cut into halves of 64 values; a box past head_dim (96) or in a block outside
+// the cache reads as zeros.  Rows of V behind the last key are zeroed before
+// they are used, since a weight of 0 would not hide a NaN there.
+//
+// Every wait is bounded (2 s of %globaltimer): one that runs out sets the error
+// word, all roles give up, copies and matrix instructions in flight are waited
+// for (bounded again), and TMEM is freed.
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "paged_split.cuh"
+
+namespace xb {
+namespace {
+
+constexpr int kKeys = 128;
+constexpr int kMinTiles = 2;   // key tiles per CTA below which fewer CTAs run
+constexpr float kSlack = 8.f;  // log2 of the largest weight
+constexpr unsigned long long kWaitNs = 2000000000ull;
+
+__device__ int g_chunk_error;
+
+template <int D>
+struct Shape {
+    static constexpr int kQ = D > 128 ? 1 : 2;  // query tiles
+    static constexpr int kRows = 128 * kQ;
+    static constexpr int kHalves = (D + 63) / 64;
+    static constexpr int kStages = D == 64 ? 4 : D <= 128 ? 2 : 1;
+    static constexpr int kTile = kHalves * 128 * 128;  // bytes of 128 rows
+    // 12 warps: the last two only make up the fourth group of registers, so that
+    // the softmax warps can take registers from the others
+    static constexpr int kThreads = kQ == 2 ? 384 : 192;
+    static constexpr int kLaunchRegs = 168, kSoftmaxRegs = 224, kOtherRegs = 56;
+    static_assert(kQ == 1 || 256 * kSoftmaxRegs + 128 * kOtherRegs <= 384 * kLaunchRegs, "registers of the launch");
+    static constexpr int kSmem = (kQ + 2 * kStages) * kTile + 1024;  // 1024: alignment
+    static constexpr int kS = 0, kO = 256, kPitch = 128;             // TMEM columns of q's S and O: + 128 q
+};
+
+struct ChunkArgs {
+    SplitArgs g;
+    CUtensorMap k, v;
+    int box_tokens;  // tokens per TMA box: a block, or a tile of one
+};
+
+// ------------------------------------------------------------------- barriers
+struct Bars {
+    uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
+    uint64_t qfull[2], sfull[2], pfull[2], ofull[2], drain;
+};
+
+__device__ __forceinline__ void bar_init(uint64_t* b, int count) {
+    asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_addr(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+// Waits for the phase; false when 2 s have passed or another wait has given up.
+__device__ __forceinline__ bool bar_wait_slow(uint64_t* b, uint32_t parity, volatile int* dead) {
+    const unsigned long long t0 = now_ns();
+    for (;;) {
+        for (int i = 0; i < 64; ++i)
+            if (bar_try(b, parity)) return true;
+        if (dead && *dead) return false;
+        if (now_ns() - t0 > kWaitNs) {
+            if (dead) *dead = 1;
+            atomicExch(&g_chunk_error, 1);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* dead) {
+    bool ok = bar_try(b, parity) || bar_try(b, parity) || bar_wait_slow(b, parity, dead);
+    return __all_sync(0xffffffffu, ok);  // the warp goes on, or gives up, as one
+}
+
+// ------------------------------------------------------------ matrix unit, TMEM
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(b))
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+        : "memory");
+}
+// Shared-memory operand in rows of 128 swizzled bytes, groups of 8 rows 1024
+// bytes apart.  K-major (Q, K): `lead` unused.  MN-major (V): `lead` bytes
+// between 64-value groups.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3fff) | static_cast<uint64_t>((lead >> 4) & 0x3fff) << 16 |
+           static_cast<uint64_t>(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// kind::f16 instruction descriptor: F32 sums, 128 x n, both factors of `T`.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_mn_major) {
+    const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return 1u << 4 | type << 7 | type << 10 | (b_mn_major ? 1u << 16 : 0u) | static_cast<uint32_t>(n / 8) << 17 |
+           (128u / 16) << 24;
+}
+
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_ld32(uint32_t addr, float* r) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tm_ld16(uint32_t addr, float* r) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* u) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+        "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+        : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                        int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
+// ------------------------------------------------------------------ the work list
+// Key tiles [t0, t1) of row tile `tile`, and of one of its query tiles.
+template <int R>
+__device__ __forceinline__ void item_tiles(const AttnArgs& a, const Request& rq, int rows, int tile, int& t0, int& t1,
+                                           int& hi) {
+    int lo;
+    key_range(a, rq, tile * R / a.group, (min(tile * R + R, rows) - 1) / a.group, lo, hi);
+    t0 = lo / kKeys;
+    t1 = max(t0 + 1, (hi + kKeys - 1) / kKeys);
+}
+template <int R>
+__device__ __forceinline__ int item_units(const AttnArgs& a, const Request& rq, int rows, int tile) {
+    int t0, t1, hi;
+    item_tiles<R>(a, rq, rows, tile, t0, t1, hi);
+    return t1 - t0;
+}
+__device__ __forceinline__ long long warp_sum(long long v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+// Units of all row tiles of one request (the same one on every lane), for one KV head.
+template <int R>
+__device__ __forceinline__ long long request_units(const AttnArgs& a, const Request& rq, int rows) {
+    const int lane = threadIdx.x & 31, tiles = (rows + R - 1) / R;
+    long long n = 0;
+    for (int t = lane; t < tiles; t += 32) n += item_units<R>(a, rq, rows, t);
+    return warp_sum(n);
+}
+
+// Walks the items of a CTA's run; all lanes of a warp hold the same values.
+struct Walk {
+    int b, kvh, tile;
+    Request rq;
+    int rows, tiles;
+    int t0, t1, hi;   // the item's key tiles, and the end of its keys
+    int s0, s1;       // those of this run
+    long long left;   // units of the run from s0 on
+
+    template <int R>
+    __device__ __forceinline__ void enter_request(const AttnArgs& a) {
+        rq = read_request(a, b);
+        rows = my_rows(a, rq);
+        tiles = (rows + R - 1) / R;
+    }
+    template <int R>
+    __device__ __forceinline__ void enter_item(const AttnArgs& a, int skip) {
+        item_tiles<R>(a, rq, rows, tile, t0, t1, hi);
+        s0 = t0 + skip;
+        s1 = static_cast<int>(min(static_cast<long long>(t1), s0 + left));
+    }
+    // The next item of the run; false at its end.
+    template <int R>
+    __device__ __forceinline__ bool next(const AttnArgs& a) {
+        left -= s1 - s0;
+        if (left <= 0) return false;
+        if (++tile == tiles) {
+            tile = 0;
+            if (++kvh == a.kv.kv_heads) {
+                kvh = 0;
+                do {
+                    ++b;
+                    enter_request<R>(a);
+                } while (!rows);
+            }
+        }
+        enter_item<R>(a, 0);
+        return true;
+    }
+};
+
+// The key tiles of query tile q that fall into [s0, s1): [lo, hi), empty when lo == hi.
+__device__ __forceinline__ void query_tiles(const AttnArgs& a, const Walk& w, int r0, int& lo, int& hi) {
+    lo = hi = 0;
+    if (r0 >= w.rows) return;
+    int k0, k1;
+    key_range(a, w.rq, r0 / a.group, (min(r0 + 128, w.rows) - 1) / a.group, k0, k1);
+    lo = max(w.s0, k0 / kKeys);
+    hi = max(lo, min(w.s1, (k1 + kKeys - 1) / kKeys));
+}
+
+// kGeneral: a cap, a bias or a scale that is not positive; else the scale is
+// folded into the exponential.
+template <typename T, int D, bool kGeneral>
+__global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const __grid_constant__ ChunkArgs c) {
+    using L = Shape<D>;
+    constexpr int R = L::kRows;
+    extern __shared__ uint8_t raw[];
+    __shared__ Bars bars;
+    __shared__ long long before[L::kThreads + 1];
+    __shared__ long long warp_units[L::kThreads / 32];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int dead_word;
+    volatile int* dead = &dead_word;
+    const AttnArgs& a = c.g.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.p.n_seqs;
+    constexpr int kMmaWarp = L::kQ * 4, kLoadWarp = kMmaWarp + 1;
+    const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+    const uint32_t qs = base, ks = qs + L::kQ * L::kTile, vs = ks + L::kStages * L::kTile;
+
+    if (tid == 0) {
+        for (int i = 0; i < 4; ++i) {
+            bar_init(&bars.kfull[i], 1);
+            bar_init(&bars.kempty[i], 1);
+            bar_init(&bars.vfull[i], 1);
+            bar_init(&bars.vempty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&bars.qfull[i], 128);
+            bar_init(&bars.sfull[i], 1);
+            bar_init(&bars.pfull[i], 128);
+            bar_init(&bars.ofull[i], 1);
+        }
+        bar_init(&bars.drain, 1);
+        dead_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    grid_wait();
+
+    // units of all requests, summed up over the threads
+    const int per = (B + L::kThreads - 1) / L::kThreads;
+    {
+        long long mine = 0;
+        for (int i = 0; i < per; ++i) {
+            const int b = tid * per + i;
+            Request rq{0, 0, 0};
+            int rows = 0;
+            if (b < B) {
+                rq = read_request(a, b);
+                rows = my_rows(a, rq);
+            }
+            const int tiles = (rows + R - 1) / R;
+            long long n = 0;
+            if (tiles <= 4)
+                for (int t = 0; t < tiles; ++t) n += item_units<R>(a, rq, rows, t);
+            for (unsigned big = __ballot_sync(0xffffffffu, tiles > 4); big; big &= big - 1) {
+                const int from = __ffs(big) - 1;  // a long request: its row tiles over all lanes
+                Request r{__shfl_sync(0xffffffffu, rq.first, from), __shfl_sync(0xffffffffu, rq.count, from),
+                          __shfl_sync(0xffffffffu, rq.kv, from)};
+                const long long s = request_units<R>(a, r, __shfl_sync(0xffffffffu, rows, from));
+                if (lane == from) n = s;
+            }
+            mine += n * a.kv.kv_heads;
+        }
+        long long inc = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += o;
+        }
+        if (lane == 31) warp_units[warp] = inc;
+        tc_before();
+        __syncthreads();
+        tc_after();
+        for (int w = 0; w < warp; ++w) inc += warp_units[w];
+        before[tid + 1] = inc;
+        if (tid == 0) before[0] = 0;
+        __syncthreads();
+    }
+    const uint32_t tmem = tmem_slot;
+    const long long all = before[L::kThreads];
+    const long long streams = min(static_cast<long long>(gridDim.x), max(1LL, all / kMinTiles));
+    const long long me = blockIdx.x;
+    if (tid == 0) c.g.heads[me].parts = 0;
+    const bool working = me < streams && all > 0;
+
+    if (working) {
+        // the first item of the run
+        const long long u0 = all * me / streams, u1 = all * (me + 1) / streams;
+        Walk w;
+        long long item0;  // units before the first item
+        {
+            int lo = 0, hi = L::kThreads;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (before[mid] <= u0) lo = mid; else hi = mid;
+            }
+            long long u = before[lo], one = 0;
+            for (w.b = lo * per;; ++w.b) {
+                w.enter_request<R>(a);
+                one = request_units<R>(a, w.rq, w.rows);
+                if (u0 < u + one * a.kv.kv_heads) break;
+                u += one * a.kv.kv_heads;
+            }
+            w.kvh = static_cast<int>((u0 - u) / one);
+            u += one * w.kvh;
+            for (w.tile = 0;; w.tile += 32) {  // 32 row tiles at a time
+                const int t = w.tile + lane;
+                const long long n = t < w.tiles ? item_units<R>(a, w.rq, w.rows, t) : 0;
+                long long inc = n;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+                    if (lane >= d) inc += o;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, u0 < u + inc);
+                if (hit) {
+                    const int at = __ffs(hit) - 1;
+                    u += __shfl_sync(0xffffffffu, inc - n, at);
+                    w.tile += at;
+                    break;
+                }
+                u += __shfl_sync(0xffffffffu, inc, 31);
+            }
+            item0 = u;
+            w.left = u1 - u0;
+            w.enter_item<R>(a, static_cast<int>(u0 - u));
+        }
+
+        if (warp >= kMmaWarp) {
+        if constexpr (L::kQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegs));
+        if (warp == kLoadWarp) {
+            // ---------------------------------------------------------------- loads
+            const int boxes = kKeys / c.box_tokens;  // per half; lane i issues box i
+            int n = 0;                               // tiles so far
+            bool ok = true;
+            do {
+                for (int t = w.s0; t < w.s1 && ok; ++t, ++n) {
+                    const int stage = n % L::kStages, j = t * kKeys + lane * c.box_tokens;
+                    const bool on = lane < boxes && j < w.hi;
+                    const int id = on ? key_block(a, w.b, j >> a.log_bs) : 0;
+                    const int block = id < 0 ? static_cast<int>(a.kv.num_blocks) : id;  // behind the last: zeros
+                    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, on)) * L::kHalves * c.box_tokens * 128;
+                    const uint32_t parity = ((n / L::kStages) & 1) ^ 1;
+#pragma unroll
+                    for (int kv = 0; kv < 2 && ok; ++kv) {
+                        uint64_t* full = kv ? &bars.vfull[stage] : &bars.kfull[stage];
+                        if (n >= L::kStages) ok = bar_wait(kv ? &bars.vempty[stage] : &bars.kempty[stage], parity, dead);
+                        if (!ok) break;
+                        if (lane == 0) bar_expect(full, bytes);
+                        __syncwarp();
+                        if (on)
+#pragma unroll
+                            for (int h = 0; h < L::kHalves; ++h)
+                                tma_box((kv ? vs : ks) + stage * L::kTile + h * 128 * 128 + lane * c.box_tokens * 128,
+                                        kv ? &c.v : &c.k, full, h * 64, j & (a.kv.block_size - 1), w.kvh, block);
+                    }
+                }
+            } while (ok && w.next<R>(a));
+            if (!ok) {  // copies in flight land before the CTA ends
+                for (int i = max(0, n - L::kStages); i <= n; ++i) {
+                    bar_wait(&bars.kfull[i % L::kStages], (i / L::kStages) & 1, nullptr);
+                    bar_wait(&bars.vfull[i % L::kStages], (i / L::kStages) & 1, nullptr);
+                }
+            }
+        } else if (warp == kMmaWarp) {
+            // ----------------------------------------------------- matrix instructions
+            constexpr uint32_t kIdescS = instruction<T>(kKeys, false), kIdescO = instruction<T>(D, true);
+            int n = 0;                         // tiles before the item's
+            uint32_t nq[2] = {0, 0}, np[2] = {0, 0};  // phases of qfull and pfull
+            bool ok = true;
+            do {
+                int lo[2] = {0, 0}, hi[2] = {0, 0};
+                for (int q = 0; q < L::kQ; ++q) query_tiles(a, w, w.tile * R + q * 128, lo[q], hi[q]);
+                // step t: O of tile t - 1, then S of tile t, for each query tile in turn
+                for (int t = w.s0; t <= w.s1 && ok; ++t) {
+                    const int i = n + t - w.s0, ks_i = i % L::kStages, vs_i = (i + L::kStages - 1) % L::kStages;
+                    const bool score = t < w.s1, value = t > w.s0;
+                    if (value) {
+                        ok = bar_wait(&bars.vfull[vs_i], ((i - 1) / L::kStages) & 1, dead);
+                        const int gone = w.hi - (t - 1) * kKeys;  // keys of tile t - 1 that exist
+                        if (ok && gone < kKeys) {
+                            for (int x = lane; x < (kKeys - max(gone, 0)) * 8 * L::kHalves; x += 32) {
+                                const int row = max(gone, 0) + x / (8 * L::kHalves), col = x % (8 * L::kHalves);
+                                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                                 vs + vs_i * L::kTile + (col >> 3) * 128 * 128 + row * 128 + (col & 7) * 16),
+                                             "r"(0)
+                                             : "memory");
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                        }
+                    }
+                    if (ok && score) ok = bar_wait(&bars.kfull[ks_i], (i / L::kStages) & 1, dead);
+#pragma unroll
+                    for (int q = 0; q < L::kQ; ++q) {
+                        const uint32_t s_at = tmem + L::kS + q * L::kPitch, o_at = tmem + L::kO + q * L::kPitch;
+                        if (ok && value && t - 1 >= lo[q] && t - 1 < hi[q]) {
+                            ok = bar_wait(&bars.pfull[q], np[q]++ & 1, dead);
+                            tc_after();
+                            if (ok && lane == 0) {
+#pragma unroll
+                                for (int k = 0; k < kKeys / 16; ++k)
+                                    mma_ts(o_at, s_at + k * 8, operand(vs + vs_i * L::kTile + k * 2048, 128 * 128),
+                                           kIdescO, k > 0 || t - 1 > lo[q]);
+                                if (t == hi[q]) tc_commit(&bars.ofull[q]);
+                            }
+                            __syncwarp();
+                        }
+                        if (ok && score && t >= lo[q] && t < hi[q]) {
+                            if (t == lo[q]) ok = bar_wait(&bars.qfull[q], nq[q]++ & 1, dead);
+                            tc_after();
+                            if (ok && lane == 0) {
+#pragma unroll
+                                for (int k = 0; k < D / 16; ++k) {
+                                    const uint32_t off = (k >> 2) * 128 * 128 + (k & 3) * 32;
+                                    mma_ss(s_at, operand(qs + q * L::kTile + off, 16),
+                                           operand(ks + ks_i * L::kTile + off, 16), kIdescS, k > 0);
+                                }
+                                tc_commit(&bars.sfull[q]);
+                            }
+                            __syncwarp();
+                        }
+                    }
+                    if (ok && lane == 0) {
+                        if (value) tc_commit(&bars.vempty[vs_i]);
+                        if (score) tc_commit(&bars.kempty[ks_i]);
+                    }
+                    __syncwarp();
+                }
+                n += w.s1 - w.s0;
+            } while (ok && w.next<R>(a));
+            if (!ok) {  // matrix instructions in flight end before TMEM is freed
+                if (lane == 0) tc_commit(&bars.drain);
+                __syncwarp();
+                bar_wait(&bars.drain, 0, nullptr);
+            }
+        }
+        } else {
+            // ------------------------------------------------------------------ softmax
+            if constexpr (L::kQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));
+            const int q = warp >> 2, row = tid - q * 128;
+            const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+            const uint32_t s_at = tmem + lanes + L::kS + q * L::kPitch, o_at = tmem + lanes + L::kO + q * L::kPitch;
+            const uint32_t q_at = qs + q * L::kTile + row * 128;
+            uint32_t ns = 0, no = 0;  // phases of sfull and ofull
+            bool ok = true, first_item = true;
+            do {
+                const int r0 = w.tile * R + q * 128, rr = r0 + row;
+                if (r0 < w.rows) {
+                    int lo, hi;
+                    query_tiles(a, w, r0, lo, hi);
+                    const bool on = rr < w.rows;
+                    const int token = (on ? rr : r0) / a.group, head = w.kvh * a.group + (on ? rr - token * a.group : 0);
+                    const int pos = w.rq.pos0() + token;
+                    const int last = min(pos, w.hi - 1), first = a.p.window > 0 && pos >= a.p.window ? pos - a.p.window + 1 : 0;
+                    const float slope = kGeneral ? head_slope(a, head) : 0.f;
+                    float m = -INFINITY, l = 0.f;
+                    if (lo < hi) {
+                        // the row's queries into the swizzled rows the matrix unit reads
+                        const uint4* src = reinterpret_cast<const uint4*>(
+                            static_cast<const char*>(a.p.q) + (w.rq.first + token) * a.p.nb_q +
+                            static_cast<int64_t>(head) * D * 2);
+#pragma unroll
+                        for (int x = 0; x < L::kHalves * 8; ++x) {
+                            uint4 v = make_uint4(0, 0, 0, 0);
+                            if (on && x < D / 8) v = __ldg(src + x);
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                             q_at + (x >> 3) * 128 * 128 + (((x & 7) ^ (row & 7)) << 4)),
+                                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                                         : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        tc_before();  // O of the last item has been read
+                        bar_arrive(&bars.qfull[q]);
+                        // keys that every row of this query tile sees
+                        const int p0 = w.rq.pos0() + r0 / a.group;
+                        const int p1 = w.rq.pos0() + (min(r0 + 128, w.rows) - 1) / a.group;
+                        const int all_hi = min(p0 + 1, w.hi);
+                        const int all_lo = a.p.window > 0 && p1 >= a.p.window ? p1 - a.p.window + 1 : 0;
+                        for (int t = lo; t < hi && ok; ++t) {
+                            ok = bar_wait(&bars.sfull[q], ns++ & 1, dead);
+                            if (!ok) break;
+                            tc_after();
+                            const int j0 = t * kKeys;
+                            float s[kKeys];
+#pragma unroll
+                            for (int i = 0; i < kKeys / 32; ++i) tm_ld32(s_at + i * 32, s + i * 32);
+                            tm_wait_ld();
+                            float pre = a.pre;
+                            if (kGeneral) {
+                                pre = 1.f;
+#pragma unroll
+                                for (int i = 0; i < kKeys; ++i) {
+                                    float x = s[i] * a.pre;
+                                    if (a.post != 0.f) x = a.post * tanhf(x);
+                                    s[i] = a.bias_near ? fmaf(slope, static_cast<float>(j0 + i - pos), x) : x;
+                                }
+                            }
+                            if (j0 < all_lo || j0 + kKeys > all_hi) {
+                                const int c0 = first - j0, c1 = last - j0;
+#pragma unroll
+                                for (int i = 0; i < kKeys; ++i)
+                                    if (i < c0 || i > c1) s[i] = -INFINITY;
+                            }
+                            float top = s[0];
+#pragma unroll
+                            for (int i = 1; i < kKeys; ++i) top = fmaxf(top, s[i]);
+                            top *= pre;
+                            if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                                const float was = m;
+                                m = fmaxf(m, top);
+                                const float f = m == -INFINITY ? 1.f : exp2_fast(was - m);
+                                l *= f;
+                                if (t > lo) {
+#pragma unroll 2
+                                    for (int i = 0; i < D / 16; ++i) {
+                                        float o[16];
+                                        tm_ld16(o_at + i * 16, o);
+                                        tm_wait_ld();
+#pragma unroll
+                                        for (int e = 0; e < 16; ++e) o[e] *= f;
+                                        tm_st16(o_at + i * 16, reinterpret_cast<const uint32_t*>(o));
+                                    }
+                                }
+                            }
+                            const float off = m == -INFINITY ? 0.f : -m;
+                            float sum[4] = {};
+#pragma unroll
+                            for (int g = 0; g < kKeys / 32; ++g) {
+                                uint32_t p[16];
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    const float x = exp2_fast(fmaf(s[g * 32 + 2 * i], pre, off));
+                                    const float y = exp2_fast(fmaf(s[g * 32 + 2 * i + 1], pre, off));
+                                    sum[2 * (i & 1)] += x;
+                                    sum[2 * (i & 1) + 1] += y;
+                                    p[i] = Half16<T>::pack(x, y);
+                                }
+                                tm_st16(s_at + g * 16, p);
+                            }
+                            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                            tm_wait_st();
+                            tc_before();
+                            bar_arrive(&bars.pfull[q]);
+                        }
+                        if (ok) ok = bar_wait(&bars.ofull[q], no++ & 1, dead);
+                        if (!ok) break;
+                        tc_after();
+                    }
+                    // O to the output, or to the item's partial
+                    const bool whole = w.s0 == w.t0 && w.s1 == w.t1;
+                    const float inv = l == 0.f ? 0.f : whole ? 1.f / l : 1.f;
+                    float* part = c.g.parts + (static_cast<size_t>(me) * 2 + (w.s0 == w.t0)) * part_floats(R, D);
+                    char* out = static_cast<char*>(a.p.out) + (w.rq.first + token) * a.p.nb_out;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        float o[32];
+                        if (lo < hi) {
+                            tm_ld32(o_at + i * 32, o);
+                            tm_wait_ld();
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
+                        if (on) {
+                            float4* to = reinterpret_cast<float4*>(part + static_cast<size_t>(q * 128 + row) * D + i * 32);
+                            if (whole && a.p.out_type == GGML_TYPE_F32)
+                                to = reinterpret_cast<float4*>(out + (static_cast<int64_t>(head) * D + i * 32) * 4);
+                            if (!whole || a.p.out_type == GGML_TYPE_F32) {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                            } else {
+                                uint4* to16 = reinterpret_cast<uint4*>(out + (static_cast<int64_t>(head) * D + i * 32) * 2);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    to16[e] = make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]),
+                                                         Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
+                                                         Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]),
+                                                         Half16<T>::pack(o[8 * e + 6], o[8 * e + 7]));
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    if (!whole && on) {
+                        part[R * D + q * 128 + row] = m;
+                        part[R * D + R + q * 128 + row] = l;
+                    }
+                }
+                if (tid == 0 && w.s0 == w.t0 && w.s1 < w.t1) {
+                    // only the run's last item goes on in the next stream
+                    const long long end = first_item ? item0 + (w.t1 - w.t0) : u1 + (w.t1 - w.s1);
+                    c.g.heads[me] = SplitHead{w.b, w.kvh, w.tile, static_cast<int>(stream_of(end - 1, all, streams) - me + 1)};
+                }
+                first_item = false;
+            } while (w.next<R>(a));
+        }
+    }
+
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+// ------------------------------------------------------------------------ host
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+bool cache_map(CUtensorMap* map, const struct b200_kv_cache& kv, void* data, int box_tokens) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(kv.head_dim), static_cast<cuuint64_t>(kv.block_size),
+                                static_cast<cuuint64_t>(kv.kv_heads), static_cast<cuuint64_t>(kv.num_blocks)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(kv.nb_token), static_cast<cuuint64_t>(kv.nb_head),
+                                   static_cast<cuuint64_t>(kv.nb_block)};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_tokens), 1, 1}, ones[4] = {1, 1, 1, 1};
+    return encode_fn()(map,
+                       kv.type == GGML_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                       data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D, bool kGeneral>
+cudaError_t launch_form(const ChunkArgs& c, cudaStream_t stream) {
+    using L = Shape<D>;
+    const auto kernel = attn_chunk_kernel<T, D, kGeneral>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    if (e != cudaSuccess) return e;
+    const unsigned sms = static_cast<unsigned>(sm_count());
+    const cudaError_t f = launch_pdl(kernel, dim3(sms), dim3(L::kThreads), L::kSmem, stream, 1, c);
+    if (f != cudaSuccess) return f;
+    return launch_pdl(combine_kernel<D, L::kRows>, dim3(sms, L::kRows / 32), dim3(256), 0, stream, 1, c.g);
+}
+template <typename T, int D>
+cudaError_t launch_dim(const ChunkArgs& c, cudaStream_t stream) {
+    const AttnArgs& a = c.g.a;
+    return a.post != 0.f || a.bias_near || !(a.pre > 0.f) ? launch_form<T, D, true>(c, stream)
+                                                          : launch_form<T, D, false>(c, stream);
+}
+template <typename T>
+cudaError_t launch_type(const ChunkArgs& c, cudaStream_t stream) {
+    switch (c.g.a.kv.head_dim) {
+        case 64: return launch_dim<T, 64>(c, stream);
+        case 96: return launch_dim<T, 96>(c, stream);
+        case 128: return launch_dim<T, 128>(c, stream);
+        default: return launch_dim<T, 256>(c, stream);
+    }
+}
+
+}  // namespace
+
+size_t chunk_workspace(const AttnArgs& a) {
+    return split_bytes(static_cast<size_t>(sm_count()), a.kv.head_dim > 128 ? 128 : 256, a.kv.head_dim);
+}
+
+cudaError_t chunk_launch(const AttnArgs& a, cudaStream_t stream) {
+    if (!encode_fn()) return cudaErrorNotSupported;
+    ChunkArgs c;
+    c.g = split_args(a, static_cast<size_t>(sm_count()));
+    c.box_tokens = std::min(a.kv.block_size, kKeys);
+    if (!cache_map(&c.k, a.kv, a.kv.k, c.box_tokens) || !cache_map(&c.v, a.kv, a.kv.v, c.box_tokens))
+        return cudaErrorInvalidValue;
+    return a.kv.type == GGML_TYPE_F16 ? launch_type<__half>(c, stream) : launch_type<__nv_bfloat16>(c, stream);
+}
+
+cudaError_t paged_error_status(int* out) {
+    int v = 0, zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_chunk_error, sizeof(int));
+    if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(g_chunk_error, &zero, sizeof(int));
+    *out = v;
+    return e;
+}
+
+}  // namespace xb

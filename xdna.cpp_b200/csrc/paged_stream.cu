@@ -18,7 +18,7 @@
 // is at most 2^8), which a vote finds out; moving it takes the shuffles.
 #include <algorithm>
 
-#include "paged_attn.cuh"
+#include "paged_split.cuh"
 
 namespace xb {
 namespace {
@@ -34,20 +34,6 @@ struct Ring {
     static constexpr int kStride = D + 8;
     static constexpr int kHalf = kKeys * kStride;  // elements of K (and of V) in a stage
     static constexpr size_t kBytes = static_cast<size_t>(kWarps) * kStages * 2 * kHalf * sizeof(uint16_t);
-};
-
-// What a stream that begins an item, but does not end it, leaves for combine_kernel.
-struct alignas(16) Head {
-    int b, kvh, tile;
-    int parts;  // streams the item lies in; 0: none
-};
-
-__host__ __device__ __forceinline__ size_t part_floats(int R, int D) { return static_cast<size_t>(R) * (D + 2); }
-
-struct StreamArgs {
-    AttnArgs a;
-    Head* heads;   // [streams]
-    float* parts;  // [streams][2][R][D] sums, then [R] maxima and [R] l: slot 0 for an item begun elsewhere
 };
 
 // Walks the units of a stream.
@@ -84,7 +70,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 template <typename T, int D, int NP, int NT>
-__global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(const __grid_constant__ StreamArgs g) {
+__global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(const __grid_constant__ SplitArgs g) {
     using L = Ring<D>;
     constexpr int R = 8 * NT, kThreads = L::kWarps * 32, kS = L::kStride, kSteps = D / 16;
     extern __shared__ __align__(16) uint16_t smem[];
@@ -395,10 +381,8 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
                 }
             }
         if (begun_here && !ends && lane == 0) {
-            // the stream that holds the item's last unit u is the largest with all * w / streams <= u
-            const long long u = item0 + at.w.units - 1;
-            const long long w1 = ((u + 1) * streams - 1) / all;
-            g.heads[me] = Head{at.b, at.kvh, at.tile, static_cast<int>(w1 - me + 1)};
+            const long long w1 = stream_of(item0 + at.w.units - 1, all, streams);
+            g.heads[me] = SplitHead{at.b, at.kvh, at.tile, static_cast<int>(w1 - me + 1)};
         }
         if (todo > 0) {
             item0 += at.w.units;
@@ -409,64 +393,9 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Joins the partials of the item that stream blockIdx.x began: a warp per row,
-// parts in stream order.
-template <int D, int R>
-__global__ void __launch_bounds__(R < 8 ? 32 * R : 256) combine_kernel(const __grid_constant__ StreamArgs g) {
-    grid_wait();
-    const AttnArgs& a = g.a;
-    const Head head = g.heads[blockIdx.x];
-    if (!head.parts) return;
-    const Request rq = read_request(a, head.b);
-    const int rows = min(R, rq.count * a.group - head.tile * R), lane = threadIdx.x & 31;
-    const size_t slot = part_floats(R, D);
-    for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5) {
-        // lane p holds part p, p + 32, ...: the row's largest maximum, then its parts' weights
-        auto part = [&](int p) { return g.parts + (2 * (static_cast<size_t>(blockIdx.x) + p) + (p == 0)) * slot; };
-        float top = -INFINITY;
-        for (int p = lane; p < head.parts; p += 32) top = fmaxf(top, part(p)[R * D + r]);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const float base = top == -INFINITY ? 0.f : top;
-        float sum = 0.f, o[D / 32] = {};
-        for (int p0 = 0; p0 < head.parts; p0 += 32) {
-            float w = 0.f;
-            if (p0 + lane < head.parts) {
-                const float* x = part(p0 + lane);
-                w = exp2f(x[R * D + r] - base);
-                sum += w * x[R * D + R + r];
-            }
-            const int n = min(32, head.parts - p0);
-#pragma unroll 4
-            for (int p = 0; p < n; ++p) {
-                const float c = __shfl_sync(0xffffffffu, w, p);
-                const float* x = part(p0 + p) + r * D + lane * 2;
-#pragma unroll
-                for (int i = 0; i < D / 64; ++i) {
-                    const float2 v = *reinterpret_cast<const float2*>(x + i * 64);
-                    o[2 * i] = fmaf(c, v.x, o[2 * i]);
-                    o[2 * i + 1] = fmaf(c, v.y, o[2 * i + 1]);
-                }
-                if (D % 64) o[D / 32 - 1] = fmaf(c, part(p0 + p)[r * D + D / 64 * 64 + lane], o[D / 32 - 1]);
-            }
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int rr = head.tile * R + r, i = rr / a.group, h = head.kvh * a.group + rr - i * a.group;
-#pragma unroll
-        for (int k = 0; k < D / 64; ++k)
-            store_out(a, rq.first + i, h, k * 64 + lane * 2, sum == 0.f ? 0.f : o[2 * k] * inv,
-                      sum == 0.f ? 0.f : o[2 * k + 1] * inv);
-        if (D % 64)
-            store_one(a, rq.first + i, h, D / 64 * 64 + lane, sum == 0.f ? 0.f : o[D / 32 - 1] * inv);
-    }
-}
-
 template <int D>
 size_t workspace_of(int R) {
-    const size_t streams = static_cast<size_t>(sm_count()) * Ring<D>::kWarps;
-    return streams * (sizeof(Head) + 2 * part_floats(R, D) * sizeof(float));
+    return split_bytes(static_cast<size_t>(sm_count()) * Ring<D>::kWarps, R, D);
 }
 
 template <typename T, int D, int NP, int NT>
@@ -477,9 +406,7 @@ cudaError_t launch_rows(const AttnArgs& a, cudaStream_t stream) {
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L::kBytes));
     if (e != cudaSuccess) return e;
     const unsigned sms = static_cast<unsigned>(sm_count());
-    StreamArgs g{a, nullptr, nullptr};
-    g.heads = static_cast<Head*>(a.p.workspace);
-    g.parts = reinterpret_cast<float*>(g.heads + static_cast<size_t>(sms) * L::kWarps);
+    const SplitArgs g = split_args(a, static_cast<size_t>(sms) * L::kWarps);
     const cudaError_t f = launch_pdl(kernel, dim3(sms), dim3(L::kWarps * 32), L::kBytes, stream, 1, g);
     if (f != cudaSuccess) return f;
     return launch_pdl(combine_kernel<D, 8 * NT>, dim3(sms * L::kWarps), dim3(256), 0, stream, 1, g);

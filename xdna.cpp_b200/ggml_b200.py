@@ -182,6 +182,7 @@ def lib() -> C.CDLL:
         "b200_kv_plan": (C.c_int, [C.POINTER(KvPlan), vp]),
         "b200_qk_norm_rope": (C.c_int, [C.POINTER(QkNormRope), C.POINTER(KvCache), vp]),
         "b200_paged_attention_workspace": (sz, [C.POINTER(PagedAttention), C.POINTER(KvCache)]),
+        "b200_paged_attention_error": (C.c_int, [C.POINTER(C.c_int)]),
         "b200_paged_attention": (C.c_int, [C.POINTER(PagedAttention), C.POINTER(KvCache), vp]),
     }
     for name, (res, args) in sig.items():
