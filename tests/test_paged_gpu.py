@@ -310,12 +310,15 @@ TYPES = [(F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)]
 @pytest.mark.parametrize("lens", LENS, ids=str)
 def test_paged_attention(cuda, G, lens, D, q_type, cache_type):
     check_attention(G, lens, 6, 2, D, q_type, cache_type, 16, seed=D)
+    check_attention(G, lens, 6, 2, D, q_type, cache_type, 16, seed=D, max_kv=100000)  # another work split
 
 
 @pytest.mark.parametrize("q_type,cache_type", TYPES)
 @pytest.mark.parametrize("H,KH", [(1, 1), (5, 5), (8, 1), (14, 2), (17, 1), (64, 8), (72, 2)])
 def test_paged_attention_groups(cuda, G, H, KH, q_type, cache_type):
     check_attention(G, [(100, 1), (33, 3), (257, 20)], H, KH, 128, q_type, cache_type, 32, seed=H)
+    check_attention(G, [(100, 1), (33, 2), (257, 1)], H, KH, 128, q_type, cache_type, 32, seed=H)
+    check_attention(G, [(100, 1), (33, 2), (257, 1)], H, KH, 128, q_type, cache_type, 32, seed=H, max_kv=100000)
 
 
 @pytest.mark.parametrize("q_type,cache_type", TYPES)
@@ -325,6 +328,7 @@ def test_paged_attention_groups(cuda, G, H, KH, q_type, cache_type):
 def test_paged_attention_masks(cuda, G, opts, lens, q_type, cache_type):
     check_attention(G, lens, 12, 4, 128, q_type, cache_type, 64, seed=11, **opts)
     check_attention(G, lens, 3, 1, 64, q_type, cache_type, 16, seed=12, **opts)
+    check_attention(G, lens, 3, 1, 64, q_type, cache_type, 16, seed=12, max_kv=100000, **opts)
 
 
 @pytest.mark.parametrize("lens", [[(3000, 1)], [(5000, 1), (1, 1), (1024, 1)], [(1500, 700), (900, 1), (257, 64)]], ids=str)
@@ -332,6 +336,7 @@ def test_paged_attention_masks(cuda, G, opts, lens, q_type, cache_type):
 @pytest.mark.parametrize("q_type,cache_type", TYPES)
 def test_paged_attention_long(cuda, G, lens, bs, q_type, cache_type):
     check_attention(G, lens, 16, 2, 128, q_type, cache_type, bs, seed=bs)
+    check_attention(G, lens, 16, 2, 128, q_type, cache_type, bs, seed=bs, max_kv=100000)  # another work split
 
 
 @pytest.mark.parametrize("lens", [[(200, 1), (90, 1)], [(200, 100), (90, 1)]], ids=str)

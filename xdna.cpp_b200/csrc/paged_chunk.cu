@@ -723,7 +723,9 @@ cudaError_t launch_form(const ChunkArgs& c, cudaStream_t stream) {
     const unsigned sms = static_cast<unsigned>(sm_count());
     const cudaError_t f = launch_pdl(kernel, dim3(sms), dim3(L::kThreads), L::kSmem, stream, 1, c);
     if (f != cudaSuccess) return f;
-    return launch_pdl(combine_kernel<D, L::kRows>, dim3(sms, L::kRows / 32), dim3(256), 0, stream, 1, c.g);
+    const AttnArgs& a = c.g.a;
+    const int64_t items = (a.p.n_tokens * a.group / L::kRows + 1) * a.kv.kv_heads;
+    return combine_launch<D, L::kRows>(c.g, items, stream);
 }
 template <typename T, int D>
 cudaError_t launch_dim(const ChunkArgs& c, cudaStream_t stream) {

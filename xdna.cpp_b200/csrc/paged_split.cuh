@@ -6,6 +6,8 @@
 // that begins in it and goes on.  combine_kernel looks at every stream that
 // began such an item and adds its parts up in stream order.
 #pragma once
+#include <algorithm>
+
 #include "paged_attn.cuh"
 
 namespace xb {
@@ -23,13 +25,15 @@ struct SplitArgs {
     AttnArgs a;
     SplitHead* heads;  // [streams]
     float* parts;      // [streams][2] partials
+    int streams;       // that may have work
+    int tiles;         // joining form of the stream kernel: row tiles its grid has for each request
 };
 
 inline size_t split_bytes(size_t streams, int R, int D) {
     return streams * (sizeof(SplitHead) + 2 * part_floats(R, D) * sizeof(float));
 }
 inline SplitArgs split_args(const AttnArgs& a, size_t streams) {
-    SplitArgs g{a, static_cast<SplitHead*>(a.p.workspace), nullptr};
+    SplitArgs g{a, static_cast<SplitHead*>(a.p.workspace), nullptr, static_cast<int>(streams), 1};
     g.parts = reinterpret_cast<float*>(g.heads + streams);
     return g;
 }
@@ -41,57 +45,98 @@ __device__ __forceinline__ long long stream_of(long long u, long long all, long 
     return ((u + 1) * streams - 1) / all;
 }
 
-// Stream blockIdx.x's item: a warp per row, the rows dealt out over blockIdx.y.
-template <int D, int R>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ SplitArgs g) {
+constexpr int kCombineWarps = 8;
+
+// Joins the item that stream blockIdx.x began.  Block y takes the rows y, y +
+// gridDim.y, ...; kSpread: all warps share the parts of one row at a time (few
+// items, many parts), else every warp takes rows of its own.
+template <int D, int R, bool kSpread>
+__global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const __grid_constant__ SplitArgs g) {
+    __shared__ float shared_o[kSpread ? kCombineWarps : 1][D];
+    __shared__ float shared_l[kCombineWarps];
     grid_wait();
     const AttnArgs& a = g.a;
     const SplitHead head = g.heads[blockIdx.x];
     if (!head.parts) return;
     const Request rq = read_request(a, head.b);
-    const int rows = min(R, rq.count * a.group - head.tile * R), lane = threadIdx.x & 31;
+    const int rows = min(R, rq.count * a.group - head.tile * R), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t slot = part_floats(R, D);
-    for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += 8 * gridDim.y) {
-        // lane p holds part p, p + 32, ...: the row's largest maximum, then its parts' weights
-        auto part = [&](int p) { return g.parts + (2 * (static_cast<size_t>(blockIdx.x) + p) + (p == 0)) * slot; };
+    const float* mine = g.parts + 2 * static_cast<size_t>(blockIdx.x) * slot;
+    auto part = [&](int p) { return mine + (2 * static_cast<size_t>(p) + (p == 0)) * slot; };
+    const int step = kSpread ? gridDim.y : gridDim.y * kCombineWarps;
+    for (int r = kSpread ? blockIdx.y : blockIdx.y + gridDim.y * warp; r < rows; r += step) {
+        // the row's largest maximum
         float top = -INFINITY;
         for (int p = lane; p < head.parts; p += 32) top = fmaxf(top, part(p)[R * D + r]);
 #pragma unroll
         for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         const float base = top == -INFINITY ? 0.f : top;
+        // this warp's parts: lane i holds the weight of the i-th of 32 of them
+        const int first = kSpread ? warp : 0, stride = kSpread ? kCombineWarps : 1;
         float sum = 0.f, o[D / 32] = {};
-        for (int p0 = 0; p0 < head.parts; p0 += 32) {
+        for (int p0 = first; p0 < head.parts; p0 += 32 * stride) {
             float w = 0.f;
-            if (p0 + lane < head.parts) {
-                const float* x = part(p0 + lane);
+            if (p0 + lane * stride < head.parts) {
+                const float* x = part(p0 + lane * stride);
                 w = exp2f(x[R * D + r] - base);
                 sum += w * x[R * D + R + r];
             }
-            const int n = min(32, head.parts - p0);
-#pragma unroll 4
-            for (int p = 0; p < n; ++p) {
-                const float c = __shfl_sync(0xffffffffu, w, p);
-                const float* x = part(p0 + p) + r * D + lane * 2;
+            const int n = min(32, (head.parts - p0 + stride - 1) / stride);
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) {
+                const float c = __shfl_sync(0xffffffffu, w, i);
+                const float* x = part(p0 + i * stride) + r * D;
 #pragma unroll
-                for (int i = 0; i < D / 64; ++i) {
-                    const float2 v = *reinterpret_cast<const float2*>(x + i * 64);
-                    o[2 * i] = fmaf(c, v.x, o[2 * i]);
-                    o[2 * i + 1] = fmaf(c, v.y, o[2 * i + 1]);
+                for (int k = 0; k < D / 64; ++k) {
+                    const float2 v = *reinterpret_cast<const float2*>(x + k * 64 + lane * 2);
+                    o[2 * k] = fmaf(c, v.x, o[2 * k]);
+                    o[2 * k + 1] = fmaf(c, v.y, o[2 * k + 1]);
                 }
-                if (D % 64) o[D / 32 - 1] = fmaf(c, part(p0 + p)[r * D + D / 64 * 64 + lane], o[D / 32 - 1]);
+                if (D % 64) o[D / 32 - 1] = fmaf(c, x[D / 64 * 64 + lane], o[D / 32 - 1]);
             }
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const int rr = head.tile * R + r, i = rr / a.group, h = head.kvh * a.group + rr - i * a.group;
+        if constexpr (kSpread) {
 #pragma unroll
-        for (int k = 0; k < D / 64; ++k)
-            store_out(a, rq.first + i, h, k * 64 + lane * 2, sum == 0.f ? 0.f : o[2 * k] * inv,
-                      sum == 0.f ? 0.f : o[2 * k + 1] * inv);
-        if (D % 64)
-            store_one(a, rq.first + i, h, D / 64 * 64 + lane, sum == 0.f ? 0.f : o[D / 32 - 1] * inv);
+            for (int k = 0; k < D / 64; ++k)
+                *reinterpret_cast<float2*>(&shared_o[warp][k * 64 + lane * 2]) = make_float2(o[2 * k], o[2 * k + 1]);
+            if (D % 64) shared_o[warp][D / 64 * 64 + lane] = o[D / 32 - 1];
+            if (lane == 0) shared_l[warp] = sum;
+            __syncthreads();
+            float l = 0.f;
+#pragma unroll
+            for (int w = 0; w < kCombineWarps; ++w) l += shared_l[w];
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            for (int c = threadIdx.x; c < D; c += 32 * kCombineWarps) {
+                float x = 0.f;
+#pragma unroll
+                for (int w = 0; w < kCombineWarps; ++w) x += shared_o[w][c];
+                store_one(a, rq.first + i, h, c, l == 0.f ? 0.f : x * inv);
+            }
+            __syncthreads();
+        } else {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+            for (int k = 0; k < D / 64; ++k)
+                store_out(a, rq.first + i, h, k * 64 + lane * 2, sum == 0.f ? 0.f : o[2 * k] * inv,
+                          sum == 0.f ? 0.f : o[2 * k + 1] * inv);
+            if (D % 64) store_one(a, rq.first + i, h, D / 64 * 64 + lane, sum == 0.f ? 0.f : o[D / 32 - 1] * inv);
+        }
     }
+}
+
+// Launches combine_kernel after a kernel whose items are about `items` (as the
+// hints have it).
+template <int D, int R>
+cudaError_t combine_launch(const SplitArgs& g, int64_t items, cudaStream_t stream) {
+    const int streams = g.streams;
+    if (streams >= 8 * items)
+        return launch_pdl(combine_kernel<D, R, true>, dim3(streams, std::min(R, 8)), dim3(32 * kCombineWarps), 0, stream,
+                          1, g);
+    return launch_pdl(combine_kernel<D, R, false>, dim3(streams, (R + 31) / 32), dim3(32 * kCombineWarps), 0, stream, 1,
+                      g);
 }
 #endif
 

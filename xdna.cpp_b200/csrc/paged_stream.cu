@@ -24,8 +24,10 @@ namespace xb {
 namespace {
 
 constexpr int kKeys = 16;      // a unit
-constexpr int kMinUnits = 4;   // units per stream below which fewer streams run
+constexpr int kMinUnits = 2;   // units per stream below which fewer streams run
 constexpr float kSlack = 8.f;  // log2 of the largest weight
+constexpr int kCluster = 8;    // CTAs that share an item of the joining form
+constexpr int kJoinKeys = 8192;  // keys up to which it is taken
 
 template <int D>
 struct Ring {
@@ -69,7 +71,78 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
-template <typename T, int D, int NP, int NT>
+// Joins the partials that the warps of a cluster hold in shared memory, one at
+// the start of each warp's ring, and writes the item's rows: first the warps of
+// each CTA, then the CTAs' sums over distributed shared memory (rank r writes the
+// rows r, r + kCluster, ...).
+template <int D, int R, int kWarps, int kRingBytes>
+__device__ __forceinline__ void cluster_join(const AttnArgs& a, const Request& rq, int kvh, int tile, int rows,
+                                             uint16_t* smem) {
+    constexpr int kThreads = kWarps * 32, kEach = R * D / kThreads;
+    const int tid = threadIdx.x, rank = static_cast<int>(blockIdx.x) % kCluster;
+    auto part = [&](int w) { return reinterpret_cast<float*>(reinterpret_cast<char*>(smem) + static_cast<size_t>(w) * kRingBytes); };
+    __syncthreads();
+    float o[kEach], top[kEach], sum[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int x = i * kThreads + tid, r = x / D;
+        top[i] = -INFINITY, sum[i] = 0.f, o[i] = 0.f;
+        if (r >= rows) continue;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top[i] = fmaxf(top[i], part(w)[R * D + r]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float m = part(w)[R * D + r];
+            if (m == -INFINITY) continue;  // its sums are not written
+            const float c = exp2f(m - top[i]);
+            sum[i] = fmaf(c, part(w)[R * D + R + r], sum[i]);
+            o[i] = fmaf(c, part(w)[x], o[i]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int x = i * kThreads + tid, r = x / D;
+        part(0)[x] = o[i];
+        if (x % D == 0) part(0)[R * D + r] = top[i], part(0)[R * D + R + r] = sum[i];
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    uint32_t from[kCluster];
+#pragma unroll
+    for (int c = 0; c < kCluster; ++c)
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from[c]) : "r"(smem_addr(part(0))), "r"(c));
+    auto get = [&](int c, int x) {
+        float v;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(from[c] + 4 * x) : "memory");
+        return v;
+    };
+    for (int x = tid; x < (R + kCluster - 1) / kCluster * D; x += kThreads) {
+        const int r = rank + x / D * kCluster, col = x % D;
+        if (r >= rows) continue;
+        float m[kCluster], v[kCluster], l[kCluster], t = -INFINITY, all = 0.f, y = 0.f;
+#pragma unroll
+        for (int c = 0; c < kCluster; ++c) m[c] = get(c, R * D + r), l[c] = get(c, R * D + R + r), v[c] = get(c, r * D + col);
+#pragma unroll
+        for (int c = 0; c < kCluster; ++c) t = fmaxf(t, m[c]);
+        t = t == -INFINITY ? 0.f : t;
+#pragma unroll
+        for (int c = 0; c < kCluster; ++c) {
+            const float f = exp2f(m[c] - t);
+            all = fmaf(f, l[c], all);
+            y = fmaf(f, v[c], y);
+        }
+        const int rr = tile * R + r, i = rr / a.group;
+        store_one(a, rq.first + i, kvh * a.group + rr - i * a.group, col, all == 0.f ? 0.f : y / all);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // until then the sums stay
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// kJoin: a cluster of kCluster CTAs takes one item (and those g.tiles row tiles
+// further on), its warps equal runs of the item's units, and joins them in shared
+// memory: one launch and no workspace, for few items with few keys.
+template <typename T, int D, int NP, int NT, bool kJoin>
 __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(const __grid_constant__ SplitArgs g) {
     using L = Ring<D>;
     constexpr int R = 8 * NT, kThreads = L::kWarps * 32, kS = L::kStride, kSteps = D / 16;
@@ -79,7 +152,19 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
     const AttnArgs& a = g.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.p.n_seqs;
     grid_wait();
+    if (!kJoin) grid_release();  // combine_kernel may take its place on the SMs; it waits for this grid's end
 
+    Cursor at;
+    int left = 0;         // units to fetch
+    long long item0 = 0;  // units before the item `at` is in
+    long long me = 0, all = 0, streams = 0;
+    if constexpr (kJoin) {
+        const int item = static_cast<int>(blockIdx.x) / kCluster;
+        at.kvh = item % a.kv.kv_heads;
+        at.tile = item / a.kv.kv_heads % g.tiles;
+        at.b = item / a.kv.kv_heads / g.tiles;
+        at.enter<R>(a);
+    } else {
     // units of all requests, summed up over the threads
     const int per = (B + kThreads - 1) / kThreads;
     {
@@ -101,20 +186,16 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
         if (tid == 0) before[0] = 0;
         __syncthreads();
     }
-    const long long all = before[kThreads];
-    const long long most = static_cast<long long>(gridDim.x) * L::kWarps;
-    const long long streams = min(most, max(1LL, all / kMinUnits));
+    all = before[kThreads];
+    streams = min(static_cast<long long>(g.streams), max(1LL, all / kMinUnits));
     // neighbouring streams lie on different SMs: a short run of units uses all of them
-    const long long me = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
-    if (lane == 0) g.heads[me].parts = 0;
+    me = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
+    if (lane == 0 && me < g.streams) g.heads[me].parts = 0;
     if (me >= streams || all == 0) return;
     const long long u0 = all * me / streams, u1 = all * (me + 1) / streams;
-    int left = static_cast<int>(u1 - u0);  // units to fetch
-    int todo = left;                       // units to work off
+    left = static_cast<int>(u1 - u0);
 
     // the first unit
-    Cursor at;
-    long long item0;  // units before the item `at` is in
     {
         int lo = 0, hi = kThreads;
         while (hi - lo > 1) {
@@ -137,20 +218,31 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
         at.tile = static_cast<int>(item - static_cast<long long>(at.kvh) * at.w.tiles);
         item0 = u0 - at.unit;
     }
+    }
+    for (; !kJoin || at.tile < at.w.tiles; at.tile += g.tiles) {
+    if constexpr (kJoin) {
+        const int n = at.w.units, i = warp * kCluster + static_cast<int>(blockIdx.x) % kCluster;
+        constexpr int kAll = kCluster * L::kWarps;
+        at.unit = static_cast<int>(static_cast<long long>(n) * i / kAll);
+        left = static_cast<int>(static_cast<long long>(n) * (i + 1) / kAll) - at.unit;
+    }
+    int todo = left;  // units to work off
 
     // the ring: `fetch` runs ahead of `at`
     uint16_t* ring = smem + static_cast<size_t>(warp) * L::kStages * 2 * L::kHalf;
     Cursor fetch = at;
+    // the table entry of a unit's block, not looked at before the unit is loaded
     auto block_of = [&](const Cursor& c) {
         const int j0 = c.w.lo + c.unit * kKeys;
-        return j0 < c.w.hi ? key_block(a, c.b, j0 >> a.log_bs) : -1;
+        return j0 < c.w.hi ? __ldg(a.p.block_table + static_cast<int64_t>(c.b) * a.p.table_width + (j0 >> a.log_bs)) : -1;
     };
     int id = block_of(fetch), fill = 0;
     auto load = [&]() {
         if (left > 0) {
             const int j0 = fetch.w.lo + fetch.unit * kKeys;
-            const int n = id < 0 ? 0 : fetch.w.hi - j0;  // keys of the unit that exist
-            const int64_t base = id < 0 ? 0
+            const bool known = id >= 0 && id < a.kv.num_blocks;
+            const int n = known ? fetch.w.hi - j0 : 0;  // keys of the unit that exist
+            const int64_t base = !known ? 0
                                         : id * a.kv.nb_block + fetch.kvh * a.kv.nb_head +
                                               (j0 & (a.kv.block_size - 1)) * a.kv.nb_token;
             uint16_t* to = ring + fill * 2 * L::kHalf;
@@ -340,6 +432,10 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
         stage = stage + 1 == L::kStages ? 0 : stage + 1;
         --todo;
         const bool ends = at.unit + 1 == at.w.units;
+        if constexpr (kJoin) {
+            if (todo > 0) ++at.unit;
+            continue;
+        }
         if (!ends && todo > 0) {
             ++at.unit;
             continue;
@@ -391,6 +487,38 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if constexpr (!kJoin) {
+        break;
+    } else {
+        // this warp's sums to the start of its ring (all of it has been read)
+        __syncwarp();
+        float* to = reinterpret_cast<float*>(ring);
+        const bool any = at.w.units > 0 && !fresh;
+        const int r0 = at.tile * R;
+        rows = min(R, at.w.rows - r0);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int r = nt * 8 + 2 * (lane & 3) + q;
+                float sum = any ? l[nt][q] : 0.f;
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                if (any)
+#pragma unroll
+                    for (int n = 0; n < kSteps; ++n) {
+                        to[r * D + n * 16 + (lane >> 2)] = o[nt][n][q];
+                        to[r * D + n * 16 + 8 + (lane >> 2)] = o[nt][n][2 + q];
+                    }
+                if ((lane >> 2) == 0) {
+                    to[R * D + r] = any ? m[nt][q] : -INFINITY;
+                    to[R * D + R + r] = sum;
+                }
+            }
+        cluster_join<D, R, L::kWarps, L::kStages * 2 * L::kHalf * 2>(a, at.rq, at.kvh, at.tile, rows, smem);
+    }
+    }
 }
 
 template <int D>
@@ -398,18 +526,44 @@ size_t workspace_of(int R) {
     return split_bytes(static_cast<size_t>(sm_count()) * Ring<D>::kWarps, R, D);
 }
 
-template <typename T, int D, int NP, int NT>
-cudaError_t launch_rows(const AttnArgs& a, cudaStream_t stream) {
+// The joining form is taken where its clusters fit on the SMs at once and no
+// warp gets a long run.
+struct Items {
+    int64_t tiles, count;  // row tiles of a request, items of the call (as the hints have it)
+    bool join;
+};
+Items count_items(const AttnArgs& a, int R) {
+    Items i;
+    i.tiles = std::max<int64_t>(1, (static_cast<int64_t>(a.p.max_new) * a.group + R - 1) / R);
+    i.count = i.tiles * a.p.n_seqs * a.kv.kv_heads;
+    i.join = i.count * kCluster <= sm_count() && a.p.max_kv <= kJoinKeys;
+    return i;
+}
+
+template <typename T, int D, int NP, int NT, bool kJoin>
+cudaError_t launch_form(const SplitArgs& g, int ctas, cudaStream_t stream) {
     using L = Ring<D>;
-    const auto kernel = attn_stream_kernel<T, D, NP, NT>;
+    const auto kernel = attn_stream_kernel<T, D, NP, NT, kJoin>;
     const cudaError_t e =
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L::kBytes));
     if (e != cudaSuccess) return e;
-    const unsigned sms = static_cast<unsigned>(sm_count());
-    const SplitArgs g = split_args(a, static_cast<size_t>(sms) * L::kWarps);
-    const cudaError_t f = launch_pdl(kernel, dim3(sms), dim3(L::kWarps * 32), L::kBytes, stream, 1, g);
-    if (f != cudaSuccess) return f;
-    return launch_pdl(combine_kernel<D, 8 * NT>, dim3(sms * L::kWarps), dim3(256), 0, stream, 1, g);
+    return launch_pdl(kernel, dim3(ctas), dim3(L::kWarps * 32), L::kBytes, stream, kJoin ? kCluster : 1, g);
+}
+
+template <typename T, int D, int NP, int NT>
+cudaError_t launch_rows(const AttnArgs& a, cudaStream_t stream) {
+    using L = Ring<D>;
+    const Items items = count_items(a, 8 * NT);
+    const int sms = sm_count();
+    SplitArgs g = split_args(a, static_cast<size_t>(sms) * L::kWarps);
+    g.tiles = static_cast<int>(items.tiles);
+    if (items.join) return launch_form<T, D, NP, NT, true>(g, static_cast<int>(items.count) * kCluster, stream);
+    // no more streams than the hints give work for
+    const int64_t units = items.count * std::max(1, (a.p.max_kv + kKeys - 1) / kKeys);
+    g.streams = static_cast<int>(std::min<int64_t>(sms * L::kWarps, std::max<int64_t>(1, units / kMinUnits)));
+    const cudaError_t e = launch_form<T, D, NP, NT, false>(g, std::min(sms, g.streams), stream);
+    if (e != cudaSuccess) return e;
+    return combine_launch<D, 8 * NT>(g, items.count, stream);
 }
 
 // Rows of an item: as few 8-column blocks as the hints ask for, as many as the
@@ -450,6 +604,7 @@ cudaError_t launch_type(const AttnArgs& a, cudaStream_t stream) {
 
 size_t stream_workspace(const AttnArgs& a) {
     const int R = 8 * row_blocks(a);
+    if (count_items(a, R).join) return 0;
     switch (a.kv.head_dim) {
         case 64: return workspace_of<64>(R);
         case 96: return workspace_of<96>(R);
