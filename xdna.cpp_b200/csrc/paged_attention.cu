@@ -362,4 +362,11 @@ cudaError_t paged_attention_launch(const struct b200_paged_attention_args& p, co
     return kv.type == GGML_TYPE_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream);
 }
 
+cudaError_t paged_error_status(int* out) {
+    int stream = 0, chunk = 0;
+    const cudaError_t e = stream_error(&stream), f = chunk_error(&chunk);
+    *out = stream || chunk;
+    return e != cudaSuccess ? e : f;
+}
+
 }  // namespace xb

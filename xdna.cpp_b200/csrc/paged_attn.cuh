@@ -34,10 +34,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kStreamRows = 32;
 size_t stream_workspace(const AttnArgs& a);
 cudaError_t stream_launch(const AttnArgs& a, cudaStream_t stream);
+cudaError_t stream_error(int* out);  // reads and clears the error word of its bounded waits
 
 // The chunk kernel (paged_chunk.cu), for 16-bit queries: its workspace and launch.
 size_t chunk_workspace(const AttnArgs& a);
 cudaError_t chunk_launch(const AttnArgs& a, cudaStream_t stream);
+cudaError_t chunk_error(int* out);
 
 #ifdef __CUDACC__
 // Slope of a query head, times log2(e).

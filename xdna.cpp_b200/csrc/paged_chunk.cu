@@ -28,12 +28,10 @@
 // Every wait is bounded (2 s of %globaltimer): one that runs out sets the error
 // word, all roles give up, copies and matrix instructions in flight are waited
 // for (bounded again), and TMEM is freed.
-#include <cuda.h>
-
 #include <algorithm>
-#include <mutex>
 
 #include "paged_split.cuh"
+#include "paged_tma.cuh"
 
 namespace xb {
 namespace {
@@ -41,9 +39,6 @@ namespace {
 constexpr int kKeys = 128;
 constexpr int kMinTiles = 2;   // key tiles per CTA below which fewer CTAs run
 constexpr float kSlack = 8.f;  // log2 of the largest weight
-constexpr unsigned long long kWaitNs = 2000000000ull;
-
-__device__ int g_chunk_error;
 
 template <int D>
 struct Shape {
@@ -72,48 +67,6 @@ struct Bars {
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
     uint64_t qfull[2], sfull[2], pfull[2], ofull[2], drain;
 };
-
-__device__ __forceinline__ void bar_init(uint64_t* b, int count) {
-    asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t* b) {
-    asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(smem_addr(b)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-// Waits for the phase; false when 2 s have passed or another wait has given up.
-__device__ __forceinline__ bool bar_wait_slow(uint64_t* b, uint32_t parity, volatile int* dead) {
-    const unsigned long long t0 = now_ns();
-    for (;;) {
-        for (int i = 0; i < 64; ++i)
-            if (bar_try(b, parity)) return true;
-        if (dead && *dead) return false;
-        if (now_ns() - t0 > kWaitNs) {
-            if (dead) *dead = 1;
-            atomicExch(&g_chunk_error, 1);
-            return false;
-        }
-    }
-}
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* dead) {
-    bool ok = bar_try(b, parity) || bar_try(b, parity) || bar_wait_slow(b, parity, dead);
-    return __all_sync(0xffffffffu, ok);  // the warp goes on, or gives up, as one
-}
 
 // ------------------------------------------------------------ matrix unit, TMEM
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -179,19 +132,6 @@ __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* u) {
         "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
         : "memory");
 }
-__device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
-                                        int c3) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-        ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-        : "memory");
-}
-
 // ------------------------------------------------------------------ the work list
 // Key tiles [t0, t1) of row tile `tile`, and of one of its query tiles.
 template <int R>
@@ -686,34 +626,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
 }
 
 // ------------------------------------------------------------------------ host
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encode_fn() {
-    static EncodeFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
-            found != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeFn>(p);
-    }();
-    return fn;
-}
-
-bool cache_map(CUtensorMap* map, const struct b200_kv_cache& kv, void* data, int box_tokens) {
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(kv.head_dim), static_cast<cuuint64_t>(kv.block_size),
-                                static_cast<cuuint64_t>(kv.kv_heads), static_cast<cuuint64_t>(kv.num_blocks)};
-    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(kv.nb_token), static_cast<cuuint64_t>(kv.nb_head),
-                                   static_cast<cuuint64_t>(kv.nb_block)};
-    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_tokens), 1, 1}, ones[4] = {1, 1, 1, 1};
-    return encode_fn()(map,
-                       kv.type == GGML_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                       data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int D, bool kGeneral>
 cudaError_t launch_form(const ChunkArgs& c, cudaStream_t stream) {
     using L = Shape<D>;
@@ -750,7 +662,6 @@ size_t chunk_workspace(const AttnArgs& a) {
 }
 
 cudaError_t chunk_launch(const AttnArgs& a, cudaStream_t stream) {
-    if (!encode_fn()) return cudaErrorNotSupported;
     ChunkArgs c;
     c.g = split_args(a, static_cast<size_t>(sm_count()));
     c.box_tokens = std::min(a.kv.block_size, kKeys);
@@ -759,12 +670,6 @@ cudaError_t chunk_launch(const AttnArgs& a, cudaStream_t stream) {
     return a.kv.type == GGML_TYPE_F16 ? launch_type<__half>(c, stream) : launch_type<__nv_bfloat16>(c, stream);
 }
 
-cudaError_t paged_error_status(int* out) {
-    int v = 0, zero = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&v, g_chunk_error, sizeof(int));
-    if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(g_chunk_error, &zero, sizeof(int));
-    *out = v;
-    return e;
-}
+cudaError_t chunk_error(int* out) { return take_wait_error(out); }
 
 }  // namespace xb

@@ -19,23 +19,34 @@
 #include <algorithm>
 
 #include "paged_split.cuh"
+#include "paged_tma.cuh"
 
 namespace xb {
 namespace {
 
-constexpr int kKeys = 16;      // a unit
-constexpr int kMinUnits = 2;   // units per stream below which fewer streams run
-constexpr float kSlack = 8.f;  // log2 of the largest weight
-constexpr int kCluster = 8;    // CTAs that share an item of the joining form
+constexpr int kMinUnits = 1;     // units per stream below which fewer streams run
+constexpr float kSlack = 8.f;    // log2 of the largest weight
+constexpr int kCluster = 8;      // CTAs that share an item of the joining form
 constexpr int kJoinKeys = 8192;  // keys up to which it is taken
 
+// A unit is kKeys keys of an item: K and V in kHalves blocks of 64 values a row,
+// each row 128 swizzled bytes.
 template <int D>
 struct Ring {
-    static constexpr int kWarps = D > 128 ? 4 : 8;
-    static constexpr int kStages = D == 64 ? 5 : D == 96 ? 4 : 3;
-    static constexpr int kStride = D + 8;
-    static constexpr int kHalf = kKeys * kStride;  // elements of K (and of V) in a stage
-    static constexpr size_t kBytes = static_cast<size_t>(kWarps) * kStages * 2 * kHalf * sizeof(uint16_t);
+    static constexpr int kKeys = D > 128 ? 16 : 32;
+    static constexpr int kWarps = D == 64 ? 8 : 4;
+    static constexpr int kStages = 3;
+    static constexpr int kHalves = (D + 63) / 64;
+    static constexpr int kBlock = kKeys * 128;         // bytes of 64 values of every key
+    static constexpr int kStage = 2 * kHalves * kBlock;  // K, then V
+    static constexpr int kWarpBytes = kStages * kStage;
+    static constexpr int kBytes = kWarps * kWarpBytes + 1024;  // 1024: alignment
+};
+
+struct StreamArgs {
+    SplitArgs g;
+    CUtensorMap k, v;
+    int box_tokens;  // tokens per TMA box: a block, or a unit of one
 };
 
 // Walks the units of a stream.
@@ -44,13 +55,13 @@ struct Cursor {
     Request rq;
     Work w;
 
-    template <int R>
+    template <int R, int kKeys>
     __device__ __forceinline__ void enter(const AttnArgs& a) {
         rq = read_request(a, b);
         w = request_work<kKeys>(a, rq, R);
     }
     // The next unit (there is one).
-    template <int R>
+    template <int R, int kKeys>
     __device__ __forceinline__ void next(const AttnArgs& a) {
         if (++unit < w.units) return;
         unit = 0;
@@ -60,7 +71,7 @@ struct Cursor {
         kvh = 0;
         do {
             ++b;
-            enter<R>(a);
+            enter<R, kKeys>(a);
         } while (!w.rows);
     }
 };
@@ -77,10 +88,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // rows r, r + kCluster, ...).
 template <int D, int R, int kWarps, int kRingBytes>
 __device__ __forceinline__ void cluster_join(const AttnArgs& a, const Request& rq, int kvh, int tile, int rows,
-                                             uint16_t* smem) {
+                                             uint8_t* smem) {
     constexpr int kThreads = kWarps * 32, kEach = R * D / kThreads;
     const int tid = threadIdx.x, rank = static_cast<int>(blockIdx.x) % kCluster;
-    auto part = [&](int w) { return reinterpret_cast<float*>(reinterpret_cast<char*>(smem) + static_cast<size_t>(w) * kRingBytes); };
+    auto part = [&](int w) { return reinterpret_cast<float*>(smem + static_cast<size_t>(w) * kRingBytes); };
     __syncthreads();
     float o[kEach], top[kEach], sum[kEach];
 #pragma unroll
@@ -135,7 +146,8 @@ __device__ __forceinline__ void cluster_join(const AttnArgs& a, const Request& r
         const int rr = tile * R + r, i = rr / a.group;
         store_one(a, rq.first + i, kvh * a.group + rr - i * a.group, col, all == 0.f ? 0.f : y / all);
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // until then the sums stay
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");           // before the next item's copies
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // until here the sums stay
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
@@ -143,15 +155,27 @@ __device__ __forceinline__ void cluster_join(const AttnArgs& a, const Request& r
 // further on), its warps equal runs of the item's units, and joins them in shared
 // memory: one launch and no workspace, for few items with few keys.
 template <typename T, int D, int NP, int NT, bool kJoin>
-__global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(const __grid_constant__ SplitArgs g) {
+__global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(const __grid_constant__ StreamArgs c) {
     using L = Ring<D>;
-    constexpr int R = 8 * NT, kThreads = L::kWarps * 32, kS = L::kStride, kSteps = D / 16;
-    extern __shared__ __align__(16) uint16_t smem[];
+    constexpr int R = 8 * NT, kThreads = L::kWarps * 32, kSteps = D / 16, kKeys = L::kKeys;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t full[L::kWarps][L::kStages];
+    __shared__ int dead_word;
+    volatile int* dead = &dead_word;
+    const SplitArgs& g = c.g;
+    uint8_t* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
     __shared__ long long before[kThreads + 1];  // units of the requests before each thread's
     __shared__ long long warp_units[L::kWarps];
     const AttnArgs& a = g.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.p.n_seqs;
+    if (tid == 0) {
+        dead_word = 0;
+        for (int i = 0; i < L::kWarps * L::kStages; ++i) bar_init(&full[0][0] + i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     grid_wait();
+    __syncthreads();
     if (!kJoin) grid_release();  // combine_kernel may take its place on the SMs; it waits for this grid's end
 
     Cursor at;
@@ -163,7 +187,7 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
         at.kvh = item % a.kv.kv_heads;
         at.tile = item / a.kv.kv_heads % g.tiles;
         at.b = item / a.kv.kv_heads / g.tiles;
-        at.enter<R>(a);
+        at.enter<R, kKeys>(a);
     } else {
     // units of all requests, summed up over the threads
     const int per = (B + kThreads - 1) / kThreads;
@@ -204,13 +228,13 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
         }
         long long u = before[lo];
         at.b = lo * per;
-        at.enter<R>(a);
+        at.enter<R, kKeys>(a);
         for (;;) {
             const long long n = static_cast<long long>(at.w.units) * at.w.tiles * a.kv.kv_heads;
             if (u0 < u + n) break;
             u += n;
             ++at.b;
-            at.enter<R>(a);
+            at.enter<R, kKeys>(a);
         }
         const long long item = (u0 - u) / at.w.units;
         at.unit = static_cast<int>(u0 - u - item * at.w.units);
@@ -219,6 +243,8 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
         item0 = u0 - at.unit;
     }
     }
+    const uint32_t ring = smem_addr(smem) + warp * L::kWarpBytes;
+    uint32_t fetched = 0, used = 0;  // units
     for (; !kJoin || at.tile < at.w.tiles; at.tile += g.tiles) {
     if constexpr (kJoin) {
         const int n = at.w.units, i = warp * kCluster + static_cast<int>(blockIdx.x) % kCluster;
@@ -228,56 +254,59 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
     }
     int todo = left;  // units to work off
 
-    // the ring: `fetch` runs ahead of `at`
-    uint16_t* ring = smem + static_cast<size_t>(warp) * L::kStages * 2 * L::kHalf;
+    // the ring: `fetch` runs ahead of `at`; lane i < boxes loads box i of a unit
     Cursor fetch = at;
-    // the table entry of a unit's block, not looked at before the unit is loaded
-    auto block_of = [&](const Cursor& c) {
-        const int j0 = c.w.lo + c.unit * kKeys;
-        return j0 < c.w.hi ? __ldg(a.p.block_table + static_cast<int64_t>(c.b) * a.p.table_width + (j0 >> a.log_bs)) : -1;
+    const int boxes = kKeys / c.box_tokens;
+    // the table entry of a box's block, not looked at before the unit is loaded
+    auto block_of = [&](const Cursor& f) {
+        const int j = f.w.lo + f.unit * kKeys + lane * c.box_tokens, page = j >> a.log_bs;
+        return lane < boxes && j < f.w.hi ? __ldg(a.p.block_table + static_cast<int64_t>(f.b) * a.p.table_width + page) : 0;
     };
-    int id = block_of(fetch), fill = 0;
+    int id = block_of(fetch);
     auto load = [&]() {
         if (left > 0) {
-            const int j0 = fetch.w.lo + fetch.unit * kKeys;
-            const bool known = id >= 0 && id < a.kv.num_blocks;
-            const int n = known ? fetch.w.hi - j0 : 0;  // keys of the unit that exist
-            const int64_t base = !known ? 0
-                                        : id * a.kv.nb_block + fetch.kvh * a.kv.nb_head +
-                                              (j0 & (a.kv.block_size - 1)) * a.kv.nb_token;
-            uint16_t* to = ring + fill * 2 * L::kHalf;
-            constexpr int kChunks = D / 8;
+            const int j = fetch.w.lo + fetch.unit * kKeys + lane * c.box_tokens;
+            const bool on = lane < boxes && j < fetch.w.hi;
+            const int stage = fetched % L::kStages;
+            uint64_t* bar = &full[warp][stage];
+            const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, on)) * c.box_tokens * 128 * 2 * L::kHalves;
+            if (lane == 0) bar_expect(bar, bytes);
+            __syncwarp();
+            if (on) {
+                // a block outside the cache: behind the last one, zeros
+                const int block = id >= 0 && id < a.kv.num_blocks ? id : static_cast<int>(a.kv.num_blocks);
+                const uint32_t to = ring + stage * L::kStage + lane * c.box_tokens * 128;
 #pragma unroll
-            for (int i = 0; i < kKeys * kChunks / 32; ++i) {
-                const int x = i * 32 + lane, r = x / kChunks, c = x - r * kChunks;
-                const int bytes = r < n ? 16 : 0;  // 0: fills with zeros
-                const int64_t from = r < n ? base + r * a.kv.nb_token + c * 16 : 0;
-                const uint32_t d = smem_addr(to + r * kS + c * 8);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d),
-                             "l"(static_cast<const char*>(a.kv.k) + from), "r"(bytes)
-                             : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + L::kHalf * 2),
-                             "l"(static_cast<const char*>(a.kv.v) + from), "r"(bytes)
-                             : "memory");
+                for (int h = 0; h < L::kHalves; ++h) {
+                    tma_box(to + h * L::kBlock, &c.k, bar, h * 64, j & (a.kv.block_size - 1), fetch.kvh, block);
+                    tma_box(to + (L::kHalves + h) * L::kBlock, &c.v, bar, h * 64, j & (a.kv.block_size - 1), fetch.kvh,
+                            block);
+                }
             }
+            ++fetched;
             if (--left > 0) {
-                fetch.next<R>(a);
+                fetch.next<R, kKeys>(a);
                 id = block_of(fetch);
             }
-            fill = fill + 1 == L::kStages ? 0 : fill + 1;
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
     for (int i = 0; i < L::kStages - 1; ++i) load();
 
+    // Addresses of this lane's matrix rows: 16-byte column x of row r lies at
+    // column x ^ (r & 7) of it.
+    uint32_t k_at[4], v_at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        k_at[i] = (lane & 15) * 128 + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4);
+        v_at[i] = ((lane & 7) + ((lane >> 4) & 1) * 8) * 128 + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
+    }
     uint32_t qf[NP][NT][kSteps][2];
     float o[NT][kSteps][4], m[NT][2], l[NT][2], mul[NT][2], slope[NT][2];
     int pos[NT][2];
     int rows = 0, all_lo = 0, all_hi = 0;  // keys [all_lo, all_hi) are seen by every row
 
-    int stage = 0;
-    bool fresh = true, begun_here = at.unit == 0;
+    bool fresh = true, begun_here = at.unit == 0, ok = true;
     while (todo > 0) {
         if (fresh) {  // a new item: its queries, and nothing seen yet
             fresh = false;
@@ -339,97 +368,119 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
             all_lo = a.p.window > 0 && p1 >= a.p.window ? p1 - a.p.window + 1 : 0;
         }
         load();
-        asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 1) : "memory");
-        __syncwarp();
-        const uint16_t* kt = ring + stage * 2 * L::kHalf;
-        const uint16_t* vt = kt + L::kHalf;
+        const uint32_t stage = used % L::kStages, kt = ring + stage * L::kStage, vt = kt + L::kHalves * L::kBlock;
+        ok = bar_wait(&full[warp][stage], (used / L::kStages) & 1, dead);
+        if (!ok) break;
+        ++used;
+        const int j0 = at.w.lo + at.unit * kKeys, exist = at.w.hi - j0;
+        if (exist < kKeys) {  // values of keys that do not exist: a weight of 0 would not hide a NaN
+            for (int x = lane; x < (kKeys - max(exist, 0)) * 8 * L::kHalves; x += 32) {
+                const int r = max(exist, 0) + x / (8 * L::kHalves), col = x % (8 * L::kHalves);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (col >> 3) * L::kBlock + r * 128 +
+                                                                             (col & 7) * 16),
+                             "r"(0)
+                             : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into the stage
+            __syncwarp();
+        }
 
-        // scores: two chains of matrix instructions, joined by an addition
-        float s[NT][2][4];
+        // scores: two chains of matrix instructions per 16 keys, joined by an addition
+        float s[kKeys / 16][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int kb = 0; kb < kKeys / 16; ++kb) {
+            float t[NT][2][4] = {};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][0][e] = s[nt][1][e] = 0.f;
+            for (int k = 0; k < kSteps; ++k) {
+                uint32_t kf[4];
+                ldsm4(kf, kt + (k >> 2) * L::kBlock + kb * 2048 + k_at[k & 3]);
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            uint32_t kf[4];
-            ldsm4(kf, smem_addr(kt + (lane & 15) * kS + k * 16 + (lane >> 4) * 8));
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = NP - 1; i >= 0; --i) mma16816<T>(t[nt][k & 1], kf, qf[i][nt][k][0], qf[i][nt][k][1]);
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int c = NP - 1; c >= 0; --c) mma16816<T>(s[nt][k & 1], kf, qf[c][nt][k][0], qf[c][nt][k][1]);
+                for (int e = 0; e < 4; ++e) s[kb][nt][e] = t[nt][0][e] + t[nt][1][e];
         }
-        const int j0 = at.w.lo + at.unit * kKeys;
         const bool whole = j0 >= all_lo && j0 + kKeys <= all_hi;
         bool higher = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int kb = 0; kb < kKeys / 16; ++kb)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int q = e & 1, j = j0 + (lane >> 2) + 8 * (e >> 1);
-                float x = (s[nt][0][e] + s[nt][1][e]) * mul[nt][q];
-                if (a.post != 0.f) x = a.post * tanhf(x);
-                if (a.bias_near) x = fmaf(slope[nt][q], static_cast<float>(j - pos[nt][q]), x);
-                if (!whole && (j > min(pos[nt][q], at.w.hi - 1) || (a.p.window > 0 && pos[nt][q] - j >= a.p.window)))
-                    x = -INFINITY;
-                s[nt][0][e] = x;
-                higher |= x > m[nt][q] + kSlack;
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int q = e & 1, j = j0 + kb * 16 + (lane >> 2) + 8 * (e >> 1);
+                    float x = s[kb][nt][e] * mul[nt][q];
+                    if (a.post != 0.f) x = a.post * tanhf(x);
+                    if (a.bias_near) x = fmaf(slope[nt][q], static_cast<float>(j - pos[nt][q]), x);
+                    if (!whole && (j > min(pos[nt][q], at.w.hi - 1) || (a.p.window > 0 && pos[nt][q] - j >= a.p.window)))
+                        x = -INFINITY;
+                    s[kb][nt][e] = x;
+                    higher |= x > m[nt][q] + kSlack;
+                }
         if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    float top = fmaxf(s[nt][0][q], s[nt][0][2 + q]);
+                    float top = m[nt][q];
+#pragma unroll
+                    for (int kb = 0; kb < kKeys / 16; ++kb) top = fmaxf(top, fmaxf(s[kb][nt][q], s[kb][nt][2 + q]));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    top = fmaxf(top, m[nt][q]);
-                    const float c = top == -INFINITY ? 1.f : exp2f(m[nt][q] - top);
+                    const float f = top == -INFINITY ? 1.f : exp2f(m[nt][q] - top);
                     m[nt][q] = top;
-                    l[nt][q] *= c;
+                    l[nt][q] *= f;
 #pragma unroll
-                    for (int n = 0; n < kSteps; ++n) o[nt][n][q] *= c, o[nt][n][2 + q] *= c;
+                    for (int n = 0; n < kSteps; ++n) o[nt][n][q] *= f, o[nt][n][2 + q] *= f;
                 }
         }
-        uint32_t pf[NP][NT][2];
+        uint32_t pf[kKeys / 16][NP][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            const float base[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0], m[nt][1] == -INFINITY ? 0.f : m[nt][1]};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float base = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
-                s[nt][0][e] = exp2f(s[nt][0][e] - base);
-                l[nt][e & 1] += s[nt][0][e];
-            }
+            for (int kb = 0; kb < kKeys / 16; ++kb) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {  // keys 0-7, then 8-15
-                uint32_t piece[NP];
-                split_pair<T, NP>(s[nt][0][2 * e], s[nt][0][2 * e + 1], piece);
+                for (int e = 0; e < 4; ++e) {
+                    s[kb][nt][e] = exp2f(s[kb][nt][e] - base[e & 1]);
+                    l[nt][e & 1] += s[kb][nt][e];
+                }
 #pragma unroll
-                for (int c = 0; c < NP; ++c) pf[c][nt][e] = transpose8x8(piece[c]);
+                for (int e = 0; e < 2; ++e) {  // keys 0-7, then 8-15
+                    uint32_t piece[NP];
+                    split_pair<T, NP>(s[kb][nt][2 * e], s[kb][nt][2 * e + 1], piece);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) pf[kb][i][nt][e] = transpose8x8(piece[i]);
+                }
             }
         }
 #pragma unroll
         for (int n = 0; n < kSteps; ++n) {
-            uint32_t vf[4];
-            ldsm4_t(vf, smem_addr(vt + ((lane & 7) + ((lane >> 4) & 1) * 8) * kS + n * 16 + ((lane >> 3) & 1) * 8));
+            // the matrix unit cuts its sums off: with F32 queries every unit's sum starts
+            // at 0 and is added by a rounded addition, or a long axis would show it
+            float t[NT][4] = {};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                if (NP == 1) {
-                    mma16816<T>(o[nt][n], vf, pf[0][nt][0], pf[0][nt][1]);
-                } else {
-                    // the matrix unit cuts its sums off: every unit's sum starts at 0 and
-                    // is added by a rounded addition, or a long axis would show it
-                    float t[4] = {};
+            for (int kb = 0; kb < kKeys / 16; ++kb) {
+                uint32_t vf[4];
+                ldsm4_t(vf, vt + (n >> 2) * L::kBlock + kb * 2048 + v_at[n & 3]);
 #pragma unroll
-                    for (int c = NP - 1; c >= 0; --c) mma16816<T>(t, vf, pf[c][nt][0], pf[c][nt][1]);
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[nt][n][e] += t[e];
-                }
+                    for (int i = NP - 1; i >= 0; --i)
+                        mma16816<T>(NP > 1 ? t[nt] : o[nt][n], vf, pf[kb][i][nt][0], pf[kb][i][nt][1]);
             }
+            if (NP > 1)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][n][e] += t[nt][e];
         }
         __syncwarp();  // every lane has read the stage
-        stage = stage + 1 == L::kStages ? 0 : stage + 1;
         --todo;
         const bool ends = at.unit + 1 == at.w.units;
         if constexpr (kJoin) {
@@ -482,17 +533,18 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
         }
         if (todo > 0) {
             item0 += at.w.units;
-            at.next<R>(a);
+            at.next<R, kKeys>(a);
             fresh = begun_here = true;
         }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!ok)  // copies in flight land before the CTA ends
+        for (; used < fetched; ++used) bar_wait(&full[warp][used % L::kStages], (used / L::kStages) & 1, nullptr);
     if constexpr (!kJoin) {
         break;
     } else {
         // this warp's sums to the start of its ring (all of it has been read)
         __syncwarp();
-        float* to = reinterpret_cast<float*>(ring);
+        float* to = reinterpret_cast<float*>(smem + warp * L::kWarpBytes);
         const bool any = at.w.units > 0 && !fresh;
         const int r0 = at.tile * R;
         rows = min(R, at.w.rows - r0);
@@ -516,7 +568,7 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
                     to[R * D + R + r] = sum;
                 }
             }
-        cluster_join<D, R, L::kWarps, L::kStages * 2 * L::kHalf * 2>(a, at.rq, at.kvh, at.tile, rows, smem);
+        cluster_join<D, R, L::kWarps, L::kWarpBytes>(a, at.rq, at.kvh, at.tile, rows, smem);
     }
     }
 }
@@ -541,13 +593,13 @@ Items count_items(const AttnArgs& a, int R) {
 }
 
 template <typename T, int D, int NP, int NT, bool kJoin>
-cudaError_t launch_form(const SplitArgs& g, int ctas, cudaStream_t stream) {
+cudaError_t launch_form(const StreamArgs& c, int ctas, cudaStream_t stream) {
     using L = Ring<D>;
     const auto kernel = attn_stream_kernel<T, D, NP, NT, kJoin>;
     const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L::kBytes));
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, dim3(ctas), dim3(L::kWarps * 32), L::kBytes, stream, kJoin ? kCluster : 1, g);
+    return launch_pdl(kernel, dim3(ctas), dim3(L::kWarps * 32), L::kBytes, stream, kJoin ? kCluster : 1, c);
 }
 
 template <typename T, int D, int NP, int NT>
@@ -555,13 +607,18 @@ cudaError_t launch_rows(const AttnArgs& a, cudaStream_t stream) {
     using L = Ring<D>;
     const Items items = count_items(a, 8 * NT);
     const int sms = sm_count();
-    SplitArgs g = split_args(a, static_cast<size_t>(sms) * L::kWarps);
+    StreamArgs c;
+    SplitArgs& g = c.g;
+    g = split_args(a, static_cast<size_t>(sms) * L::kWarps);
+    c.box_tokens = std::min(a.kv.block_size, L::kKeys);
+    if (!cache_map(&c.k, a.kv, a.kv.k, c.box_tokens) || !cache_map(&c.v, a.kv, a.kv.v, c.box_tokens))
+        return cudaErrorInvalidValue;
     g.tiles = static_cast<int>(items.tiles);
-    if (items.join) return launch_form<T, D, NP, NT, true>(g, static_cast<int>(items.count) * kCluster, stream);
+    if (items.join) return launch_form<T, D, NP, NT, true>(c, static_cast<int>(items.count) * kCluster, stream);
     // no more streams than the hints give work for
-    const int64_t units = items.count * std::max(1, (a.p.max_kv + kKeys - 1) / kKeys);
+    const int64_t units = items.count * std::max(1, (a.p.max_kv + L::kKeys - 1) / L::kKeys);
     g.streams = static_cast<int>(std::min<int64_t>(sms * L::kWarps, std::max<int64_t>(1, units / kMinUnits)));
-    const cudaError_t e = launch_form<T, D, NP, NT, false>(g, std::min(sms, g.streams), stream);
+    const cudaError_t e = launch_form<T, D, NP, NT, false>(c, std::min(sms, g.streams), stream);
     if (e != cudaSuccess) return e;
     return combine_launch<D, 8 * NT>(g, items.count, stream);
 }
@@ -612,6 +669,8 @@ size_t stream_workspace(const AttnArgs& a) {
         default: return workspace_of<256>(R);
     }
 }
+
+cudaError_t stream_error(int* out) { return take_wait_error(out); }
 
 cudaError_t stream_launch(const AttnArgs& a, cudaStream_t stream) {
     return a.kv.type == GGML_TYPE_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream);
