@@ -27,15 +27,16 @@ namespace {
 constexpr int kMinUnits = 1;     // units per stream below which fewer streams run
 constexpr float kSlack = 8.f;    // log2 of the largest weight
 constexpr int kCluster = 8;      // CTAs that share an item of the joining form
-constexpr int kJoinKeys = 8192;  // keys up to which it is taken
+constexpr int kJoinKeys = 16384;  // keys up to which it is taken
 
 // A unit is kKeys keys of an item: K and V in kHalves blocks of 64 values a row,
 // each row 128 swizzled bytes.
 template <int D>
 struct Ring {
     static constexpr int kKeys = D > 128 ? 16 : 32;
-    static constexpr int kWarps = D == 64 ? 8 : 4;
-    static constexpr int kStages = 3;
+    static constexpr int kWarps = 4;  // streams; as many warps more load for them
+    static constexpr int kThreads = kWarps * 64;
+    static constexpr int kStages = D == 64 ? 6 : 3;
     static constexpr int kHalves = (D + 63) / 64;
     static constexpr int kBlock = kKeys * 128;         // bytes of 64 values of every key
     static constexpr int kStage = 2 * kHalves * kBlock;  // K, then V
@@ -86,10 +87,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // the start of each warp's ring, and writes the item's rows: first the warps of
 // each CTA, then the CTAs' sums over distributed shared memory (rank r writes the
 // rows r, r + kCluster, ...).
-template <int D, int R, int kWarps, int kRingBytes>
+template <int D, int R, int kThreads, int kWarps, int kRingBytes>
 __device__ __forceinline__ void cluster_join(const AttnArgs& a, const Request& rq, int kvh, int tile, int rows,
                                              uint8_t* smem) {
-    constexpr int kThreads = kWarps * 32, kEach = R * D / kThreads;
+    constexpr int kEach = R * D / kThreads;
     const int tid = threadIdx.x, rank = static_cast<int>(blockIdx.x) % kCluster;
     auto part = [&](int w) { return reinterpret_cast<float*>(smem + static_cast<size_t>(w) * kRingBytes); };
     __syncthreads();
@@ -155,22 +156,24 @@ __device__ __forceinline__ void cluster_join(const AttnArgs& a, const Request& r
 // further on), its warps equal runs of the item's units, and joins them in shared
 // memory: one launch and no workspace, for few items with few keys.
 template <typename T, int D, int NP, int NT, bool kJoin>
-__global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(const __grid_constant__ StreamArgs c) {
+__global__ void __launch_bounds__(Ring<D>::kThreads, 1) attn_stream_kernel(const __grid_constant__ StreamArgs c) {
     using L = Ring<D>;
-    constexpr int R = 8 * NT, kThreads = L::kWarps * 32, kSteps = D / 16, kKeys = L::kKeys;
+    constexpr int R = 8 * NT, kThreads = L::kThreads, kSteps = D / 16, kKeys = L::kKeys;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t full[L::kWarps][L::kStages];
+    __shared__ uint64_t full[L::kWarps][L::kStages], empty[L::kWarps][L::kStages];
     __shared__ int dead_word;
     volatile int* dead = &dead_word;
     const SplitArgs& g = c.g;
     uint8_t* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
     __shared__ long long before[kThreads + 1];  // units of the requests before each thread's
-    __shared__ long long warp_units[L::kWarps];
+    __shared__ long long warp_units[kThreads / 32];
     const AttnArgs& a = g.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.p.n_seqs;
+    const int own = warp % L::kWarps;  // the stream of this CTA that the warp loads for or works on
+    const bool loads = warp >= L::kWarps;
     if (tid == 0) {
         dead_word = 0;
-        for (int i = 0; i < L::kWarps * L::kStages; ++i) bar_init(&full[0][0] + i, 1);
+        for (int i = 0; i < L::kWarps * L::kStages; ++i) bar_init(&full[0][0] + i, 1), bar_init(&empty[0][0] + i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -213,8 +216,8 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
     all = before[kThreads];
     streams = min(static_cast<long long>(g.streams), max(1LL, all / kMinUnits));
     // neighbouring streams lie on different SMs: a short run of units uses all of them
-    me = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
-    if (lane == 0 && me < g.streams) g.heads[me].parts = 0;
+    me = static_cast<long long>(own) * gridDim.x + blockIdx.x;
+    if (lane == 0 && !loads && me < g.streams) g.heads[me].parts = 0;
     if (me >= streams || all == 0) return;
     const long long u0 = all * me / streams, u1 = all * (me + 1) / streams;
     left = static_cast<int>(u1 - u0);
@@ -243,55 +246,61 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
         item0 = u0 - at.unit;
     }
     }
-    const uint32_t ring = smem_addr(smem) + warp * L::kWarpBytes;
-    uint32_t fetched = 0, used = 0;  // units
+    const uint32_t ring = smem_addr(smem) + own * L::kWarpBytes;
+    uint32_t done = 0;  // units loaded, or worked off, by this warp
     for (; !kJoin || at.tile < at.w.tiles; at.tile += g.tiles) {
     if constexpr (kJoin) {
-        const int n = at.w.units, i = warp * kCluster + static_cast<int>(blockIdx.x) % kCluster;
+        const int n = at.w.units, i = own * kCluster + static_cast<int>(blockIdx.x) % kCluster;
         constexpr int kAll = kCluster * L::kWarps;
         at.unit = static_cast<int>(static_cast<long long>(n) * i / kAll);
         left = static_cast<int>(static_cast<long long>(n) * (i + 1) / kAll) - at.unit;
     }
-    int todo = left;  // units to work off
+    bool fresh = true;  // no unit of the item worked off yet
 
-    // the ring: `fetch` runs ahead of `at`; lane i < boxes loads box i of a unit
-    Cursor fetch = at;
-    const int boxes = kKeys / c.box_tokens;
-    // the table entry of a box's block, not looked at before the unit is loaded
-    auto block_of = [&](const Cursor& f) {
-        const int j = f.w.lo + f.unit * kKeys + lane * c.box_tokens, page = j >> a.log_bs;
-        return lane < boxes && j < f.w.hi ? __ldg(a.p.block_table + static_cast<int64_t>(f.b) * a.p.table_width + page) : 0;
-    };
-    int id = block_of(fetch);
-    auto load = [&]() {
-        if (left > 0) {
-            const int j = fetch.w.lo + fetch.unit * kKeys + lane * c.box_tokens;
+    // ------------------------------------------------------------------- loads
+    if (loads) {
+        const int boxes = kKeys / c.box_tokens;  // lane i < boxes loads box i of a unit
+        // the table entry of a box's block, not looked at before the unit is loaded
+        auto block_of = [&](const Cursor& f) {
+            const int j = f.w.lo + f.unit * kKeys + lane * c.box_tokens, page = j >> a.log_bs;
+            return lane < boxes && j < f.w.hi ? __ldg(a.p.block_table + static_cast<int64_t>(f.b) * a.p.table_width + page)
+                                              : 0;
+        };
+        Cursor fetch = at;
+        int id = block_of(fetch);
+        bool ok = true;
+        for (int todo = left; todo > 0; ++done) {
+            const int j = fetch.w.lo + fetch.unit * kKeys + lane * c.box_tokens, kvh = fetch.kvh;
             const bool on = lane < boxes && j < fetch.w.hi;
-            const int stage = fetched % L::kStages;
-            uint64_t* bar = &full[warp][stage];
+            // a block outside the cache: behind the last one, zeros
+            const int block = id >= 0 && id < a.kv.num_blocks ? id : static_cast<int>(a.kv.num_blocks);
+            if (--todo > 0) {
+                fetch.next<R, kKeys>(a);
+                id = block_of(fetch);
+            }
+            const uint32_t stage = done % L::kStages;
+            if (done >= L::kStages) ok = bar_wait(&empty[own][stage], ((done / L::kStages) & 1) ^ 1, dead);
+            if (!ok) break;
+            uint64_t* bar = &full[own][stage];
             const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, on)) * c.box_tokens * 128 * 2 * L::kHalves;
             if (lane == 0) bar_expect(bar, bytes);
             __syncwarp();
             if (on) {
-                // a block outside the cache: behind the last one, zeros
-                const int block = id >= 0 && id < a.kv.num_blocks ? id : static_cast<int>(a.kv.num_blocks);
                 const uint32_t to = ring + stage * L::kStage + lane * c.box_tokens * 128;
 #pragma unroll
-                for (int h = 0; h < L::kHalves; ++h) {
-                    tma_box(to + h * L::kBlock, &c.k, bar, h * 64, j & (a.kv.block_size - 1), fetch.kvh, block);
-                    tma_box(to + (L::kHalves + h) * L::kBlock, &c.v, bar, h * 64, j & (a.kv.block_size - 1), fetch.kvh,
-                            block);
-                }
-            }
-            ++fetched;
-            if (--left > 0) {
-                fetch.next<R, kKeys>(a);
-                id = block_of(fetch);
-            }
-        }
-    };
+                for (int h = 0; h < L::kHalves; ++h)
+                    tma_box(to + h * L::kBlock, &c.k, bar, h * 64, j & (a.kv.block_size - 1), kvh, block);
 #pragma unroll
-    for (int i = 0; i < L::kStages - 1; ++i) load();
+                for (int h = 0; h < L::kHalves; ++h)
+                    tma_box(to + (L::kHalves + h) * L::kBlock, &c.v, bar, h * 64, j & (a.kv.block_size - 1), kvh, block);
+            }
+            __syncwarp();
+        }
+        if (!ok)  // copies in flight land before the CTA ends
+            for (uint32_t i = done < L::kStages ? 0 : done - L::kStages; i < done; ++i)
+                bar_wait(&full[own][i % L::kStages], (i / L::kStages) & 1, nullptr);
+        if constexpr (!kJoin) return;
+    }
 
     // Addresses of this lane's matrix rows: 16-byte column x of row r lies at
     // column x ^ (r & 7) of it.
@@ -306,7 +315,8 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
     int pos[NT][2];
     int rows = 0, all_lo = 0, all_hi = 0;  // keys [all_lo, all_hi) are seen by every row
 
-    bool fresh = true, begun_here = at.unit == 0, ok = true;
+    bool begun_here = at.unit == 0, ok = true;
+    int todo = loads ? 0 : left;  // units to work off
     while (todo > 0) {
         if (fresh) {  // a new item: its queries, and nothing seen yet
             fresh = false;
@@ -367,11 +377,10 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
             all_hi = min(p0 + 1, at.w.hi);
             all_lo = a.p.window > 0 && p1 >= a.p.window ? p1 - a.p.window + 1 : 0;
         }
-        load();
-        const uint32_t stage = used % L::kStages, kt = ring + stage * L::kStage, vt = kt + L::kHalves * L::kBlock;
-        ok = bar_wait(&full[warp][stage], (used / L::kStages) & 1, dead);
+        const uint32_t stage = done % L::kStages, kt = ring + stage * L::kStage, vt = kt + L::kHalves * L::kBlock;
+        ok = bar_wait(&full[own][stage], (done / L::kStages) & 1, dead);
         if (!ok) break;
-        ++used;
+        ++done;
         const int j0 = at.w.lo + at.unit * kKeys, exist = at.w.hi - j0;
         if (exist < kKeys) {  // values of keys that do not exist: a weight of 0 would not hide a NaN
             for (int x = lane; x < (kKeys - max(exist, 0)) * 8 * L::kHalves; x += 32) {
@@ -481,6 +490,7 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
                     for (int e = 0; e < 4; ++e) o[nt][n][e] += t[nt][e];
         }
         __syncwarp();  // every lane has read the stage
+        if (lane == 0) bar_arrive(&empty[own][stage]);
         --todo;
         const bool ends = at.unit + 1 == at.w.units;
         if constexpr (kJoin) {
@@ -537,17 +547,16 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
             fresh = begun_here = true;
         }
     }
-    if (!ok)  // copies in flight land before the CTA ends
-        for (; used < fetched; ++used) bar_wait(&full[warp][used % L::kStages], (used / L::kStages) & 1, nullptr);
     if constexpr (!kJoin) {
         break;
     } else {
         // this warp's sums to the start of its ring (all of it has been read)
         __syncwarp();
-        float* to = reinterpret_cast<float*>(smem + warp * L::kWarpBytes);
+        float* to = reinterpret_cast<float*>(smem + own * L::kWarpBytes);
         const bool any = at.w.units > 0 && !fresh;
         const int r0 = at.tile * R;
         rows = min(R, at.w.rows - r0);
+        if (!loads)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -568,7 +577,7 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_stream_kernel(co
                     to[R * D + R + r] = sum;
                 }
             }
-        cluster_join<D, R, L::kWarps, L::kWarpBytes>(a, at.rq, at.kvh, at.tile, rows, smem);
+        cluster_join<D, R, kThreads, L::kWarps, L::kWarpBytes>(a, at.rq, at.kvh, at.tile, rows, smem);
     }
     }
 }
@@ -599,7 +608,7 @@ cudaError_t launch_form(const StreamArgs& c, int ctas, cudaStream_t stream) {
     const cudaError_t e =
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, dim3(ctas), dim3(L::kWarps * 32), L::kBytes, stream, kJoin ? kCluster : 1, c);
+    return launch_pdl(kernel, dim3(ctas), dim3(L::kThreads), L::kBytes, stream, kJoin ? kCluster : 1, c);
 }
 
 template <typename T, int D, int NP, int NT>
