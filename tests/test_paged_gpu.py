@@ -89,7 +89,8 @@ def lens_of(B, most_cached, most_new, seed):
 
 @pytest.mark.parametrize("B,most_cached,most_new,bs,pad", [
     (1, 0, 1, 16, 0), (1, 31, 5, 16, 0), (3, 64, 1, 32, 2), (33, 100, 40, 16, 7), (1024, 300, 1, 64, 0),
-    (1025, 50, 3, 256, 100), (7, 0, 1000, 128, 0), (300, 17, 33, 16, 2000)])
+    (1025, 50, 3, 256, 100), (7, 0, 1000, 128, 0), (300, 17, 33, 16, 2000),
+    (20, 100, 3000, 32, 500), (900, 50, 60, 16, 3)])
 def test_kv_plan(cuda, G, B, most_cached, most_new, bs, pad):
     cached, new = lens_of(B, most_cached, most_new, B + bs)
     if B == 1:

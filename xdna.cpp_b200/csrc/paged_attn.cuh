@@ -12,9 +12,6 @@
 
 namespace xb {
 
-// Streaming multiprocessors of the current device (0 without one).
-int sm_count();
-
 struct AttnArgs {
     struct b200_paged_attention_args p;
     struct b200_kv_cache kv;
