@@ -8,7 +8,9 @@
 // one request and KV head.  Per tile of keys: S = Q K^T into TMEM, weights
 // P = 2^(s - m) back into TMEM over S in 16 bits, O += P V in TMEM.  Roles:
 //   4 warps per query tile   one row per thread: softmax, rescaling and output
-//   one warp                 issues the matrix instructions
+//   one warp per query tile  issues its matrix instructions (one warp for both was
+//                            the bound: its waits and issues in a row took longer
+//                            than the matrix unit)
 //   one warp                 TMA loads of K and V, page by page, into a ring
 // While one query tile is in its softmax the matrix unit works on the other
 // one.  O is rescaled only when a row's maximum grows by more than 8 (weights
@@ -39,6 +41,7 @@ namespace {
 constexpr int kKeys = 128;
 constexpr int kMinTiles = 2;   // key tiles per CTA below which fewer CTAs run
 constexpr float kSlack = 8.f;  // log2 of the largest weight
+constexpr int kTurnClocks = 4000;  // longest wait for a turn (a courtesy: nothing depends on it)
 
 template <int D>
 struct Shape {
@@ -47,11 +50,7 @@ struct Shape {
     static constexpr int kHalves = (D + 63) / 64;
     static constexpr int kStages = D == 64 ? 4 : D <= 128 ? 2 : 1;
     static constexpr int kTile = kHalves * 128 * 128;  // bytes of 128 rows
-    // 12 warps: the last two only make up the fourth group of registers, so that
-    // the softmax warps can take registers from the others
-    static constexpr int kThreads = kQ == 2 ? 384 : 192;
-    static constexpr int kLaunchRegs = 168, kSoftmaxRegs = 224, kOtherRegs = 56;
-    static_assert(kQ == 1 || 256 * kSoftmaxRegs + 128 * kOtherRegs <= 384 * kLaunchRegs, "registers of the launch");
+    static constexpr int kThreads = kQ * 160 + 32;  // 4 softmax warps and a matrix warp per query tile, a loading warp
     static constexpr int kSmem = (kQ + 2 * kStages) * kTile + 1024;  // 1024: alignment
     static constexpr int kS = 0, kO = 256, kPitch = 128;             // TMEM columns of q's S and O: + 128 q
 };
@@ -65,7 +64,7 @@ struct ChunkArgs {
 // ------------------------------------------------------------------- barriers
 struct Bars {
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-    uint64_t qfull[2], sfull[2], pfull[2], ofull[2], drain;
+    uint64_t qfull[2], sfull[2], pfull[2][2], ofull[2], drain[2];  // pfull: a barrier for each half of the keys
 };
 
 // ------------------------------------------------------------ matrix unit, TMEM
@@ -104,7 +103,49 @@ __device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_mn_major
            (128u / 16) << 24;
 }
 
-__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for this thread's TMEM loads; the values go through it, so that nothing
+// that uses them is moved in front.
+__device__ __forceinline__ void tm_wait16(float* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
+                   "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tm_wait32(float* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
+                   "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(r[16]),
+                   "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]),
+                   "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+                 :
+                 : "memory");
+}
+// Two F32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
+        "fma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// True on one lane of a converged warp.  Branches on it, with addresses that are
+// the same on every lane, keep what a matrix instruction takes in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_ld32(uint32_t addr, float* r) {
     uint32_t* u = reinterpret_cast<uint32_t*>(r);
@@ -225,28 +266,31 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
     __shared__ long long warp_units[L::kThreads / 32];
     __shared__ uint32_t tmem_slot;
     __shared__ int dead_word;
+    __shared__ volatile int turns[8];  // key tiles whose weights a softmax warp has formed
     volatile int* dead = &dead_word;
     const AttnArgs& a = c.g.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.p.n_seqs;
-    constexpr int kMmaWarp = L::kQ * 4, kLoadWarp = kMmaWarp + 1;
+    constexpr int kLoadWarp = L::kQ * 4, kMmaWarp = kLoadWarp + 1;  // and kMmaWarp + 1 for the second query tile
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     const uint32_t qs = base, ks = qs + L::kQ * L::kTile, vs = ks + L::kStages * L::kTile;
 
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) {
             bar_init(&bars.kfull[i], 1);
-            bar_init(&bars.kempty[i], 1);
+            bar_init(&bars.kempty[i], L::kQ);
             bar_init(&bars.vfull[i], 1);
-            bar_init(&bars.vempty[i], 1);
+            bar_init(&bars.vempty[i], L::kQ);
         }
         for (int i = 0; i < 2; ++i) {
             bar_init(&bars.qfull[i], 128);
             bar_init(&bars.sfull[i], 1);
-            bar_init(&bars.pfull[i], 128);
+            bar_init(&bars.pfull[i][0], 4);
+            bar_init(&bars.pfull[i][1], 4);
             bar_init(&bars.ofull[i], 1);
+            bar_init(&bars.drain[i], 1);
         }
-        bar_init(&bars.drain, 1);
         dead_word = 0;
+        for (int i = 0; i < 8; ++i) turns[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -347,8 +391,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
             w.enter_item<R>(a, static_cast<int>(u0 - u));
         }
 
-        if (warp >= kMmaWarp) {
-        if constexpr (L::kQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegs));
+        if (warp >= kLoadWarp) {
         if (warp == kLoadWarp) {
             // ---------------------------------------------------------------- loads
             const int boxes = kKeys / c.box_tokens;  // per half; lane i issues box i
@@ -383,93 +426,88 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                     bar_wait(&bars.vfull[i % L::kStages], (i / L::kStages) & 1, nullptr);
                 }
             }
-        } else if (warp == kMmaWarp) {
+        } else if (warp < kMmaWarp + L::kQ) {
             // ----------------------------------------------------- matrix instructions
             constexpr uint32_t kIdescS = instruction<T>(kKeys, false), kIdescO = instruction<T>(D, true);
-            int n = 0;                         // tiles before the item's
-            uint32_t nq[2] = {0, 0}, np[2] = {0, 0};  // phases of qfull and pfull
+            const int q = uniform(warp) - kMmaWarp;
+            const uint32_t s_at = uniform(tmem) + L::kS + q * L::kPitch, o_at = uniform(tmem) + L::kO + q * L::kPitch;
+            const uint64_t q_op = operand(qs + q * L::kTile, 16), k_op = operand(ks, 16), v_op = operand(vs, 128 * 128);
+            uint32_t i = 0, nq = 0, np = 0;  // key tiles, phases of qfull and pfull
             bool ok = true;
             do {
-                int lo[2] = {0, 0}, hi[2] = {0, 0};
-                for (int q = 0; q < L::kQ; ++q) query_tiles(a, w, w.tile * R + q * 128, lo[q], hi[q]);
-                // step t: O of tile t - 1, then S of tile t, for each query tile in turn
-                for (int t = w.s0; t <= w.s1 && ok; ++t) {
-                    const int i = n + t - w.s0, ks_i = i % L::kStages, vs_i = (i + L::kStages - 1) % L::kStages;
-                    const bool score = t < w.s1, value = t > w.s0;
-                    if (value) {
-                        ok = bar_wait(&bars.vfull[vs_i], ((i - 1) / L::kStages) & 1, dead);
-                        const int gone = w.hi - (t - 1) * kKeys;  // keys of tile t - 1 that exist
-                        if (ok && gone < kKeys) {
-                            for (int x = lane; x < (kKeys - max(gone, 0)) * 8 * L::kHalves; x += 32) {
-                                const int row = max(gone, 0) + x / (8 * L::kHalves), col = x % (8 * L::kHalves);
-                                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
-                                                 vs + vs_i * L::kTile + (col >> 3) * 128 * 128 + row * 128 + (col & 7) * 16),
-                                             "r"(0)
-                                             : "memory");
+                int lo, hi;
+                query_tiles(a, w, w.tile * R + q * 128, lo, hi);
+                lo = uniform(lo), hi = uniform(hi);
+                const int s0 = uniform(w.s0), s1 = uniform(w.s1);
+                // step t: O of tile t - 1, then S of tile t
+                for (int t = s0; t <= s1 && ok; ++t, ++i) {
+                    if (t > s0) {
+                        const uint32_t stage = (i - 1) % L::kStages;
+                        ok = bar_wait(&bars.vfull[stage], ((i - 1) / L::kStages) & 1, dead);
+                        if (ok && t > lo && t <= hi) {
+                            const uint64_t v = v_op + (stage * L::kTile >> 4);
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                if (ok) ok = bar_wait(&bars.pfull[q][half], np & 1, dead);
+                                tc_after();
+                                if (ok && elect_one()) {
+#pragma unroll
+                                    for (int k = half * 4; k < half * 4 + 4; ++k)
+                                        mma_ts(o_at, s_at + k * 8, v + (k * 2048 >> 4), kIdescO, k > 0 || t - 1 > lo);
+                                    if (half == 1 && t == hi) tc_commit(&bars.ofull[q]);
+                                }
+                                __syncwarp();
                             }
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                            __syncwarp();
+                            ++np;
+                        } else if (ok && lane == 0) {
+                            bar_arrive(&bars.vempty[stage]);
                         }
                     }
-                    if (ok && score) ok = bar_wait(&bars.kfull[ks_i], (i / L::kStages) & 1, dead);
-#pragma unroll
-                    for (int q = 0; q < L::kQ; ++q) {
-                        const uint32_t s_at = tmem + L::kS + q * L::kPitch, o_at = tmem + L::kO + q * L::kPitch;
-                        if (ok && value && t - 1 >= lo[q] && t - 1 < hi[q]) {
-                            ok = bar_wait(&bars.pfull[q], np[q]++ & 1, dead);
+                    if (ok && t < s1) {
+                        const uint32_t stage = i % L::kStages;
+                        ok = bar_wait(&bars.kfull[stage], (i / L::kStages) & 1, dead);
+                        if (ok && t >= lo && t < hi) {
+                            if (t == lo) ok = bar_wait(&bars.qfull[q], nq++ & 1, dead);
                             tc_after();
-                            if (ok && lane == 0) {
-#pragma unroll
-                                for (int k = 0; k < kKeys / 16; ++k)
-                                    mma_ts(o_at, s_at + k * 8, operand(vs + vs_i * L::kTile + k * 2048, 128 * 128),
-                                           kIdescO, k > 0 || t - 1 > lo[q]);
-                                if (t == hi[q]) tc_commit(&bars.ofull[q]);
-                            }
-                            __syncwarp();
-                        }
-                        if (ok && score && t >= lo[q] && t < hi[q]) {
-                            if (t == lo[q]) ok = bar_wait(&bars.qfull[q], nq[q]++ & 1, dead);
-                            tc_after();
-                            if (ok && lane == 0) {
+                            const uint64_t k_at = k_op + (stage * L::kTile >> 4);
+                            if (ok && elect_one()) {
 #pragma unroll
                                 for (int k = 0; k < D / 16; ++k) {
-                                    const uint32_t off = (k >> 2) * 128 * 128 + (k & 3) * 32;
-                                    mma_ss(s_at, operand(qs + q * L::kTile + off, 16),
-                                           operand(ks + ks_i * L::kTile + off, 16), kIdescS, k > 0);
+                                    const uint32_t off = ((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4;
+                                    mma_ss(s_at, q_op + off, k_at + off, kIdescS, k > 0);
                                 }
                                 tc_commit(&bars.sfull[q]);
                             }
                             __syncwarp();
+                        } else if (ok && lane == 0) {
+                            bar_arrive(&bars.kempty[stage]);
                         }
                     }
-                    if (ok && lane == 0) {
-                        if (value) tc_commit(&bars.vempty[vs_i]);
-                        if (score) tc_commit(&bars.kempty[ks_i]);
-                    }
-                    __syncwarp();
                 }
-                n += w.s1 - w.s0;
+                --i;  // the last step has no tile of its own
             } while (ok && w.next<R>(a));
             if (!ok) {  // matrix instructions in flight end before TMEM is freed
-                if (lane == 0) tc_commit(&bars.drain);
+                if (elect_one()) tc_commit(&bars.drain[q]);
                 __syncwarp();
-                bar_wait(&bars.drain, 0, nullptr);
+                bar_wait(&bars.drain[q], 0, nullptr);
             }
         }
         } else {
             // ------------------------------------------------------------------ softmax
-            if constexpr (L::kQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));
             const int q = warp >> 2, row = tid - q * 128;
             const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
             const uint32_t s_at = tmem + lanes + L::kS + q * L::kPitch, o_at = tmem + lanes + L::kO + q * L::kPitch;
             const uint32_t q_at = qs + q * L::kTile + row * 128;
             uint32_t ns = 0, no = 0;  // phases of sfull and ofull
+            uint32_t n = 0;           // key tiles before the item's
+            int mine = 0, theirs = 0;  // key tiles of this and of the other query tile before the item's
             bool ok = true, first_item = true;
             do {
                 const int r0 = w.tile * R + q * 128, rr = r0 + row;
                 if (r0 < w.rows) {
-                    int lo, hi;
+                    int lo, hi, other_lo = 0, other_hi = 0;
                     query_tiles(a, w, r0, lo, hi);
+                    if (L::kQ == 2) query_tiles(a, w, w.tile * R + (q ^ 1) * 128, other_lo, other_hi);
                     const bool on = rr < w.rows;
                     const int token = (on ? rr : r0) / a.group, head = w.kvh * a.group + (on ? rr - token * a.group : 0);
                     const int pos = w.rq.pos0() + token;
@@ -502,30 +540,55 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             ok = bar_wait(&bars.sfull[q], ns++ & 1, dead);
                             if (!ok) break;
                             tc_after();
+                            // S is there, and so is O of the tile before: K and that tile's V are free
+                            if (row == 0) {
+                                const uint32_t x = n + t - w.s0;
+                                bar_arrive(&bars.kempty[x % L::kStages]);
+                                if (t > lo) bar_arrive(&bars.vempty[(x - 1) % L::kStages]);
+                            }
                             const int j0 = t * kKeys;
-                            float s[kKeys];
+                            const bool cut = j0 < all_lo || j0 + kKeys > all_hi, change = kGeneral || cut;
+                            const float pre = kGeneral ? 1.f : a.pre;
+                            const int k0 = first - j0, k1 = last - j0;
+                            float s0[32], s1[32];  // columns of S: one half worked on, the other on its way
+                            // First pass: the row's maximum, in eight chains.  Scores that the cap,
+                            // the bias or a hidden key change go back for the second pass.
+                            float tops[8];
 #pragma unroll
-                            for (int i = 0; i < kKeys / 32; ++i) tm_ld32(s_at + i * 32, s + i * 32);
-                            tm_wait_ld();
-                            float pre = a.pre;
-                            if (kGeneral) {
-                                pre = 1.f;
+                            for (int i = 0; i < 8; ++i) tops[i] = -INFINITY;
+                            auto look = [&](float (&s)[32], int col) {
+                                if (change) {
+                                    if (kGeneral)
 #pragma unroll
-                                for (int i = 0; i < kKeys; ++i) {
-                                    float x = s[i] * a.pre;
-                                    if (a.post != 0.f) x = a.post * tanhf(x);
-                                    s[i] = a.bias_near ? fmaf(slope, static_cast<float>(j0 + i - pos), x) : x;
+                                        for (int i = 0; i < 32; ++i) {
+                                            float x = s[i] * a.pre;
+                                            if (a.post != 0.f) x = a.post * tanhf(x);
+                                            s[i] = a.bias_near ? fmaf(slope, static_cast<float>(j0 + col + i - pos), x) : x;
+                                        }
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i)
+                                        if (i < k0 - col || i > k1 - col) s[i] = -INFINITY;
+                                    tm_st16(s_at + col, reinterpret_cast<const uint32_t*>(s));
+                                    tm_st16(s_at + col + 16, reinterpret_cast<const uint32_t*>(s + 16));
                                 }
-                            }
-                            if (j0 < all_lo || j0 + kKeys > all_hi) {
-                                const int c0 = first - j0, c1 = last - j0;
 #pragma unroll
-                                for (int i = 0; i < kKeys; ++i)
-                                    if (i < c0 || i > c1) s[i] = -INFINITY;
+                                for (int i = 0; i < 8; ++i)
+                                    tops[i] = fmaxf(tops[i], fmaxf(fmaxf(s[i], s[i + 8]), fmaxf(s[i + 16], s[i + 24])));
+                            };
+                            tm_ld32(s_at, s0);
+#pragma unroll 1
+                            for (int half = 0; half < 2; ++half) {
+                                tm_wait32(s0);
+                                tm_ld32(s_at + half * 64 + 32, s1);
+                                look(s0, half * 64);
+                                tm_wait32(s1);
+                                if (half == 0) tm_ld32(s_at + 64, s0);
+                                look(s1, half * 64 + 32);
                             }
-                            float top = s[0];
-#pragma unroll
-                            for (int i = 1; i < kKeys; ++i) top = fmaxf(top, s[i]);
+                            if (change) tm_wait_st();
+                            tm_ld32(s_at, s0);
+                            float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
+                                              fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
                             top *= pre;
                             if (__any_sync(0xffffffffu, top > m + kSlack)) {
                                 const float was = m;
@@ -533,40 +596,75 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                                 const float f = m == -INFINITY ? 1.f : exp2_fast(was - m);
                                 l *= f;
                                 if (t > lo) {
-#pragma unroll 2
+#pragma unroll 1
                                     for (int i = 0; i < D / 16; ++i) {
                                         float o[16];
                                         tm_ld16(o_at + i * 16, o);
-                                        tm_wait_ld();
+                                        tm_wait16(o);
 #pragma unroll
                                         for (int e = 0; e < 16; ++e) o[e] *= f;
                                         tm_st16(o_at + i * 16, reinterpret_cast<const uint32_t*>(o));
                                     }
                                 }
                             }
+                            if (j0 + kKeys > w.hi) {  // values of keys that do not exist: a weight of 0 would not hide a NaN
+                                const uint32_t x = n + t - w.s0, stage = x % L::kStages;
+                                ok = bar_wait(&bars.vfull[stage], (x / L::kStages) & 1, dead);
+                                if (!ok) break;
+                                const int gone = max(w.hi - j0, 0);
+                                for (int y = row; y < (kKeys - gone) * 8 * L::kHalves; y += 128)
+                                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                                     vs + stage * L::kTile + (y % (8 * L::kHalves) >> 3) * 128 * 128 +
+                                                     (gone + y / (8 * L::kHalves)) * 128 + (y & 7) * 16),
+                                                 "r"(0)
+                                                 : "memory");
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            }
                             const float off = m == -INFINITY ? 0.f : -m;
-                            float sum[4] = {};
-#pragma unroll
-                            for (int g = 0; g < kKeys / 32; ++g) {
+                            // The two query tiles' warps on a scheduler take turns in the exponentials,
+                            // so that the matrix unit has the other one's work meanwhile (left alone
+                            // they run in step, and the matrix unit waits for both).
+                            if (L::kQ == 2) {
+                                const int due = theirs + min(max(t + q - other_lo, 0), other_hi - other_lo);
+                                const long long since = clock64();
+                                while (turns[warp ^ 4] < due && clock64() - since < kTurnClocks) {}
+                                __syncwarp();
+                            }
+                            const float2 pre2 = make_float2(pre, pre), off2 = make_float2(off, off);
+                            // Second pass: the weights.
+                            float2 sum[4] = {};
+                            auto weigh = [&](const float (&s)[32], int col) {
                                 uint32_t p[16];
 #pragma unroll
                                 for (int i = 0; i < 16; ++i) {
-                                    const float x = exp2_fast(fmaf(s[g * 32 + 2 * i], pre, off));
-                                    const float y = exp2_fast(fmaf(s[g * 32 + 2 * i + 1], pre, off));
-                                    sum[2 * (i & 1)] += x;
-                                    sum[2 * (i & 1) + 1] += y;
-                                    p[i] = Half16<T>::pack(x, y);
+                                    float2 x = fma2(make_float2(s[2 * i], s[2 * i + 1]), pre2, off2);
+                                    x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                                    sum[i & 3] = add2(sum[i & 3], x);
+                                    p[i] = Half16<T>::pack(x.x, x.y);
                                 }
-                                tm_st16(s_at + g * 16, p);
+                                tm_st16(s_at + col / 2, p);
+                            };
+#pragma unroll 1
+                            for (int half = 0; half < 2; ++half) {
+                                tm_wait32(s0);
+                                tm_ld32(s_at + half * 64 + 32, s1);
+                                weigh(s0, half * 64);
+                                tm_wait32(s1);
+                                if (half == 0) tm_ld32(s_at + 64, s0);
+                                weigh(s1, half * 64 + 32);
+                                tm_wait_st();  // half of the weights: the matrix unit may take them
+                                tc_before();
+                                __syncwarp();
+                                if (lane == 0) bar_arrive(&bars.pfull[q][half]);
                             }
-                            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                            tm_wait_st();
-                            tc_before();
-                            bar_arrive(&bars.pfull[q]);
+                            if (L::kQ == 2 && lane == 0) turns[warp] = mine + t + 1 - lo;
+                            const float2 both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                            l += both.x + both.y;
                         }
                         if (ok) ok = bar_wait(&bars.ofull[q], no++ & 1, dead);
                         if (!ok) break;
                         tc_after();
+                        if (row == 0) bar_arrive(&bars.vempty[(n + hi - 1 - w.s0) % L::kStages]);
                     }
                     // O to the output, or to the item's partial
                     const bool whole = w.s0 == w.t0 && w.s1 == w.t1;
@@ -578,7 +676,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                         float o[32];
                         if (lo < hi) {
                             tm_ld32(o_at + i * 32, o);
-                            tm_wait_ld();
+                            tm_wait32(o);
                         }
 #pragma unroll
                         for (int e = 0; e < 32; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
@@ -613,6 +711,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                     c.g.heads[me] = SplitHead{w.b, w.kvh, w.tile, static_cast<int>(stream_of(end - 1, all, streams) - me + 1)};
                 }
                 first_item = false;
+                int lo, hi;
+                query_tiles(a, w, r0, lo, hi);
+                mine += hi - lo;
+                if (L::kQ == 2) query_tiles(a, w, w.tile * R + (q ^ 1) * 128, lo, hi);
+                theirs += hi - lo;
+                n += w.s1 - w.s0;
             } while (w.next<R>(a));
         }
     }

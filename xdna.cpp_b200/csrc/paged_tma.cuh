@@ -58,9 +58,13 @@ __device__ __forceinline__ bool bar_wait_slow(uint64_t* b, uint32_t parity, vola
         }
     }
 }
+// For one thread.
+__device__ __forceinline__ bool bar_wait_one(uint64_t* b, uint32_t parity, volatile int* dead) {
+    return bar_try(b, parity) || bar_try(b, parity) || bar_wait_slow(b, parity, dead);
+}
+// For a warp: it goes on, or gives up, as one.
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* dead) {
-    bool ok = bar_try(b, parity) || bar_try(b, parity) || bar_wait_slow(b, parity, dead);
-    return __all_sync(0xffffffffu, ok);  // the warp goes on, or gives up, as one
+    return __all_sync(0xffffffffu, bar_wait_one(b, parity, dead));
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place
