@@ -50,7 +50,11 @@ struct Shape {
     static constexpr int kHalves = (D + 63) / 64;
     static constexpr int kStages = D == 64 ? 4 : D <= 128 ? 2 : 1;
     static constexpr int kTile = kHalves * 128 * 128;  // bytes of 128 rows
-    static constexpr int kThreads = kQ * 160 + 32;  // 4 softmax warps and a matrix warp per query tile, a loading warp
+    // 4 softmax warps and a matrix warp per query tile, a loading warp; 12 warps, so
+    // that the softmax warps can take registers from a whole group of others
+    static constexpr int kThreads = kQ == 2 ? 384 : 192;
+    static constexpr int kLaunchRegs = 168, kSoftmaxRegs = 224, kOtherRegs = 56;
+    static_assert(kQ == 1 || 256 * kSoftmaxRegs + 128 * kOtherRegs <= 384 * kLaunchRegs, "registers of the launch");
     static constexpr int kSmem = (kQ + 2 * kStages) * kTile + 1024;  // 1024: alignment
     static constexpr int kS = 0, kO = 256, kPitch = 128;             // TMEM columns of q's S and O: + 128 q
 };
@@ -392,6 +396,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
         }
 
         if (warp >= kLoadWarp) {
+        if constexpr (L::kQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegs));
         if (warp == kLoadWarp) {
             // ---------------------------------------------------------------- loads
             const int boxes = kKeys / c.box_tokens;  // per half; lane i issues box i
@@ -494,6 +499,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
         }
         } else {
             // ------------------------------------------------------------------ softmax
+            if constexpr (L::kQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));
             const int q = warp >> 2, row = tid - q * 128;
             const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
             const uint32_t s_at = tmem + lanes + L::kS + q * L::kPitch, o_at = tmem + lanes + L::kO + q * L::kPitch;
@@ -547,46 +553,36 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                                 if (t > lo) bar_arrive(&bars.vempty[(x - 1) % L::kStages]);
                             }
                             const int j0 = t * kKeys;
-                            const bool cut = j0 < all_lo || j0 + kKeys > all_hi, change = kGeneral || cut;
+                            const bool cut = j0 < all_lo || j0 + kKeys > all_hi;
                             const float pre = kGeneral ? 1.f : a.pre;
                             const int k0 = first - j0, k1 = last - j0;
-                            float s0[32], s1[32];  // columns of S: one half worked on, the other on its way
-                            // First pass: the row's maximum, in eight chains.  Scores that the cap,
-                            // the bias or a hidden key change go back for the second pass.
+                            float s[kKeys];
+                            // the row's maximum, in eight chains, while the next columns are on their way
                             float tops[8];
+                            tm_ld32(s_at, s);
+                            tm_wait32(s);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) tops[i] = -INFINITY;
-                            auto look = [&](float (&s)[32], int col) {
-                                if (change) {
-                                    if (kGeneral)
+                            for (int g = 0; g < kKeys / 32; ++g) {
+                                if (g + 1 < kKeys / 32) tm_ld32(s_at + (g + 1) * 32, s + (g + 1) * 32);
+                                if (kGeneral)
 #pragma unroll
-                                        for (int i = 0; i < 32; ++i) {
-                                            float x = s[i] * a.pre;
-                                            if (a.post != 0.f) x = a.post * tanhf(x);
-                                            s[i] = a.bias_near ? fmaf(slope, static_cast<float>(j0 + col + i - pos), x) : x;
-                                        }
+                                    for (int i = g * 32; i < g * 32 + 32; ++i) {
+                                        float x = s[i] * a.pre;
+                                        if (a.post != 0.f) x = a.post * tanhf(x);
+                                        s[i] = a.bias_near ? fmaf(slope, static_cast<float>(j0 + i - pos), x) : x;
+                                    }
+                                if (cut)
 #pragma unroll
-                                    for (int i = 0; i < 32; ++i)
-                                        if (i < k0 - col || i > k1 - col) s[i] = -INFINITY;
-                                    tm_st16(s_at + col, reinterpret_cast<const uint32_t*>(s));
-                                    tm_st16(s_at + col + 16, reinterpret_cast<const uint32_t*>(s + 16));
+                                    for (int i = g * 32; i < g * 32 + 32; ++i)
+                                        if (i < k0 || i > k1) s[i] = -INFINITY;
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const float* x = s + g * 32 + i;
+                                    const float y = fmaxf(fmaxf(x[0], x[8]), fmaxf(x[16], x[24]));
+                                    tops[i] = g ? fmaxf(tops[i], y) : y;
                                 }
-#pragma unroll
-                                for (int i = 0; i < 8; ++i)
-                                    tops[i] = fmaxf(tops[i], fmaxf(fmaxf(s[i], s[i + 8]), fmaxf(s[i + 16], s[i + 24])));
-                            };
-                            tm_ld32(s_at, s0);
-#pragma unroll 1
-                            for (int half = 0; half < 2; ++half) {
-                                tm_wait32(s0);
-                                tm_ld32(s_at + half * 64 + 32, s1);
-                                look(s0, half * 64);
-                                tm_wait32(s1);
-                                if (half == 0) tm_ld32(s_at + 64, s0);
-                                look(s1, half * 64 + 32);
+                                if (g + 1 < kKeys / 32) tm_wait32(s + (g + 1) * 32);
                             }
-                            if (change) tm_wait_st();
-                            tm_ld32(s_at, s0);
                             float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
                                               fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
                             top *= pre;
@@ -631,31 +627,24 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                                 __syncwarp();
                             }
                             const float2 pre2 = make_float2(pre, pre), off2 = make_float2(off, off);
-                            // Second pass: the weights.
                             float2 sum[4] = {};
-                            auto weigh = [&](const float (&s)[32], int col) {
+#pragma unroll
+                            for (int g = 0; g < kKeys / 32; ++g) {
                                 uint32_t p[16];
 #pragma unroll
                                 for (int i = 0; i < 16; ++i) {
-                                    float2 x = fma2(make_float2(s[2 * i], s[2 * i + 1]), pre2, off2);
+                                    float2 x = fma2(make_float2(s[g * 32 + 2 * i], s[g * 32 + 2 * i + 1]), pre2, off2);
                                     x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
                                     sum[i & 3] = add2(sum[i & 3], x);
                                     p[i] = Half16<T>::pack(x.x, x.y);
                                 }
-                                tm_st16(s_at + col / 2, p);
-                            };
-#pragma unroll 1
-                            for (int half = 0; half < 2; ++half) {
-                                tm_wait32(s0);
-                                tm_ld32(s_at + half * 64 + 32, s1);
-                                weigh(s0, half * 64);
-                                tm_wait32(s1);
-                                if (half == 0) tm_ld32(s_at + 64, s0);
-                                weigh(s1, half * 64 + 32);
-                                tm_wait_st();  // half of the weights: the matrix unit may take them
-                                tc_before();
-                                __syncwarp();
-                                if (lane == 0) bar_arrive(&bars.pfull[q][half]);
+                                tm_st16(s_at + g * 16, p);
+                                if (g % 2) {  // half of the weights: the matrix unit may take them
+                                    tm_wait_st();
+                                    tc_before();
+                                    __syncwarp();
+                                    if (lane == 0) bar_arrive(&bars.pfull[q][g / 2]);
+                                }
                             }
                             if (L::kQ == 2 && lane == 0) turns[warp] = mine + t + 1 - lo;
                             const float2 both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
