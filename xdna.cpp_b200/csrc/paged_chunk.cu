@@ -7,7 +7,7 @@
 // A CTA works on an item of up to 2 x 128 rows (query tile q: rows 128 q ..) of
 // one request and KV head.  Per tile of keys: S = Q K^T into TMEM, weights
 // P = 2^(s - m) back into TMEM over S in 16 bits, O += P V in TMEM.  Roles:
-//   4 warps per query tile   one row per thread: softmax, rescaling and output
+//   8 warps per query tile   half a row per thread: softmax, rescaling and output
 //   one warp per query tile  issues its matrix instructions (one warp for both was
 //                            the bound: its waits and issues in a row took longer
 //                            than the matrix unit)
@@ -50,11 +50,12 @@ struct Shape {
     static constexpr int kHalves = (D + 63) / 64;
     static constexpr int kStages = D == 64 ? 4 : D <= 128 ? 2 : 1;
     static constexpr int kTile = kHalves * 128 * 128;  // bytes of 128 rows
-    // 4 softmax warps and a matrix warp per query tile, a loading warp; 12 warps, so
-    // that the softmax warps can take registers from a whole group of others
-    static constexpr int kThreads = kQ == 2 ? 384 : 192;
-    static constexpr int kLaunchRegs = 168, kSoftmaxRegs = 224, kOtherRegs = 56;
-    static_assert(kQ == 1 || 256 * kSoftmaxRegs + 128 * kOtherRegs <= 384 * kLaunchRegs, "registers of the launch");
+    // 8 softmax warps and a matrix warp per query tile, a loading warp; made up to
+    // whole groups of 4 warps, so that with two query tiles the softmax warps can
+    // take registers from the others
+    static constexpr int kThreads = kQ * 256 + 128;
+    static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 64;
+    static_assert(kQ == 1 || 512 * kSoftmaxRegs + 128 * kOtherRegs <= 640 * kLaunchRegs, "registers of the launch");
     static constexpr int kSmem = (kQ + 2 * kStages) * kTile + 1024;  // 1024: alignment
     static constexpr int kS = 0, kO = 256, kPitch = 128;             // TMEM columns of q's S and O: + 128 q
 };
@@ -68,7 +69,8 @@ struct ChunkArgs {
 // ------------------------------------------------------------------- barriers
 struct Bars {
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-    uint64_t qfull[2], sfull[2], pfull[2][2], ofull[2], drain[2];  // pfull: a barrier for each half of the keys
+    uint64_t qfull[2], sfull[2], pfull[2], ofull[2], drain[2];
+    uint64_t pair[2][4];
 };
 
 // ------------------------------------------------------------ matrix unit, TMEM
@@ -139,6 +141,16 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ void tm_st8(uint32_t addr, const uint32_t* u) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(u[0]), "r"(u[1]),
+                 "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                 : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 // True on one lane of a converged warp.  Branches on it, with addresses that are
@@ -270,11 +282,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
     __shared__ long long warp_units[L::kThreads / 32];
     __shared__ uint32_t tmem_slot;
     __shared__ int dead_word;
-    __shared__ volatile int turns[8];  // key tiles whose weights a softmax warp has formed
+    __shared__ volatile int turns[8 * L::kQ];  // key tiles whose weights a softmax warp has formed
+    __shared__ float swap[L::kQ][2][2][128];   // what the two halves of a row tell each other, twice
     volatile int* dead = &dead_word;
     const AttnArgs& a = c.g.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.p.n_seqs;
-    constexpr int kLoadWarp = L::kQ * 4, kMmaWarp = kLoadWarp + 1;  // and kMmaWarp + 1 for the second query tile
+    constexpr int kLoadWarp = L::kQ * 8, kMmaWarp = kLoadWarp + 1;  // and kMmaWarp + 1 for the second query tile
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     const uint32_t qs = base, ks = qs + L::kQ * L::kTile, vs = ks + L::kStages * L::kTile;
 
@@ -286,15 +299,15 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
             bar_init(&bars.vempty[i], L::kQ);
         }
         for (int i = 0; i < 2; ++i) {
-            bar_init(&bars.qfull[i], 128);
+            bar_init(&bars.qfull[i], 256);
             bar_init(&bars.sfull[i], 1);
-            bar_init(&bars.pfull[i][0], 4);
-            bar_init(&bars.pfull[i][1], 4);
+            bar_init(&bars.pfull[i], 8);
+            for (int j = 0; j < 4; ++j) bar_init(&bars.pair[i][j], 2);
             bar_init(&bars.ofull[i], 1);
             bar_init(&bars.drain[i], 1);
         }
         dead_word = 0;
-        for (int i = 0; i < 8; ++i) turns[i] = 0;
+        for (int i = 0; i < 8 * L::kQ; ++i) turns[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -451,18 +464,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                         ok = bar_wait(&bars.vfull[stage], ((i - 1) / L::kStages) & 1, dead);
                         if (ok && t > lo && t <= hi) {
                             const uint64_t v = v_op + (stage * L::kTile >> 4);
+                            ok = bar_wait(&bars.pfull[q], np & 1, dead);
+                            tc_after();
+                            if (ok && elect_one()) {
 #pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                if (ok) ok = bar_wait(&bars.pfull[q][half], np & 1, dead);
-                                tc_after();
-                                if (ok && elect_one()) {
-#pragma unroll
-                                    for (int k = half * 4; k < half * 4 + 4; ++k)
-                                        mma_ts(o_at, s_at + k * 8, v + (k * 2048 >> 4), kIdescO, k > 0 || t - 1 > lo);
-                                    if (half == 1 && t == hi) tc_commit(&bars.ofull[q]);
-                                }
-                                __syncwarp();
+                                for (int k = 0; k < kKeys / 16; ++k)  // weights of keys 64 .. lie 64 columns further on
+                                    mma_ts(o_at, s_at + (k >> 2) * 64 + (k & 3) * 8, v + (k * 2048 >> 4), kIdescO,
+                                           k > 0 || t - 1 > lo);
+                                if (t == hi) tc_commit(&bars.ofull[q]);
                             }
+                            __syncwarp();
                             ++np;
                         } else if (ok && lane == 0) {
                             bar_arrive(&bars.vempty[stage]);
@@ -500,14 +511,24 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
         } else {
             // ------------------------------------------------------------------ softmax
             if constexpr (L::kQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));
-            const int q = warp >> 2, row = tid - q * 128;
+            // Warps 8 q + 4 h + i: rows 32 i .. of query tile q, half h of the columns
+            const int q = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
             const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-            const uint32_t s_at = tmem + lanes + L::kS + q * L::kPitch, o_at = tmem + lanes + L::kO + q * L::kPitch;
+            const uint32_t s_at = tmem + lanes + L::kS + q * L::kPitch + half * 64;
+            const uint32_t o_at = tmem + lanes + L::kO + q * L::kPitch + half * (D / 2);
             const uint32_t q_at = qs + q * L::kTile + row * 128;
-            uint32_t ns = 0, no = 0;  // phases of sfull and ofull
-            uint32_t n = 0;           // key tiles before the item's
-            int mine = 0, theirs = 0;  // key tiles of this and of the other query tile before the item's
+            uint32_t ns = 0, no = 0, nx = 0;  // phases of sfull and ofull, exchanges
+            uint32_t n = 0;                   // key tiles before the item's
+            int mine = 0, theirs = 0;         // key tiles of this and of the other query tile before the item's
             bool ok = true, first_item = true;
+            // The value of the thread that holds the row's other half.
+            auto other_half = [&](float x) {
+                swap[q][nx & 1][half][row] = x;
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.pair[q][warp & 3]);
+                ok = bar_wait(&bars.pair[q][warp & 3], nx & 1, dead);
+                return swap[q][nx++ & 1][half ^ 1][row];
+            };
             do {
                 const int r0 = w.tile * R + q * 128, rr = r0 + row;
                 if (r0 < w.rows) {
@@ -521,12 +542,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                     const float slope = kGeneral ? head_slope(a, head) : 0.f;
                     float m = -INFINITY, l = 0.f;
                     if (lo < hi) {
-                        // the row's queries into the swizzled rows the matrix unit reads
+                        // half of the row's queries into the swizzled rows the matrix unit reads
                         const uint4* src = reinterpret_cast<const uint4*>(
                             static_cast<const char*>(a.p.q) + (w.rq.first + token) * a.p.nb_q +
                             static_cast<int64_t>(head) * D * 2);
 #pragma unroll
-                        for (int x = 0; x < L::kHalves * 8; ++x) {
+                        for (int i = 0; i < L::kHalves * 4; ++i) {
+                            const int x = half * L::kHalves * 4 + i;
                             uint4 v = make_uint4(0, 0, 0, 0);
                             if (on && x < D / 8) v = __ldg(src + x);
                             asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
@@ -547,53 +569,64 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             if (!ok) break;
                             tc_after();
                             // S is there, and so is O of the tile before: K and that tile's V are free
-                            if (row == 0) {
+                            if (row == 0 && half == 0) {
                                 const uint32_t x = n + t - w.s0;
                                 bar_arrive(&bars.kempty[x % L::kStages]);
                                 if (t > lo) bar_arrive(&bars.vempty[(x - 1) % L::kStages]);
                             }
-                            const int j0 = t * kKeys;
-                            const bool cut = j0 < all_lo || j0 + kKeys > all_hi;
+                            const int j0 = t * kKeys + half * 64;
+                            const bool cut = t * kKeys < all_lo || (t + 1) * kKeys > all_hi;
                             const float pre = kGeneral ? 1.f : a.pre;
                             const int k0 = first - j0, k1 = last - j0;
-                            float s[kKeys];
-                            // the row's maximum, in eight chains, while the next columns are on their way
-                            float tops[8];
-                            tm_ld32(s_at, s);
-                            tm_wait32(s);
+                            // Columns of S, 16 worked on and 16 on their way (so few registers that 16
+                            // softmax warps fit).  First pass: the maximum of half the row, in eight
+                            // chains.  Scores that the cap, the bias or a hidden key change go back
+                            // for the second pass.
+                            float s0[16], s1[16], tops[8];
+                            auto look = [&](float (&s)[16], int col) {
+                                if (kGeneral || cut) {
+                                    if (kGeneral)
 #pragma unroll
-                            for (int g = 0; g < kKeys / 32; ++g) {
-                                if (g + 1 < kKeys / 32) tm_ld32(s_at + (g + 1) * 32, s + (g + 1) * 32);
-                                if (kGeneral)
+                                        for (int i = 0; i < 16; ++i) {
+                                            float x = s[i] * a.pre;
+                                            if (a.post != 0.f) x = a.post * tanhf(x);
+                                            s[i] = a.bias_near ? fmaf(slope, static_cast<float>(j0 + col + i - pos), x) : x;
+                                        }
 #pragma unroll
-                                    for (int i = g * 32; i < g * 32 + 32; ++i) {
-                                        float x = s[i] * a.pre;
-                                        if (a.post != 0.f) x = a.post * tanhf(x);
-                                        s[i] = a.bias_near ? fmaf(slope, static_cast<float>(j0 + i - pos), x) : x;
-                                    }
-                                if (cut)
-#pragma unroll
-                                    for (int i = g * 32; i < g * 32 + 32; ++i)
-                                        if (i < k0 || i > k1) s[i] = -INFINITY;
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    const float* x = s + g * 32 + i;
-                                    const float y = fmaxf(fmaxf(x[0], x[8]), fmaxf(x[16], x[24]));
-                                    tops[i] = g ? fmaxf(tops[i], y) : y;
+                                    for (int i = 0; i < 16; ++i)
+                                        if (i < k0 - col || i > k1 - col) s[i] = -INFINITY;
+                                    tm_st16(s_at + col, reinterpret_cast<const uint32_t*>(s));
                                 }
-                                if (g + 1 < kKeys / 32) tm_wait32(s + (g + 1) * 32);
-                            }
-                            float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
-                                              fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) tops[i] = col ? max3(tops[i], s[i], s[i + 8]) : fmaxf(s[i], s[i + 8]);
+                            };
+                            tm_ld16(s_at, s0);
+                            tm_wait16(s0);
+                            tm_ld16(s_at + 16, s1);
+                            look(s0, 0);
+                            tm_wait16(s1);
+                            tm_ld16(s_at + 32, s0);
+                            look(s1, 16);
+                            tm_wait16(s0);
+                            tm_ld16(s_at + 48, s1);
+                            look(s0, 32);
+                            tm_wait16(s1);
+                            look(s1, 48);
+                            if (kGeneral || cut) tm_wait_st();
+                            tm_ld16(s_at, s0);
+                            float top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]),
+                                             fmaxf(tops[6], tops[7]));
                             top *= pre;
-                            if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                            top = fmaxf(top, other_half(top));
+                            if (!ok) break;
+                            if (__any_sync(0xffffffffu, top > m + kSlack)) {  // both halves alike
                                 const float was = m;
                                 m = fmaxf(m, top);
                                 const float f = m == -INFINITY ? 1.f : exp2_fast(was - m);
                                 l *= f;
                                 if (t > lo) {
 #pragma unroll 1
-                                    for (int i = 0; i < D / 16; ++i) {
+                                    for (int i = 0; i < D / 32; ++i) {
                                         float o[16];
                                         tm_ld16(o_at + i * 16, o);
                                         tm_wait16(o);
@@ -603,12 +636,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                                     }
                                 }
                             }
-                            if (j0 + kKeys > w.hi) {  // values of keys that do not exist: a weight of 0 would not hide a NaN
+                            if ((t + 1) * kKeys > w.hi) {  // values of keys that do not exist: a weight of 0 would not hide a NaN
                                 const uint32_t x = n + t - w.s0, stage = x % L::kStages;
                                 ok = bar_wait(&bars.vfull[stage], (x / L::kStages) & 1, dead);
                                 if (!ok) break;
-                                const int gone = max(w.hi - j0, 0);
-                                for (int y = row; y < (kKeys - gone) * 8 * L::kHalves; y += 128)
+                                const int gone = max(w.hi - t * kKeys, 0);
+                                for (int y = half * 128 + row; y < (kKeys - gone) * 8 * L::kHalves; y += 256)
                                     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
                                                      vs + stage * L::kTile + (y % (8 * L::kHalves) >> 3) * 128 * 128 +
                                                      (gone + y / (8 * L::kHalves)) * 128 + (y & 7) * 16),
@@ -620,67 +653,80 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             // The two query tiles' warps on a scheduler take turns in the exponentials,
                             // so that the matrix unit has the other one's work meanwhile (left alone
                             // they run in step, and the matrix unit waits for both).
-                            if (L::kQ == 2) {
+                            if (L::kQ == 2 && kTurnClocks > 0) {
                                 const int due = theirs + min(max(t + q - other_lo, 0), other_hi - other_lo);
                                 const long long since = clock64();
-                                while (turns[warp ^ 4] < due && clock64() - since < kTurnClocks) {}
+                                while (turns[warp ^ 8] < due && clock64() - since < kTurnClocks) {}
                                 __syncwarp();
                             }
                             const float2 pre2 = make_float2(pre, pre), off2 = make_float2(off, off);
-                            float2 sum[4] = {};
+                            // Second pass: the weights.
+                            float2 sum[2] = {};
+                            auto weigh = [&](const float (&s)[16], int col) {
+                                uint32_t p[8];
 #pragma unroll
-                            for (int g = 0; g < kKeys / 32; ++g) {
-                                uint32_t p[16];
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) {
-                                    float2 x = fma2(make_float2(s[g * 32 + 2 * i], s[g * 32 + 2 * i + 1]), pre2, off2);
+                                for (int i = 0; i < 8; ++i) {
+                                    float2 x = fma2(make_float2(s[2 * i], s[2 * i + 1]), pre2, off2);
                                     x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                                    sum[i & 3] = add2(sum[i & 3], x);
+                                    sum[i & 1] = add2(sum[i & 1], x);
                                     p[i] = Half16<T>::pack(x.x, x.y);
                                 }
-                                tm_st16(s_at + g * 16, p);
-                                if (g % 2) {  // half of the weights: the matrix unit may take them
-                                    tm_wait_st();
-                                    tc_before();
-                                    __syncwarp();
-                                    if (lane == 0) bar_arrive(&bars.pfull[q][g / 2]);
-                                }
+                                tm_st8(s_at + col / 2, p);
+                            };
+                            tm_wait16(s0);
+                            tm_ld16(s_at + 16, s1);
+                            weigh(s0, 0);
+                            tm_wait16(s1);
+                            tm_ld16(s_at + 32, s0);
+                            weigh(s1, 16);
+                            tm_wait16(s0);
+                            tm_ld16(s_at + 48, s1);
+                            weigh(s0, 32);
+                            tm_wait16(s1);
+                            weigh(s1, 48);
+                            tm_wait_st();
+                            tc_before();
+                            __syncwarp();
+                            if (lane == 0) {
+                                bar_arrive(&bars.pfull[q]);
+                                if (L::kQ == 2) turns[warp] = mine + t + 1 - lo;
                             }
-                            if (L::kQ == 2 && lane == 0) turns[warp] = mine + t + 1 - lo;
-                            const float2 both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                            const float2 both = add2(sum[0], sum[1]);
                             l += both.x + both.y;
                         }
+                        if (ok) l += other_half(l);
                         if (ok) ok = bar_wait(&bars.ofull[q], no++ & 1, dead);
                         if (!ok) break;
                         tc_after();
-                        if (row == 0) bar_arrive(&bars.vempty[(n + hi - 1 - w.s0) % L::kStages]);
+                        if (row == 0 && half == 0) bar_arrive(&bars.vempty[(n + hi - 1 - w.s0) % L::kStages]);
                     }
-                    // O to the output, or to the item's partial
+                    // half of O to the output, or to the item's partial
                     const bool whole = w.s0 == w.t0 && w.s1 == w.t1;
                     const float inv = l == 0.f ? 0.f : whole ? 1.f / l : 1.f;
                     float* part = c.g.parts + (static_cast<size_t>(me) * 2 + (w.s0 == w.t0)) * part_floats(R, D);
                     char* out = static_cast<char*>(a.p.out) + (w.rq.first + token) * a.p.nb_out;
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i) {
-                        float o[32];
+                        const int col = half * (D / 2) + i * 16;
+                        float o[16];
                         if (lo < hi) {
-                            tm_ld32(o_at + i * 32, o);
-                            tm_wait32(o);
+                            tm_ld16(o_at + i * 16, o);
+                            tm_wait16(o);
                         }
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
+                        for (int e = 0; e < 16; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
                         if (on) {
-                            float4* to = reinterpret_cast<float4*>(part + static_cast<size_t>(q * 128 + row) * D + i * 32);
+                            float4* to = reinterpret_cast<float4*>(part + static_cast<size_t>(q * 128 + row) * D + col);
                             if (whole && a.p.out_type == GGML_TYPE_F32)
-                                to = reinterpret_cast<float4*>(out + (static_cast<int64_t>(head) * D + i * 32) * 4);
+                                to = reinterpret_cast<float4*>(out + (static_cast<int64_t>(head) * D + col) * 4);
                             if (!whole || a.p.out_type == GGML_TYPE_F32) {
 #pragma unroll
-                                for (int e = 0; e < 8; ++e)
+                                for (int e = 0; e < 4; ++e)
                                     to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                             } else {
-                                uint4* to16 = reinterpret_cast<uint4*>(out + (static_cast<int64_t>(head) * D + i * 32) * 2);
+                                uint4* to16 = reinterpret_cast<uint4*>(out + (static_cast<int64_t>(head) * D + col) * 2);
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
+                                for (int e = 0; e < 2; ++e)
                                     to16[e] = make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]),
                                                          Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
                                                          Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]),
@@ -689,7 +735,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                         }
                         __syncwarp();
                     }
-                    if (!whole && on) {
+                    if (!whole && on && half == 0) {
                         part[R * D + q * 128 + row] = m;
                         part[R * D + R + q * 128 + row] = l;
                     }
