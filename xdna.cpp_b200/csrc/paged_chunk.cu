@@ -41,6 +41,7 @@ namespace {
 constexpr int kKeys = 128;
 constexpr int kMinTiles = 2;   // key tiles per CTA below which fewer CTAs run
 constexpr float kSlack = 8.f;  // log2 of the largest weight
+constexpr int kPoly = 0;        // of 8 pairs of weights, those formed by the polynomial
 constexpr int kTurnClocks = 4000;  // longest wait for a turn (a courtesy: nothing depends on it)
 
 template <int D>
@@ -70,7 +71,6 @@ struct ChunkArgs {
 struct Bars {
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
     uint64_t qfull[2], sfull[2], pfull[2], ofull[2], drain[2];
-    uint64_t pair[2][4];
 };
 
 // ------------------------------------------------------------ matrix unit, TMEM
@@ -118,15 +118,6 @@ __device__ __forceinline__ void tm_wait16(float* r) {
                  :
                  : "memory");
 }
-__device__ __forceinline__ void tm_wait32(float* r) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
-                   "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(r[16]),
-                   "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]),
-                   "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
-                 :
-                 : "memory");
-}
 // Two F32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -134,6 +125,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         "fma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -163,17 +161,6 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tm_ld32(uint32_t addr, float* r) {
-    uint32_t* u = reinterpret_cast<uint32_t*>(r);
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
-          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
-          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
-          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
-        : "r"(addr));
-}
 __device__ __forceinline__ void tm_ld16(uint32_t addr, float* r) {
     uint32_t* u = reinterpret_cast<uint32_t*>(r);
     asm volatile(
@@ -189,6 +176,35 @@ __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* u) {
         "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
         : "memory");
 }
+// 2^x without the exponential unit: x = i + f with i the nearest whole number
+// (x + 1.5 2^23 + 127 rounds to it, and shifted left its bits are 2^i), 2^f on
+// [-1/2, 1/2] by the polynomial of least relative error (Remez exchange; 7.5e-5
+// with 4 terms, under 2^-13, for weights rounded to 8 bits; 2.6e-6 with 5 for 11
+// bits).  x below -126 counts as -126; NaN stays NaN.
+template <typename T>
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    constexpr float kMagic = 12582912.f + 127.f;
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+    const float2 t = add2(x, make_float2(kMagic, kMagic));
+    const float2 r = add2(t, make_float2(-kMagic, -kMagic));
+    const float2 f = fma2(r, make_float2(-1.f, -1.f), x);
+    auto c = [](float v) { return make_float2(v, v); };
+    float2 p;
+    if (std::is_same<T, __half>::value) {
+        p = fma2(f, c(0.009570102207362652f), c(0.05591785907745361f));
+        p = fma2(p, f, c(0.240247443318367f));
+        p = fma2(p, f, c(0.6931217908859253f));
+        p = fma2(p, f, c(0.9999992847442627f));
+    } else {
+        p = fma2(f, c(0.0551716685295105f), c(0.2426111251115799f));
+        p = fma2(p, f, c(0.6932609677314758f));
+        p = fma2(p, f, c(0.9999280571937561f));
+    }
+    const float2 two = make_float2(__int_as_float(__float_as_int(t.x) << 23), __int_as_float(__float_as_int(t.y) << 23));
+    return mul2(p, two);
+}
+
 // ------------------------------------------------------------------ the work list
 // Key tiles [t0, t1) of row tile `tile`, and of one of its query tiles.
 template <int R>
@@ -302,7 +318,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
             bar_init(&bars.qfull[i], 256);
             bar_init(&bars.sfull[i], 1);
             bar_init(&bars.pfull[i], 8);
-            for (int j = 0; j < 4; ++j) bar_init(&bars.pair[i][j], 2);
             bar_init(&bars.ofull[i], 1);
             bar_init(&bars.drain[i], 1);
         }
@@ -457,48 +472,39 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                 query_tiles(a, w, w.tile * R + q * 128, lo, hi);
                 lo = uniform(lo), hi = uniform(hi);
                 const int s0 = uniform(w.s0), s1 = uniform(w.s1);
-                // step t: O of tile t - 1, then S of tile t
+                // step t: O of tile t - 1, then S of tile t.  What S needs is waited for
+                // before the weights, so that it follows at once.
                 for (int t = s0; t <= s1 && ok; ++t, ++i) {
-                    if (t > s0) {
-                        const uint32_t stage = (i - 1) % L::kStages;
-                        ok = bar_wait(&bars.vfull[stage], ((i - 1) / L::kStages) & 1, dead);
-                        if (ok && t > lo && t <= hi) {
-                            const uint64_t v = v_op + (stage * L::kTile >> 4);
-                            ok = bar_wait(&bars.pfull[q], np & 1, dead);
-                            tc_after();
-                            if (ok && elect_one()) {
+                    const uint32_t k_stage = i % L::kStages, v_stage = (i + L::kStages - 1) % L::kStages;
+                    const bool value = t > lo && t <= hi && t > s0, score = t >= lo && t < hi && t < s1;
+                    if (t > s0) ok = bar_wait(&bars.vfull[v_stage], ((i - 1) / L::kStages) & 1, dead);
+                    if (ok && t < s1) ok = bar_wait(&bars.kfull[k_stage], (i / L::kStages) & 1, dead);
+                    if (ok && score && t == lo) ok = bar_wait(&bars.qfull[q], nq++ & 1, dead);
+                    if (ok && value) ok = bar_wait(&bars.pfull[q], np++ & 1, dead);
+                    tc_after();
+                    const uint64_t v = v_op + (v_stage * L::kTile >> 4), k_at = k_op + (k_stage * L::kTile >> 4);
+                    if (ok && elect_one()) {
+                        if (value) {
 #pragma unroll
-                                for (int k = 0; k < kKeys / 16; ++k)  // weights of keys 64 .. lie 64 columns further on
-                                    mma_ts(o_at, s_at + (k >> 2) * 64 + (k & 3) * 8, v + (k * 2048 >> 4), kIdescO,
-                                           k > 0 || t - 1 > lo);
-                                if (t == hi) tc_commit(&bars.ofull[q]);
+                            for (int k = 0; k < kKeys / 16; ++k)  // weights of keys 64 .. lie 64 columns further on
+                                mma_ts(o_at, s_at + (k >> 2) * 64 + (k & 3) * 8, v + (k * 2048 >> 4), kIdescO,
+                                       k > 0 || t - 1 > lo);
+                            if (t == hi) tc_commit(&bars.ofull[q]);
+                        } else if (t > s0) {
+                            bar_arrive(&bars.vempty[v_stage]);
+                        }
+                        if (score) {
+#pragma unroll
+                            for (int k = 0; k < D / 16; ++k) {
+                                const uint32_t off = ((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4;
+                                mma_ss(s_at, q_op + off, k_at + off, kIdescS, k > 0);
                             }
-                            __syncwarp();
-                            ++np;
-                        } else if (ok && lane == 0) {
-                            bar_arrive(&bars.vempty[stage]);
+                            tc_commit(&bars.sfull[q]);
+                        } else if (t < s1) {
+                            bar_arrive(&bars.kempty[k_stage]);
                         }
                     }
-                    if (ok && t < s1) {
-                        const uint32_t stage = i % L::kStages;
-                        ok = bar_wait(&bars.kfull[stage], (i / L::kStages) & 1, dead);
-                        if (ok && t >= lo && t < hi) {
-                            if (t == lo) ok = bar_wait(&bars.qfull[q], nq++ & 1, dead);
-                            tc_after();
-                            const uint64_t k_at = k_op + (stage * L::kTile >> 4);
-                            if (ok && elect_one()) {
-#pragma unroll
-                                for (int k = 0; k < D / 16; ++k) {
-                                    const uint32_t off = ((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4;
-                                    mma_ss(s_at, q_op + off, k_at + off, kIdescS, k > 0);
-                                }
-                                tc_commit(&bars.sfull[q]);
-                            }
-                            __syncwarp();
-                        } else if (ok && lane == 0) {
-                            bar_arrive(&bars.kempty[stage]);
-                        }
-                    }
+                    __syncwarp();
                 }
                 --i;  // the last step has no tile of its own
             } while (ok && w.next<R>(a));
@@ -520,13 +526,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
             uint32_t ns = 0, no = 0, nx = 0;  // phases of sfull and ofull, exchanges
             uint32_t n = 0;                   // key tiles before the item's
             int mine = 0, theirs = 0;         // key tiles of this and of the other query tile before the item's
-            bool ok = true, first_item = true;
-            // The value of the thread that holds the row's other half.
+            bool first_item = true;
+            // The value of the thread that holds the row's other half.  Both warps of a
+            // pair pass here equally often, whatever their waits return: a warp whose wait
+            // has run out goes through the rest of its tiles all the same.
             auto other_half = [&](float x) {
                 swap[q][nx & 1][half][row] = x;
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bars.pair[q][warp & 3]);
-                ok = bar_wait(&bars.pair[q][warp & 3], nx & 1, dead);
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + q * 4 + (warp & 3)) : "memory");
                 return swap[q][nx++ & 1][half ^ 1][row];
             };
             do {
@@ -564,9 +570,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                         const int p1 = w.rq.pos0() + (min(r0 + 128, w.rows) - 1) / a.group;
                         const int all_hi = min(p0 + 1, w.hi);
                         const int all_lo = a.p.window > 0 && p1 >= a.p.window ? p1 - a.p.window + 1 : 0;
-                        for (int t = lo; t < hi && ok; ++t) {
-                            ok = bar_wait(&bars.sfull[q], ns++ & 1, dead);
-                            if (!ok) break;
+                        for (int t = lo; t < hi; ++t) {
+                            bar_wait(&bars.sfull[q], ns++ & 1, dead);
                             tc_after();
                             // S is there, and so is O of the tile before: K and that tile's V are free
                             if (row == 0 && half == 0) {
@@ -618,7 +623,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                                              fmaxf(tops[6], tops[7]));
                             top *= pre;
                             top = fmaxf(top, other_half(top));
-                            if (!ok) break;
                             if (__any_sync(0xffffffffu, top > m + kSlack)) {  // both halves alike
                                 const float was = m;
                                 m = fmaxf(m, top);
@@ -638,8 +642,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             }
                             if ((t + 1) * kKeys > w.hi) {  // values of keys that do not exist: a weight of 0 would not hide a NaN
                                 const uint32_t x = n + t - w.s0, stage = x % L::kStages;
-                                ok = bar_wait(&bars.vfull[stage], (x / L::kStages) & 1, dead);
-                                if (!ok) break;
+                                bar_wait(&bars.vfull[stage], (x / L::kStages) & 1, dead);
                                 const int gone = max(w.hi - t * kKeys, 0);
                                 for (int y = half * 128 + row; y < (kKeys - gone) * 8 * L::kHalves; y += 256)
                                     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
@@ -667,7 +670,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
 #pragma unroll
                                 for (int i = 0; i < 8; ++i) {
                                     float2 x = fma2(make_float2(s[2 * i], s[2 * i + 1]), pre2, off2);
-                                    x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                                    if (i >= 8 - kPoly && !cut)  // hidden keys have a weight of exactly 0: 2^-inf
+                                        x = exp2_poly<T>(x);
+                                    else
+                                        x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
                                     sum[i & 1] = add2(sum[i & 1], x);
                                     p[i] = Half16<T>::pack(x.x, x.y);
                                 }
@@ -694,9 +700,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             const float2 both = add2(sum[0], sum[1]);
                             l += both.x + both.y;
                         }
-                        if (ok) l += other_half(l);
-                        if (ok) ok = bar_wait(&bars.ofull[q], no++ & 1, dead);
-                        if (!ok) break;
+                        l += other_half(l);
+                        bar_wait(&bars.ofull[q], no++ & 1, dead);
                         tc_after();
                         if (row == 0 && half == 0) bar_arrive(&bars.vempty[(n + hi - 1 - w.s0) % L::kStages]);
                     }
