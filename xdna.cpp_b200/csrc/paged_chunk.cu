@@ -11,7 +11,7 @@
 //   one warp per query tile  issues its matrix instructions (one warp for both was
 //                            the bound: its waits and issues in a row took longer
 //                            than the matrix unit)
-//   one warp                 TMA loads of K and V, page by page, into a ring
+//   one warp each            TMA loads of K and of V, page by page, into rings
 // While one query tile is in its softmax the matrix unit works on the other
 // one.  O is rescaled only when a row's maximum grows by more than 8 (weights
 // stay below 2^8), which a vote of the warp finds out.  The weights are rounded
@@ -41,7 +41,6 @@ namespace {
 constexpr int kKeys = 128;
 constexpr int kMinTiles = 2;   // key tiles per CTA below which fewer CTAs run
 constexpr float kSlack = 8.f;  // log2 of the largest weight
-constexpr int kPoly = 0;        // of 8 pairs of weights, those formed by the polynomial
 constexpr int kTurnClocks = 4000;  // longest wait for a turn (a courtesy: nothing depends on it)
 
 template <int D>
@@ -70,7 +69,7 @@ struct ChunkArgs {
 // ------------------------------------------------------------------- barriers
 struct Bars {
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-    uint64_t qfull[2], sfull[2], pfull[2], ofull[2], drain[2];
+    uint64_t qfull[2], sfull[2], pfull[2][2], ofull[2], drain[2];  // pfull: keys 0-31 and 64-95, then the others
 };
 
 // ------------------------------------------------------------ matrix unit, TMEM
@@ -127,13 +126,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
     asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
@@ -176,35 +168,6 @@ __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* u) {
         "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
         : "memory");
 }
-// 2^x without the exponential unit: x = i + f with i the nearest whole number
-// (x + 1.5 2^23 + 127 rounds to it, and shifted left its bits are 2^i), 2^f on
-// [-1/2, 1/2] by the polynomial of least relative error (Remez exchange; 7.5e-5
-// with 4 terms, under 2^-13, for weights rounded to 8 bits; 2.6e-6 with 5 for 11
-// bits).  x below -126 counts as -126; NaN stays NaN.
-template <typename T>
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    constexpr float kMagic = 12582912.f + 127.f;
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
-    const float2 t = add2(x, make_float2(kMagic, kMagic));
-    const float2 r = add2(t, make_float2(-kMagic, -kMagic));
-    const float2 f = fma2(r, make_float2(-1.f, -1.f), x);
-    auto c = [](float v) { return make_float2(v, v); };
-    float2 p;
-    if (std::is_same<T, __half>::value) {
-        p = fma2(f, c(0.009570102207362652f), c(0.05591785907745361f));
-        p = fma2(p, f, c(0.240247443318367f));
-        p = fma2(p, f, c(0.6931217908859253f));
-        p = fma2(p, f, c(0.9999992847442627f));
-    } else {
-        p = fma2(f, c(0.0551716685295105f), c(0.2426111251115799f));
-        p = fma2(p, f, c(0.6932609677314758f));
-        p = fma2(p, f, c(0.9999280571937561f));
-    }
-    const float2 two = make_float2(__int_as_float(__float_as_int(t.x) << 23), __int_as_float(__float_as_int(t.y) << 23));
-    return mul2(p, two);
-}
-
 // ------------------------------------------------------------------ the work list
 // Key tiles [t0, t1) of row tile `tile`, and of one of its query tiles.
 template <int R>
@@ -303,7 +266,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
     volatile int* dead = &dead_word;
     const AttnArgs& a = c.g.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.p.n_seqs;
-    constexpr int kLoadWarp = L::kQ * 8, kMmaWarp = kLoadWarp + 1;  // and kMmaWarp + 1 for the second query tile
+    constexpr int kLoadWarp = L::kQ * 8, kMmaWarp = kLoadWarp + 2;  // two of each (one query tile: one kMmaWarp)
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     const uint32_t qs = base, ks = qs + L::kQ * L::kTile, vs = ks + L::kStages * L::kTile;
 
@@ -317,7 +280,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
         for (int i = 0; i < 2; ++i) {
             bar_init(&bars.qfull[i], 256);
             bar_init(&bars.sfull[i], 1);
-            bar_init(&bars.pfull[i], 8);
+            bar_init(&bars.pfull[i][0], 8);
+            bar_init(&bars.pfull[i][1], 8);
             bar_init(&bars.ofull[i], 1);
             bar_init(&bars.drain[i], 1);
         }
@@ -425,40 +389,42 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
 
         if (warp >= kLoadWarp) {
         if constexpr (L::kQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegs));
-        if (warp == kLoadWarp) {
+        if (warp < kMmaWarp) {
             // ---------------------------------------------------------------- loads
-            const int boxes = kKeys / c.box_tokens;  // per half; lane i issues box i
-            int n = 0;                               // tiles so far
+            const bool values = uniform(warp) == kLoadWarp + 1;  // one warp for K, one for V
+            const CUtensorMap* map = values ? &c.v : &c.k;
+            uint64_t *full = values ? bars.vfull : bars.kfull, *empty = values ? bars.vempty : bars.kempty;
+            const uint32_t ring = values ? vs : ks;
+            const int boxes = kKeys / c.box_tokens;  // per half; lane i looks up the block of box i
+            uint32_t n = 0;                          // tiles so far
             bool ok = true;
             do {
-                for (int t = w.s0; t < w.s1 && ok; ++t, ++n) {
-                    const int stage = n % L::kStages, j = t * kKeys + lane * c.box_tokens;
+                const int s0 = uniform(w.s0), s1 = uniform(w.s1), kvh = uniform(w.kvh);
+                for (int t = s0; t < s1 && ok; ++t, ++n) {
+                    const int j = t * kKeys + lane * c.box_tokens;
                     const bool on = lane < boxes && j < w.hi;
                     const int id = on ? key_block(a, w.b, j >> a.log_bs) : 0;
                     const int block = id < 0 ? static_cast<int>(a.kv.num_blocks) : id;  // behind the last: zeros
-                    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, on)) * L::kHalves * c.box_tokens * 128;
-                    const uint32_t parity = ((n / L::kStages) & 1) ^ 1;
-#pragma unroll
-                    for (int kv = 0; kv < 2 && ok; ++kv) {
-                        uint64_t* full = kv ? &bars.vfull[stage] : &bars.kfull[stage];
-                        if (n >= L::kStages) ok = bar_wait(kv ? &bars.vempty[stage] : &bars.kempty[stage], parity, dead);
-                        if (!ok) break;
-                        if (lane == 0) bar_expect(full, bytes);
-                        __syncwarp();
-                        if (on)
+                    const int count = __popc(__ballot_sync(0xffffffffu, on));
+                    const uint32_t stage = n % L::kStages;
+                    if (n >= L::kStages) ok = bar_wait(&empty[stage], ((n / L::kStages) & 1) ^ 1, dead);
+                    if (!ok) break;
+                    if (elect_one()) bar_expect(&full[stage], count * L::kHalves * c.box_tokens * 128);
+                    __syncwarp();
+                    for (int x = 0; x < count; ++x) {
+                        const int from = __shfl_sync(0xffffffffu, block, x), token = (t * kKeys + x * c.box_tokens) & (a.kv.block_size - 1);
+                        if (elect_one())
 #pragma unroll
                             for (int h = 0; h < L::kHalves; ++h)
-                                tma_box((kv ? vs : ks) + stage * L::kTile + h * 128 * 128 + lane * c.box_tokens * 128,
-                                        kv ? &c.v : &c.k, full, h * 64, j & (a.kv.block_size - 1), w.kvh, block);
+                                tma_box(ring + stage * L::kTile + h * 128 * 128 + x * c.box_tokens * 128, map, &full[stage], h * 64,
+                                        token, kvh, from);
+                        __syncwarp();
                     }
                 }
             } while (ok && w.next<R>(a));
-            if (!ok) {  // copies in flight land before the CTA ends
-                for (int i = max(0, n - L::kStages); i <= n; ++i) {
-                    bar_wait(&bars.kfull[i % L::kStages], (i / L::kStages) & 1, nullptr);
-                    bar_wait(&bars.vfull[i % L::kStages], (i / L::kStages) & 1, nullptr);
-                }
-            }
+            if (!ok)  // copies in flight land before the CTA ends
+                for (uint32_t i = n < L::kStages ? 0 : n - L::kStages; i < n; ++i)
+                    bar_wait(&full[i % L::kStages], (i / L::kStages) & 1, nullptr);
         } else if (warp < kMmaWarp + L::kQ) {
             // ----------------------------------------------------- matrix instructions
             constexpr uint32_t kIdescS = instruction<T>(kKeys, false), kIdescO = instruction<T>(D, true);
@@ -480,15 +446,28 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                     if (t > s0) ok = bar_wait(&bars.vfull[v_stage], ((i - 1) / L::kStages) & 1, dead);
                     if (ok && t < s1) ok = bar_wait(&bars.kfull[k_stage], (i / L::kStages) & 1, dead);
                     if (ok && score && t == lo) ok = bar_wait(&bars.qfull[q], nq++ & 1, dead);
-                    if (ok && value) ok = bar_wait(&bars.pfull[q], np++ & 1, dead);
-                    tc_after();
                     const uint64_t v = v_op + (v_stage * L::kTile >> 4), k_at = k_op + (k_stage * L::kTile >> 4);
+                    // 16 keys k: their weights lie in half k / 4 of S's columns
+                    auto weighted = [&](int k, bool add) {
+                        mma_ts(o_at, s_at + (k >> 2) * 64 + (k & 3) * 8, v + (k * 2048 >> 4), kIdescO, add);
+                    };
+                    if (ok && value) ok = bar_wait(&bars.pfull[q][0], np & 1, dead);
+                    tc_after();
+                    if (ok && value && elect_one()) {
+                        weighted(0, t - 1 > lo);
+                        weighted(1, true);
+                        weighted(4, true);
+                        weighted(5, true);
+                    }
+                    __syncwarp();
+                    if (ok && value) ok = bar_wait(&bars.pfull[q][1], np++ & 1, dead);
+                    tc_after();
                     if (ok && elect_one()) {
                         if (value) {
-#pragma unroll
-                            for (int k = 0; k < kKeys / 16; ++k)  // weights of keys 64 .. lie 64 columns further on
-                                mma_ts(o_at, s_at + (k >> 2) * 64 + (k & 3) * 8, v + (k * 2048 >> 4), kIdescO,
-                                       k > 0 || t - 1 > lo);
+                            weighted(2, true);
+                            weighted(3, true);
+                            weighted(6, true);
+                            weighted(7, true);
                             if (t == hi) tc_commit(&bars.ofull[q]);
                         } else if (t > s0) {
                             bar_arrive(&bars.vempty[v_stage]);
@@ -656,7 +635,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             // The two query tiles' warps on a scheduler take turns in the exponentials,
                             // so that the matrix unit has the other one's work meanwhile (left alone
                             // they run in step, and the matrix unit waits for both).
-                            if (L::kQ == 2 && kTurnClocks > 0) {
+                            if (L::kQ == 2) {
                                 const int due = theirs + min(max(t + q - other_lo, 0), other_hi - other_lo);
                                 const long long since = clock64();
                                 while (turns[warp ^ 8] < due && clock64() - since < kTurnClocks) {}
@@ -670,10 +649,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
 #pragma unroll
                                 for (int i = 0; i < 8; ++i) {
                                     float2 x = fma2(make_float2(s[2 * i], s[2 * i + 1]), pre2, off2);
-                                    if (i >= 8 - kPoly && !cut)  // hidden keys have a weight of exactly 0: 2^-inf
-                                        x = exp2_poly<T>(x);
-                                    else
-                                        x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                                    x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
                                     sum[i & 1] = add2(sum[i & 1], x);
                                     p[i] = Half16<T>::pack(x.x, x.y);
                                 }
@@ -685,18 +661,20 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             tm_wait16(s1);
                             tm_ld16(s_at + 32, s0);
                             weigh(s1, 16);
+                            auto hand_over = [&](int part) {  // weights the matrix unit may take
+                                tm_wait_st();
+                                tc_before();
+                                __syncwarp();
+                                if (lane == 0) bar_arrive(&bars.pfull[q][part]);
+                            };
+                            hand_over(0);
                             tm_wait16(s0);
                             tm_ld16(s_at + 48, s1);
                             weigh(s0, 32);
                             tm_wait16(s1);
                             weigh(s1, 48);
-                            tm_wait_st();
-                            tc_before();
-                            __syncwarp();
-                            if (lane == 0) {
-                                bar_arrive(&bars.pfull[q]);
-                                if (L::kQ == 2) turns[warp] = mine + t + 1 - lo;
-                            }
+                            hand_over(1);
+                            if (L::kQ == 2 && lane == 0) turns[warp] = mine + t + 1 - lo;
                             const float2 both = add2(sum[0], sum[1]);
                             l += both.x + both.y;
                         }
