@@ -143,6 +143,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+// tanh x = 1 - 2 / (e^2x + 1), off by at most 2^-21 (2 units in the last place of
+// the exponential and one of the reciprocal, of a term up to 2): that much of
+// the cap is far below a rounding of the weights.
+__device__ __forceinline__ float tanh_fast(float x) {
+    return 1.f - __fdividef(2.f, exp2_fast(x * (2.f * kLog2e)) + 1.f);
+}
 // True on one lane of a converged warp.  Branches on it, with addresses that are
 // the same on every lane, keep what a matrix instruction takes in uniform registers.
 __device__ __forceinline__ bool elect_one() {
@@ -573,7 +579,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
 #pragma unroll
                                         for (int i = 0; i < 16; ++i) {
                                             float x = s[i] * a.pre;
-                                            if (a.post != 0.f) x = a.post * tanhf(x);
+                                            if (a.post != 0.f) x = a.post * tanh_fast(x);
                                             s[i] = a.bias_near ? fmaf(slope, static_cast<float>(j0 + col + i - pos), x) : x;
                                         }
 #pragma unroll
