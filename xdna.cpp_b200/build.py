@@ -25,7 +25,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CU_SOURCES = ["gemv.cu", "gemv_mma.cu", "repack.cu", "quantize.cu", "kv_plan.cu", "qk_norm_rope.cu",
               "paged_attention.cu", "paged_stream.cu", "paged_chunk.cu"]
 CXX_SOURCES = ["backend.cpp", "paged_api.cpp"]
-HEADERS = ["formats.cuh", "gemv.cuh", "nccl_shim.h", "paged.cuh", "paged_attn.cuh", "paged_split.cuh", "paged_tma.cuh"]
+HEADERS = ["formats.cuh", "gemv.cuh", "nccl_shim.h", "paged.cuh", "paged_attn.cuh", "paged_split.cuh", "paged_tma.cuh",
+           "paged_walk.cuh"]
 
 
 def _stale(target: str, deps: list[str]) -> bool:

@@ -34,6 +34,7 @@
 
 #include "paged_split.cuh"
 #include "paged_tma.cuh"
+#include "paged_walk.cuh"
 
 namespace xb {
 namespace {
@@ -174,77 +175,7 @@ __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* u) {
         "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
         : "memory");
 }
-// ------------------------------------------------------------------ the work list
-// Key tiles [t0, t1) of row tile `tile`, and of one of its query tiles.
-template <int R>
-__device__ __forceinline__ void item_tiles(const AttnArgs& a, const Request& rq, int rows, int tile, int& t0, int& t1,
-                                           int& hi) {
-    int lo;
-    key_range(a, rq, tile * R / a.group, (min(tile * R + R, rows) - 1) / a.group, lo, hi);
-    t0 = lo / kKeys;
-    t1 = max(t0 + 1, (hi + kKeys - 1) / kKeys);
-}
-template <int R>
-__device__ __forceinline__ int item_units(const AttnArgs& a, const Request& rq, int rows, int tile) {
-    int t0, t1, hi;
-    item_tiles<R>(a, rq, rows, tile, t0, t1, hi);
-    return t1 - t0;
-}
-__device__ __forceinline__ long long warp_sum(long long v) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    return v;
-}
-// Units of all row tiles of one request (the same one on every lane), for one KV head.
-template <int R>
-__device__ __forceinline__ long long request_units(const AttnArgs& a, const Request& rq, int rows) {
-    const int lane = threadIdx.x & 31, tiles = (rows + R - 1) / R;
-    long long n = 0;
-    for (int t = lane; t < tiles; t += 32) n += item_units<R>(a, rq, rows, t);
-    return warp_sum(n);
-}
-
-// Walks the items of a CTA's run; all lanes of a warp hold the same values.
-struct Walk {
-    int b, kvh, tile;
-    Request rq;
-    int rows, tiles;
-    int t0, t1, hi;   // the item's key tiles, and the end of its keys
-    int s0, s1;       // those of this run
-    long long left;   // units of the run from s0 on
-
-    template <int R>
-    __device__ __forceinline__ void enter_request(const AttnArgs& a) {
-        rq = read_request(a, b);
-        rows = my_rows(a, rq);
-        tiles = (rows + R - 1) / R;
-    }
-    template <int R>
-    __device__ __forceinline__ void enter_item(const AttnArgs& a, int skip) {
-        item_tiles<R>(a, rq, rows, tile, t0, t1, hi);
-        s0 = t0 + skip;
-        s1 = static_cast<int>(min(static_cast<long long>(t1), s0 + left));
-    }
-    // The next item of the run; false at its end.
-    template <int R>
-    __device__ __forceinline__ bool next(const AttnArgs& a) {
-        left -= s1 - s0;
-        if (left <= 0) return false;
-        if (++tile == tiles) {
-            tile = 0;
-            if (++kvh == a.kv.kv_heads) {
-                kvh = 0;
-                do {
-                    ++b;
-                    enter_request<R>(a);
-                } while (!rows);
-            }
-        }
-        enter_item<R>(a, 0);
-        return true;
-    }
-};
-
+// ----------------------------------------------------------------- query tiles
 // The key tiles of query tile q that fall into [s0, s1): [lo, hi), empty when lo == hi.
 __device__ __forceinline__ void query_tiles(const AttnArgs& a, const Walk& w, int r0, int& lo, int& hi) {
     lo = hi = 0;
@@ -263,15 +194,14 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
     constexpr int R = L::kRows;
     extern __shared__ uint8_t raw[];
     __shared__ Bars bars;
-    __shared__ long long before[L::kThreads + 1];
-    __shared__ long long warp_units[L::kThreads / 32];
+    __shared__ RunUnits<L::kThreads> units;
     __shared__ uint32_t tmem_slot;
     __shared__ int dead_word;
     __shared__ volatile int turns[8 * L::kQ];  // key tiles whose weights a softmax warp has formed
     __shared__ float swap[L::kQ][2][2][128];   // what the two halves of a row tell each other, twice
     volatile int* dead = &dead_word;
     const AttnArgs& a = c.g.a;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.p.n_seqs;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kLoadWarp = L::kQ * 8, kMmaWarp = kLoadWarp + 2;  // two of each (one query tile: one kMmaWarp)
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     const uint32_t qs = base, ks = qs + L::kQ * L::kTile, vs = ks + L::kStages * L::kTile;
@@ -303,96 +233,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
     }
     grid_wait();
 
-    // units of all requests, summed up over the threads
-    const int per = (B + L::kThreads - 1) / L::kThreads;
-    {
-        long long mine = 0;
-        for (int i = 0; i < per; ++i) {
-            const int b = tid * per + i;
-            Request rq{0, 0, 0};
-            int rows = 0;
-            if (b < B) {
-                rq = read_request(a, b);
-                rows = my_rows(a, rq);
-            }
-            const int tiles = (rows + R - 1) / R;
-            long long n = 0;
-            if (tiles <= 4)
-                for (int t = 0; t < tiles; ++t) n += item_units<R>(a, rq, rows, t);
-            for (unsigned big = __ballot_sync(0xffffffffu, tiles > 4); big; big &= big - 1) {
-                const int from = __ffs(big) - 1;  // a long request: its row tiles over all lanes
-                Request r{__shfl_sync(0xffffffffu, rq.first, from), __shfl_sync(0xffffffffu, rq.count, from),
-                          __shfl_sync(0xffffffffu, rq.kv, from)};
-                const long long s = request_units<R>(a, r, __shfl_sync(0xffffffffu, rows, from));
-                if (lane == from) n = s;
-            }
-            mine += n * a.kv.kv_heads;
-        }
-        long long inc = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const long long o = __shfl_up_sync(0xffffffffu, inc, d);
-            if (lane >= d) inc += o;
-        }
-        if (lane == 31) warp_units[warp] = inc;
-        tc_before();
-        __syncthreads();
-        tc_after();
-        for (int w = 0; w < warp; ++w) inc += warp_units[w];
-        before[tid + 1] = inc;
-        if (tid == 0) before[0] = 0;
-        __syncthreads();
-    }
+    tc_before();
+    Run run;
+    start_run<R, kKeys, L::kThreads>(a, gridDim.x, kMinTiles, units, run);
+    tc_after();
     const uint32_t tmem = tmem_slot;
-    const long long all = before[L::kThreads];
-    const long long streams = min(static_cast<long long>(gridDim.x), max(1LL, all / kMinTiles));
     const long long me = blockIdx.x;
     if (tid == 0) c.g.heads[me].parts = 0;
-    const bool working = me < streams && all > 0;
 
-    if (working) {
-        // the first item of the run
-        const long long u0 = all * me / streams, u1 = all * (me + 1) / streams;
-        Walk w;
-        long long item0;  // units before the first item
-        {
-            int lo = 0, hi = L::kThreads;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (before[mid] <= u0) lo = mid; else hi = mid;
-            }
-            long long u = before[lo], one = 0;
-            for (w.b = lo * per;; ++w.b) {
-                w.enter_request<R>(a);
-                one = request_units<R>(a, w.rq, w.rows);
-                if (u0 < u + one * a.kv.kv_heads) break;
-                u += one * a.kv.kv_heads;
-            }
-            w.kvh = static_cast<int>((u0 - u) / one);
-            u += one * w.kvh;
-            for (w.tile = 0;; w.tile += 32) {  // 32 row tiles at a time
-                const int t = w.tile + lane;
-                const long long n = t < w.tiles ? item_units<R>(a, w.rq, w.rows, t) : 0;
-                long long inc = n;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const long long o = __shfl_up_sync(0xffffffffu, inc, d);
-                    if (lane >= d) inc += o;
-                }
-                const unsigned hit = __ballot_sync(0xffffffffu, u0 < u + inc);
-                if (hit) {
-                    const int at = __ffs(hit) - 1;
-                    u += __shfl_sync(0xffffffffu, inc - n, at);
-                    w.tile += at;
-                    break;
-                }
-                u += __shfl_sync(0xffffffffu, inc, 31);
-            }
-            item0 = u;
-            w.left = u1 - u0;
-            w.enter_item<R>(a, static_cast<int>(u0 - u));
-        }
-
+    if (run.units) {
+        Walk w = run.first;
         if (warp >= kLoadWarp) {
         if constexpr (L::kQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegs));
         if (warp < kMmaWarp) {
@@ -427,7 +277,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                         __syncwarp();
                     }
                 }
-            } while (ok && w.next<R>(a));
+            } while (ok && w.next<R, kKeys>(a));
             if (!ok)  // copies in flight land before the CTA ends
                 for (uint32_t i = n < L::kStages ? 0 : n - L::kStages; i < n; ++i)
                     bar_wait(&full[i % L::kStages], (i / L::kStages) & 1, nullptr);
@@ -492,7 +342,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                     __syncwarp();
                 }
                 --i;  // the last step has no tile of its own
-            } while (ok && w.next<R>(a));
+            } while (ok && w.next<R, kKeys>(a));
             if (!ok) {  // matrix instructions in flight end before TMEM is freed
                 if (elect_one()) tc_commit(&bars.drain[q]);
                 __syncwarp();
@@ -730,9 +580,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                     }
                 }
                 if (tid == 0 && w.s0 == w.t0 && w.s1 < w.t1) {
-                    // only the run's last item goes on in the next stream
-                    const long long end = first_item ? item0 + (w.t1 - w.t0) : u1 + (w.t1 - w.s1);
-                    c.g.heads[me] = SplitHead{w.b, w.kvh, w.tile, static_cast<int>(stream_of(end - 1, all, streams) - me + 1)};
+                    c.g.heads[me] = run.head(w, first_item, me);
                 }
                 first_item = false;
                 int lo, hi;
@@ -741,7 +589,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                 if (L::kQ == 2) query_tiles(a, w, w.tile * R + (q ^ 1) * 128, lo, hi);
                 theirs += hi - lo;
                 n += w.s1 - w.s0;
-            } while (w.next<R>(a));
+            } while (w.next<R, kKeys>(a));
         }
     }
 

@@ -67,11 +67,6 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile 
     return __all_sync(0xffffffffu, bar_wait_one(b, parity, dead));
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
                                         int c3) {
     asm volatile(
