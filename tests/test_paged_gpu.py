@@ -424,6 +424,71 @@ def test_paged_attention_size_of_scores(cuda, G, new, q_type, cache_type):
         near(out, ref, torch.nan_to_num(bound, posinf=100.0), f"size {size}")
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("q_type,cache_type", TYPES)
+def test_paged_attention_scale_not_positive(cuda, G, new, scale, q_type, cache_type):
+    g = gen(7)
+    c = Cache(G, 10, 2, 16, 128, cache_type)
+    ids = list(range(9))
+    c.put(ids, normal(g, 140, 2, 128), normal(g, 140, 2, 128))
+    q = normal(g, new, 4, 128).to(q_type)
+    out = torch.zeros_like(q)
+    run_attention(G, q, out, c, ints([0, new]), ints([140]), ints([ids]), scale)
+    torch.cuda.synchronize()
+    k, v = c.get(ids, 140)
+    ref, bound = attention_ref(q, k, v, 140 - new, scale, weight_half=0.0 if q_type == F32 else HALF[cache_type])
+    near(out, ref, bound, f"scale {scale}")
+
+
+@pytest.mark.parametrize("max_kv", [200, 100000])
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("q_type,cache_type", TYPES)
+def test_paged_attention_nan_stays_in_its_request(cuda, G, new, max_kv, q_type, cache_type):
+    """A NaN key or query makes the rows that see it NaN, and no row of another request."""
+    g = gen(8)
+    lens = [150, 150, 150, 33]
+    lists, table, blocks = spread_tables(lens, 16, seed=3)
+    c = Cache(G, blocks, 2, 16, 64, cache_type)
+    for n, ids in zip(lens, lists):
+        c.put(ids, normal(g, n, 2, 64), normal(g, n, 2, 64))
+    at = 150 - new // 2 - 1  # request 0: a key that half of the rows see
+    c.k[lists[0][at // 16], 0, at % 16, 5] = math.nan
+    c.k[lists[3][:1], :] = math.nan  # request 3: its first 16 keys
+    n3 = min(new, 33)
+    cu = ints([0, new, 2 * new, 3 * new, 3 * new + n3])
+    q = normal(g, 3 * new + n3, 6, 64).to(q_type)
+    q[2 * new] = math.nan  # request 2: its first row
+    out = torch.zeros_like(q)
+    run_attention(G, q, out, c, cu, ints(lens), table, 0.125, max_kv=max_kv)
+    torch.cuda.synchronize()
+    first = at - (150 - new)
+    assert out[max(first, 0): new, :3].isnan().all() and not out[: max(first, 0), :3].isnan().any()
+    assert not out[:new, 3:].isnan().any()
+    assert out[2 * new].isnan().all() and not out[2 * new + 1: 3 * new].isnan().any()
+    assert out[3 * new:].isnan().all()
+    k, v = c.get(lists[1], 150)
+    ref, bound = attention_ref(q[new: 2 * new], k, v, 150 - new, 0.125,
+                               weight_half=0.0 if q_type == F32 else HALF[cache_type])
+    near(out[new: 2 * new], ref, bound, "request 1")
+
+
+@pytest.mark.parametrize("q_type,cache_type", TYPES)
+def test_paged_attention_largest_hints(cuda, G, q_type, cache_type):
+    """Hints at the ends of their range choose a work split, nothing else."""
+    for hints in (dict(max_new=2 ** 31 - 1, max_kv=2 ** 31 - 1), dict(max_new=0, max_kv=2 ** 31 - 1),
+                  dict(max_new=2 ** 31 - 1, max_kv=0)):
+        check_attention(G, [(90, 1), (200, 20), (64, 64)], 8, 2, 64, q_type, cache_type, 32, seed=9, **hints)
+
+
+def test_paged_attention_many_requests(cuda, G):
+    """More requests than any kernel has threads."""
+    lens = [(1 + (i * 37) % 70, 1) for i in range(700)]
+    check_attention(G, lens, 4, 2, 64, F16, F16, 16, seed=13)
+    check_attention(G, lens[:400] + [(300, 90)], 4, 2, 64, BF16, BF16, 16, seed=14)
+    check_attention(G, lens[:400] + [(300, 90)], 4, 2, 64, F32, F16, 16, seed=15)
+
+
 @pytest.mark.parametrize("new", [1, 3, 70])
 @pytest.mark.parametrize("q_type,cache_type", TYPES)
 def test_paged_attention_graph_replay(cuda, G, new, q_type, cache_type):

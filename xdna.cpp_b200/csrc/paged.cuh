@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/ggml-b200.h"
 
 namespace xb {
@@ -24,6 +26,19 @@ cudaError_t paged_attention_launch(const struct b200_paged_attention_args& p, co
 // Reads and clears the current device's error word of the attention kernels'
 // bounded waits.
 cudaError_t paged_error_status(int* out);
+
+// Lets a kernel have `bytes` of dynamic shared memory; asked of the runtime once
+// per device.
+template <auto kKernel>
+cudaError_t allow_smem(int bytes) {
+    static std::atomic<uint64_t> done{0};  // a bit for each device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    return e;
+}
 
 // Launch with programmatic stream serialization: the kernel may start while
 // the one before it on the stream drains.  Every thread of every kernel

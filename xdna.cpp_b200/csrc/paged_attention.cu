@@ -297,9 +297,8 @@ template <typename T, int D>
 cudaError_t launch_tile(const AttnArgs& a, cudaStream_t stream) {
     constexpr int NP = Half16<T>::kPieces;
     using L = Tile<D, NP>;
-    const auto kernel = attn_tile_kernel<T, D, NP>;
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(L::kBytes));
+    constexpr auto kernel = attn_tile_kernel<T, D, NP>;
+    const cudaError_t e = allow_smem<kernel>(static_cast<int>(L::kBytes));
     if (e != cudaSuccess) return e;
     const int streams = tile_streams<D, NP>();
     const SplitArgs g = split_args(a, streams);

@@ -605,8 +605,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
 template <typename T, int D, bool kGeneral>
 cudaError_t launch_form(const ChunkArgs& c, cudaStream_t stream) {
     using L = Shape<D>;
-    const auto kernel = attn_chunk_kernel<T, D, kGeneral>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    constexpr auto kernel = attn_chunk_kernel<T, D, kGeneral>;
+    const cudaError_t e = allow_smem<kernel>(L::kSmem);
     if (e != cudaSuccess) return e;
     const unsigned sms = static_cast<unsigned>(sm_count());
     const cudaError_t f = launch_pdl(kernel, dim3(sms), dim3(L::kThreads), L::kSmem, stream, 1, c);

@@ -105,8 +105,8 @@ __device__ __forceinline__ void cluster_join(const AttnArgs& a, const Request& r
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float m = part(w)[R * D + r];
-            if (m == -INFINITY) continue;  // its sums are not written
-            const float c = exp2f(m - top[i]);
+            if (part(w)[R * D + R + r] == 0.f) continue;  // no key seen; a warp without units wrote no sums
+            const float c = top[i] == -INFINITY ? 1.f : exp2f(m - top[i]);
             sum[i] = fmaf(c, part(w)[R * D + R + r], sum[i]);
             o[i] = fmaf(c, part(w)[x], o[i]);
         }
@@ -590,13 +590,16 @@ size_t workspace_of(int R) {
 // The joining form is taken where its clusters fit on the SMs at once and no
 // warp gets a long run.
 struct Items {
-    int64_t tiles, count;  // row tiles of a request, items of the call (as the hints have it)
+    int tiles;      // row tiles of a request (as the hints have it)
+    int64_t count;  // items of the call, 2^40 at most
     bool join;
 };
 Items count_items(const AttnArgs& a, int R) {
     Items i;
-    i.tiles = std::max<int64_t>(1, (static_cast<int64_t>(a.p.max_new) * a.group + R - 1) / R);
-    i.count = i.tiles * a.p.n_seqs * a.kv.kv_heads;
+    const int64_t rows = std::min<int64_t>(a.p.max_new, a.p.n_tokens) * a.group;  // < 2^31
+    i.tiles = static_cast<int>(std::max<int64_t>(1, (rows + R - 1) / R));
+    i.count = static_cast<int64_t>(
+        std::min(static_cast<double>(i.tiles) * a.p.n_seqs * a.kv.kv_heads, static_cast<double>(int64_t(1) << 40)));
     i.join = i.count * kCluster <= sm_count() && a.p.max_kv <= kJoinKeys;
     return i;
 }
@@ -604,9 +607,8 @@ Items count_items(const AttnArgs& a, int R) {
 template <typename T, int D, int NP, int NT, bool kJoin>
 cudaError_t launch_form(const StreamArgs& c, int ctas, cudaStream_t stream) {
     using L = Ring<D>;
-    const auto kernel = attn_stream_kernel<T, D, NP, NT, kJoin>;
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    constexpr auto kernel = attn_stream_kernel<T, D, NP, NT, kJoin>;
+    const cudaError_t e = allow_smem<kernel>(L::kBytes);
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, dim3(ctas), dim3(L::kThreads), L::kBytes, stream, kJoin ? kCluster : 1, c);
 }
@@ -622,10 +624,10 @@ cudaError_t launch_rows(const AttnArgs& a, cudaStream_t stream) {
     c.box_tokens = std::min(a.kv.block_size, L::kKeys);
     if (!cache_map(&c.k, a.kv, a.kv.k, c.box_tokens) || !cache_map(&c.v, a.kv, a.kv.v, c.box_tokens))
         return cudaErrorInvalidValue;
-    g.tiles = static_cast<int>(items.tiles);
+    g.tiles = items.tiles;
     if (items.join) return launch_form<T, D, NP, NT, true>(c, static_cast<int>(items.count) * kCluster, stream);
     // no more streams than the hints give work for
-    const int64_t units = items.count * std::max(1, (a.p.max_kv + L::kKeys - 1) / L::kKeys);
+    const int64_t units = std::min<int64_t>(items.count, 1 << 30) * std::max<int64_t>(1, (int64_t(a.p.max_kv) + L::kKeys - 1) / L::kKeys);
     g.streams = static_cast<int>(std::min<int64_t>(sms * L::kWarps, std::max<int64_t>(1, units / kMinUnits)));
     const cudaError_t e = launch_form<T, D, NP, NT, false>(c, std::min(sms, g.streams), stream);
     if (e != cudaSuccess) return e;
