@@ -13,7 +13,7 @@
 //                            than the matrix unit)
 //   one warp each            TMA loads of K and of V, page by page, into rings
 // While one query tile is in its softmax the matrix unit works on the other
-// one.  O is rescaled only when a row's maximum grows by more than 8 (weights
+// one: their warps take turns in the exponentials.  O is rescaled only when a row's maximum grows by more than 8 (weights
 // stay below 2^8), which a vote of the warp finds out.  The weights are rounded
 // to 16 bits (the cache's type) because the matrix unit takes both factors in
 // one type; scores, sums and O are F32.
@@ -30,6 +30,15 @@
 // Every wait is bounded (2 s of %globaltimer): one that runs out sets the error
 // word, all roles give up, copies and matrix instructions in flight are waited
 // for (bounded again), and TMEM is freed.
+//
+// Measured on a B200: 4096 rows of 32 heads of 128, BF16, over 16384 keys: 850 us in
+// short bursts (1.13 PFLOP/s), 960 to 1000 us under the power cap; matrix pipe 53 %,
+// exponential unit 54 %, issue 49 %.  A key tile of a query tile is one chain: S, the
+// maximum, its exchange between the halves of a row, the exponentials, O and the
+// next S (about 4000 clocks, of which the matrix unit has 1024 for each query tile),
+// and two query tiles fill TMEM.  Tried and slower: 64-key tiles with two buffers
+// of S (923 us in bursts), a whole row per thread (1044 against 1013 us), a share of
+// the exponentials by a polynomial (every share), turns by an mbarrier (1115 us).
 #include <algorithm>
 
 #include "paged_split.cuh"
