@@ -16,8 +16,9 @@
 // warp's item: its loads are in flight together, at constant distances from one
 // address, and the norm weights, sines and cosines are fetched once for all of
 // them (with kind and address worked out for every step, instructions bound the
-// pass: 8191 tokens of 48 bf16 rows of 128 took 54 us at 69 % of the issue slots,
-// now 46 us, 4.4 TB/s, at 52 %; more warps with fewer registers were no faster).
+// pass: 8191 tokens of 48 bf16 rows of 128 took 54 us at 69 % of the issue slots;
+// now they take 43 us, 4.7 TB/s.  More warps with fewer registers, deeper loads and
+// sines formed once per CTA were no faster.)
 // One or more warps share a token's chunks; each forms the token's sines and
 // cosines in shared memory while its first chunk is on its way, and has the next
 // chunk in flight while it works on one.
@@ -36,7 +37,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = 24;  // resident on an SM
-constexpr int kRounds = 4;
+constexpr int kRounds = 5;
 constexpr int kMaxPairs = 128;
 
 struct Turns {
@@ -83,6 +84,24 @@ struct Chunk<__nv_bfloat16> {
     }
 };
 
+// The pairs that turn together, of a lane's two chunks, and back.
+template <bool kNeox>
+__device__ __forceinline__ void pairs(const float (&x)[4], const float (&y)[4], float (&u)[4], float (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        u[e] = kNeox ? x[e] : e < 2 ? x[2 * e] : y[2 * e - 4];
+        v[e] = kNeox ? y[e] : e < 2 ? x[2 * e + 1] : y[2 * e - 3];
+    }
+}
+template <bool kNeox>
+__device__ __forceinline__ void unpair(const float (&u)[4], const float (&v)[4], float (&x)[4], float (&y)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[e] = kNeox ? u[e] : e & 1 ? v[e / 2] : u[e / 2];
+        y[e] = kNeox ? v[e] : e & 1 ? v[2 + e / 2] : u[2 + e / 2];
+    }
+}
+
 struct RopeArgs {
     struct b200_qk_norm_rope_args p;
     struct b200_kv_cache kv;
@@ -100,7 +119,8 @@ struct Rows {
     static constexpr int kPerChunk = kPerStep * kDeep;
 };
 
-template <typename In, typename Out, typename Cache, int D>
+// kNeox: the pairs are (i, i + n / 2), else (2 i, 2 i + 1).
+template <typename In, typename Out, typename Cache, int D, bool kNeox>
 __global__ void __launch_bounds__(kThreads, 768 / kThreads) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a,
                                                                              const __grid_constant__ Turns turns) {
     using L = Rows<In, D>;
@@ -114,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) qk_norm_rope_kernel(
     // the lane's two chunks of a row, and whether they turn
     const bool turn = on && 8 * l < n;
     int c0 = 8 * l, c1 = 8 * l + 4;
-    if (p.neox && turn) c0 = 4 * l, c1 = half + 4 * l;
+    if (kNeox && turn) c0 = 4 * l, c1 = half + 4 * l;
     if (!on) c0 = c1 = 0;
 
     const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + warp;
@@ -167,14 +187,6 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) qk_norm_rope_kernel(
         const bool more = x_chunk + a.parts < chunks;
         if (more) fetch(x_chunk + a.parts, next_x, next_y);
 
-        const float* w = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
-        float4 wx, wy, cv, sv;
-        if (w) wx = *reinterpret_cast<const float4*>(w + c0), wy = *reinterpret_cast<const float4*>(w + c1);
-        const bool turns_here = turn && kind != 2;
-        if (turns_here) {
-            cv = *reinterpret_cast<const float4*>(&cosine[warp][4 * l]);
-            sv = *reinterpret_cast<const float4*>(&sine[warp][4 * l]);
-        }
         // where the rows go: the distance of heads in q_out, or in the cache
         char* dst = static_cast<char*>(p.q_out) + t * p.nb_q_out + h0 * D * static_cast<int>(sizeof(Out));
         int64_t step = L::kPerStep * D * static_cast<int>(sizeof(Out));
@@ -186,50 +198,67 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) qk_norm_rope_kernel(
                   (slot & (a.kv.block_size - 1)) * a.kv.nb_token + h0 * a.kv.nb_head;
             step = L::kPerStep * a.kv.nb_head;
         }
+        if (kind == 2) {
 #pragma unroll
-        for (int u = 0; u < L::kDeep; ++u) {
-            float x[4], y[4];
-            Chunk<In>::get(raw_x[u], x);
-            Chunk<In>::get(raw_y[u], y);
-            if (w) {
-                float ss = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
-#pragma unroll
-                for (int d = L::kGroup / 2; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-                const float inv = rsqrtf(fmaf(ss, 1.0f / D, p.eps));  // 2 units in the last place
-                x[0] *= inv * wx.x, x[1] *= inv * wx.y, x[2] *= inv * wx.z, x[3] *= inv * wx.w;
-                y[0] *= inv * wy.x, y[1] *= inv * wy.y, y[2] *= inv * wy.z, y[3] *= inv * wy.w;
-            }
-            if (turns_here) {
-                const float c[4] = {cv.x, cv.y, cv.z, cv.w}, s[4] = {sv.x, sv.y, sv.z, sv.w};
-                if (p.neox) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float v0 = x[e], v1 = y[e];
-                        x[e] = v0 * c[e] - v1 * s[e];
-                        y[e] = v0 * s[e] + v1 * c[e];
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float v0 = x[2 * e], v1 = x[2 * e + 1];
-                        x[2 * e] = v0 * c[e] - v1 * s[e];
-                        x[2 * e + 1] = v0 * s[e] + v1 * c[e];
-                        v0 = y[2 * e], v1 = y[2 * e + 1];
-                        y[2 * e] = v0 * c[e + 2] - v1 * s[e + 2];
-                        y[2 * e + 1] = v0 * s[e + 2] + v1 * c[e + 2];
-                    }
+            for (int u = 0; u < L::kDeep; ++u) {
+                float x[4], y[4];
+                Chunk<In>::get(raw_x[u], x);
+                Chunk<In>::get(raw_y[u], y);
+                if (stored && h0 + u * L::kPerStep < heads) {
+                    Chunk<Cache>::store(dst + u * step + c0 * sizeof(Cache), x);
+                    Chunk<Cache>::store(dst + u * step + c1 * sizeof(Cache), y);
                 }
             }
-            if (stored && h0 + u * L::kPerStep < heads) {
-                char* to = dst + u * step;
-                if (kind == 0) {
-                    Chunk<Out>::store(to + c0 * sizeof(Out), x);
-                    Chunk<Out>::store(to + c1 * sizeof(Out), y);
-                } else {
-                    Chunk<Cache>::store(to + c0 * sizeof(Cache), x);
-                    Chunk<Cache>::store(to + c1 * sizeof(Cache), y);
+        } else {
+            // The pairs (u, v) of a lane, with the norm's weights in the rotation's
+            // coefficients: u' = inv (u uc - v vs), v' = inv (u us + v vc).
+            const float* w = kind == 0 ? p.q_norm : p.k_norm;
+            float uc[4], vc[4], us[4] = {}, vs[4] = {};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) uc[e] = vc[e] = 1.f;
+            if (w) {
+                const float4 wx = *reinterpret_cast<const float4*>(w + c0), wy = *reinterpret_cast<const float4*>(w + c1);
+                const float x[4] = {wx.x, wx.y, wx.z, wx.w}, y[4] = {wy.x, wy.y, wy.z, wy.w};
+                pairs<kNeox>(x, y, uc, vc);
+            }
+            if (turn) {
+                const float4 cv = *reinterpret_cast<const float4*>(&cosine[warp][4 * l]);
+                const float4 sv = *reinterpret_cast<const float4*>(&sine[warp][4 * l]);
+                const float c[4] = {cv.x, cv.y, cv.z, cv.w}, s[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) us[e] = uc[e] * s[e], vs[e] = vc[e] * s[e], uc[e] *= c[e], vc[e] *= c[e];
+            }
+#pragma unroll
+            for (int r = 0; r < L::kDeep; ++r) {
+                float x[4], y[4], u[4], v[4];
+                Chunk<In>::get(raw_x[r], x);
+                Chunk<In>::get(raw_y[r], y);
+                pairs<kNeox>(x, y, u, v);
+                float inv = 1.f;
+                if (w) {
+                    float ss = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ss = fmaf(u[e], u[e], fmaf(v[e], v[e], ss));
+#pragma unroll
+                    for (int d = L::kGroup / 2; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+                    inv = rsqrtf(fmaf(ss, 1.0f / D, p.eps));  // 2 units in the last place
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float p0 = u[e] * uc[e], p1 = v[e] * vc[e];
+                    if (turn) p0 = fmaf(-v[e], vs[e], p0), p1 = fmaf(u[e], us[e], p1);
+                    u[e] = p0 * inv, v[e] = p1 * inv;
+                }
+                unpair<kNeox>(u, v, x, y);
+                if (stored && h0 + r * L::kPerStep < heads) {
+                    char* to = dst + r * step;
+                    if (kind == 0) {
+                        Chunk<Out>::store(to + c0 * sizeof(Out), x);
+                        Chunk<Out>::store(to + c1 * sizeof(Out), y);
+                    } else {
+                        Chunk<Cache>::store(to + c0 * sizeof(Cache), x);
+                        Chunk<Cache>::store(to + c1 * sizeof(Cache), y);
+                    }
                 }
             }
         }
@@ -239,13 +268,18 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) qk_norm_rope_kernel(
     }
 }
 
+template <typename In, typename Out, typename Cache, int D>
+cudaError_t launch_pairs(const RopeArgs& a, const Turns& t, dim3 grid, cudaStream_t stream) {
+    return launch_pdl(a.p.neox ? qk_norm_rope_kernel<In, Out, Cache, D, true> : qk_norm_rope_kernel<In, Out, Cache, D, false>,
+                      grid, dim3(kThreads), 0, stream, 1, a, t);
+}
 template <typename In, typename Out, typename Cache>
 cudaError_t launch_dim(const RopeArgs& a, const Turns& t, dim3 grid, cudaStream_t stream) {
     switch (a.kv.head_dim) {
-        case 64: return launch_pdl(qk_norm_rope_kernel<In, Out, Cache, 64>, grid, kThreads, 0, stream, 1, a, t);
-        case 96: return launch_pdl(qk_norm_rope_kernel<In, Out, Cache, 96>, grid, kThreads, 0, stream, 1, a, t);
-        case 128: return launch_pdl(qk_norm_rope_kernel<In, Out, Cache, 128>, grid, kThreads, 0, stream, 1, a, t);
-        default: return launch_pdl(qk_norm_rope_kernel<In, Out, Cache, 256>, grid, kThreads, 0, stream, 1, a, t);
+        case 64: return launch_pairs<In, Out, Cache, 64>(a, t, grid, stream);
+        case 96: return launch_pairs<In, Out, Cache, 96>(a, t, grid, stream);
+        case 128: return launch_pairs<In, Out, Cache, 128>(a, t, grid, stream);
+        default: return launch_pairs<In, Out, Cache, 256>(a, t, grid, stream);
     }
 }
 template <typename In, typename Out>
