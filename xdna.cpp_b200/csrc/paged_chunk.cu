@@ -153,11 +153,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// tanh x = 1 - 2 / (e^2x + 1), off by at most 2^-21 (2 units in the last place of
-// the exponential and one of the reciprocal, of a term up to 2): that much of
-// the cap is far below a rounding of the weights.
-__device__ __forceinline__ float tanh_fast(float x) {
-    return 1.f - __fdividef(2.f, exp2_fast(x * (2.f * kLog2e)) + 1.f);
+// post tanh(pre s), with tanh x = 1 - 2 / (e^2x + 1): off by at most 2^-21 of post
+// (2 units in the last place of the exponential and one of the reciprocal, of a
+// term up to 2), far below a rounding of the weights.
+__device__ __forceinline__ float capped(float s, float pre, float post) {
+    const float e = exp2_fast(s * (pre * (2.f * kLog2e)));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.f));
+    return fmaf(-2.f * post, r, post);
 }
 // True on one lane of a converged warp.  Branches on it, with addresses that are
 // the same on every lane, keep what a matrix instruction takes in uniform registers.
@@ -434,13 +437,19 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             float s0[16], s1[16], tops[8];
                             auto look = [&](float (&s)[16], int col) {
                                 if (kGeneral || cut) {
-                                    if (kGeneral)
+                                    if (kGeneral) {
+                                        if (a.post != 0.f)
 #pragma unroll
-                                        for (int i = 0; i < 16; ++i) {
-                                            float x = s[i] * a.pre;
-                                            if (a.post != 0.f) x = a.post * tanh_fast(x);
-                                            s[i] = a.bias_near ? fmaf(slope, static_cast<float>(j0 + col + i - pos), x) : x;
-                                        }
+                                            for (int i = 0; i < 16; ++i) s[i] = capped(s[i], a.pre, a.post);
+                                        else
+#pragma unroll
+                                            for (int i = 0; i < 16; ++i) s[i] *= a.pre;
+                                        if (a.bias_near)
+#pragma unroll
+                                            for (int i = 0; i < 16; ++i)
+                                                s[i] = fmaf(slope, static_cast<float>(j0 + col + i - pos), s[i]);
+                                    }
+                                    if (cut)
 #pragma unroll
                                     for (int i = 0; i < 16; ++i)
                                         if (i < k0 - col || i > k1 - col) s[i] = -INFINITY;
