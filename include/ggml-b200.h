@@ -361,7 +361,8 @@ struct b200_paged_attention_args {
     const int32_t *kv_lens;  /* [n_seqs] */
     const int32_t *block_table; /* [n_seqs][table_width] */
     int64_t table_width;
-    int32_t max_new, max_kv; /* the most of any request: they choose kernels and work split, not results */
+    int32_t max_new, max_kv; /* the most of any request: they choose kernels and work split; with others the
+                              * results differ by roundings only */
     float scale, logit_softcap, max_bias; /* 0: no cap, no bias */
     int32_t window;          /* 0: none */
     void *workspace;         /* device, 16-byte aligned, not shared by calls that may overlap in time */

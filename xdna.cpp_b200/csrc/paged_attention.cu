@@ -354,11 +354,13 @@ AttnArgs make_args(const struct b200_paged_attention_args& p, const struct b200_
 }  // namespace
 
 int sm_count() {
-    static int count[kMaxDevices];
+    static std::atomic<int> count[kMaxDevices];
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return 0;
-    if (!count[dev] && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) count[dev] = n;
-    return count[dev];
+    if ((n = count[dev].load(std::memory_order_relaxed)) == 0 &&
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
+        count[dev].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 // Requests of up to kStreamRows rows go to the stream kernel, the others to the
