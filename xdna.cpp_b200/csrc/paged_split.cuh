@@ -128,15 +128,16 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const __gri
 }
 
 // Launches combine_kernel after a kernel whose items are about `items` (as the
-// hints have it).
+// hints have it).  Few items have many parts each and leave most blocks nothing to
+// do: then a row is a CTA's (up to 32 rows an item) or a warp's, else a warp takes 4.
 template <int D, int R>
 cudaError_t combine_launch(const SplitArgs& g, int64_t items, cudaStream_t stream) {
-    const int streams = g.streams;
-    if (streams >= 8 * items)
-        return launch_pdl(combine_kernel<D, R, true>, dim3(streams, std::min(R, 8)), dim3(32 * kCombineWarps), 0, stream,
-                          1, g);
-    return launch_pdl(combine_kernel<D, R, false>, dim3(streams, (R + 31) / 32), dim3(32 * kCombineWarps), 0, stream, 1,
-                      g);
+    const bool few = g.streams >= 4 * items;
+    if (few && R <= 32)
+        return launch_pdl(combine_kernel<D, R, true>, dim3(g.streams, R), dim3(32 * kCombineWarps), 0, stream, 1, g);
+    const int rows = few ? kCombineWarps : 4 * kCombineWarps;  // of a block
+    return launch_pdl(combine_kernel<D, R, false>, dim3(g.streams, (R + rows - 1) / rows), dim3(32 * kCombineWarps), 0,
+                      stream, 1, g);
 }
 #endif
 
