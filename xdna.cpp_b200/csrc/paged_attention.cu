@@ -72,223 +72,223 @@ __global__ void __launch_bounds__(Tile<D, NP>::kThreads, Tile<D, NP>::kCtas)
     Walk w = run.first;
     bool first_item = true;
     do {
-    const Request rq = w.rq;
-    const int kvh = w.kvh, G = a.group, r0 = w.tile * kRows, rows = min(kRows, w.rows - r0);
-    const int lo = w.s0 * kKeys, hi = min(w.hi, w.s1 * kKeys);  // this run's keys of the item
+        const Request rq = w.rq;
+        const int kvh = w.kvh, G = a.group, r0 = w.tile * kRows, rows = min(kRows, w.rows - r0);
+        const int lo = w.s0 * kKeys, hi = min(w.hi, w.s1 * kKeys);  // this run's keys of the item
 
-    auto load = [&](int j0, int stage) {
-        constexpr int kChunks = D / 8;
+        auto load = [&](int j0, int stage) {
+            constexpr int kChunks = D / 8;
 #pragma unroll
-        for (int x = 0; x < kKeys * kChunks / kThreads; ++x) {
-            const int i = x * kThreads + tid, r = i / kChunks, c = i - r * kChunks, j = j0 + r;
-            const int id = j < hi ? key_block(a, w.b, j >> a.log_bs) : -1;
-            const int64_t at = id < 0 ? 0
-                                      : id * a.kv.nb_block + kvh * a.kv.nb_head +
-                                            (j & (a.kv.block_size - 1)) * a.kv.nb_token + c * 16;
-            const int d = stage * L::kK + r * kS + c * 8;
-            cp_async16(smem_addr(ks + d), static_cast<const char*>(a.kv.k) + at, id >= 0);
-            cp_async16(smem_addr(vs + d), static_cast<const char*>(a.kv.v) + at, id >= 0);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    if (lo < hi) load(lo, 0);
-
-    // the tile's queries, as NP pieces
-    for (int r = warp; r < kRows; r += L::kWarps) {
-        const bool on = r < rows;
-        const int i = (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
-        const char* src = static_cast<const char*>(a.p.q) + (rq.first + (on ? i : 0)) * a.p.nb_q;
-        const float2* s = reinterpret_cast<const float2*>(src) + static_cast<int64_t>(h) * (D / 2);
-        // F16 pieces reach down to 2^-24 only: the row is scaled by a power of
-        // two to a largest value in [1, 2)
-        float big = 0.f, up = 1.f;
-        if (NP == 2) {
-            for (int c = lane; on && c < D / 2; c += 32) big = fmaxf(big, fmaxf(fabsf(s[c].x), fabsf(s[c].y)));
-#pragma unroll
-            for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-            if (big > 0.f && big <= FLT_MAX) up = ldexpf(1.f, min(ilogbf(big), 126));
-        }
-        if (lane == 0) row_scale[r] = up;
-        const float down = 1.f / up;
-        for (int c = lane; c < D / 2; c += 32) {
-            const float2 x = on ? s[c] : make_float2(0.f, 0.f);
-            uint32_t piece[NP];
-            split_pair<T, NP>(x.x * down, x.y * down, piece);
-#pragma unroll
-            for (int k = 0; k < NP; ++k) *reinterpret_cast<uint32_t*>(qs + k * L::kQ + r * kS + 2 * c) = piece[k];
-        }
-    }
-    __syncthreads();
-
-    // this thread's two rows
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope[2], mul[2];
-    int p[2], last[2], row[2];  // position, last key it sees, row of the tile
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        row[e] = warp * 16 + (lane >> 2) + 8 * e;
-        const int i = (r0 + row[e]) / G;
-        p[e] = rq.pos0() + i;
-        last[e] = min(p[e], w.hi - 1);
-        slope[e] = head_slope(a, kvh * G + (r0 + row[e]) - i * G);
-        mul[e] = a.pre * row_scale[row[e]];
-    }
-    // keys [all_lo, all_hi) are seen by every row of the tile
-    const int p0 = rq.pos0() + r0 / G, p1 = rq.pos0() + (r0 + rows - 1) / G;
-    const int all_hi = min(p0 + 1, w.hi), all_lo = a.p.window > 0 && p1 >= a.p.window ? p1 - a.p.window + 1 : 0;
-    float o[D / 8][4];
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-
-    int stage = 0;
-    for (int j0 = lo; j0 < hi; j0 += kKeys, stage ^= 1) {
-        if (j0 + kKeys < hi) {
-            load(j0 + kKeys, stage ^ 1);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-        } else {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-        }
-        __syncthreads();
-        const uint16_t* kt = ks + stage * L::kK;
-        const uint16_t* vt = vs + stage * L::kK;
-
-        float s[kKeys / 8][4];
-#pragma unroll
-        for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-            uint32_t qf[NP][4];
-#pragma unroll
-            for (int i = 0; i < NP; ++i)
-                ldsm4(qf[i], smem_addr(qs + i * L::kQ + (warp * 16 + (lane & 15)) * kS + k * 16 + (lane >> 4) * 8));
-#pragma unroll
-            for (int n = 0; n < kKeys / 16; ++n) {
-                uint32_t kf[4];
-                ldsm4(kf, smem_addr(kt + (n * 16 + (lane & 7) + (lane >> 4) * 8) * kS + k * 16 + ((lane >> 3) & 1) * 8));
-#pragma unroll
-                for (int i = NP - 1; i >= 0; --i) {
-                    mma16816<T>(s[2 * n], qf[i], kf[0], kf[1]);
-                    mma16816<T>(s[2 * n + 1], qf[i], kf[2], kf[3]);
-                }
+            for (int x = 0; x < kKeys * kChunks / kThreads; ++x) {
+                const int i = x * kThreads + tid, r = i / kChunks, c = i - r * kChunks, j = j0 + r;
+                const int id = j < hi ? key_block(a, w.b, j >> a.log_bs) : -1;
+                const int64_t at = id < 0 ? 0
+                                          : id * a.kv.nb_block + kvh * a.kv.nb_head +
+                                                (j & (a.kv.block_size - 1)) * a.kv.nb_token + c * 16;
+                const int d = stage * L::kK + r * kS + c * 8;
+                cp_async16(smem_addr(ks + d), static_cast<const char*>(a.kv.k) + at, id >= 0);
+                cp_async16(smem_addr(vs + d), static_cast<const char*>(a.kv.v) + at, id >= 0);
             }
-        }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        if (lo < hi) load(lo, 0);
 
-        // scores in units of log 2, hidden keys at -inf
+        // the tile's queries, as NP pieces
+        for (int r = warp; r < kRows; r += L::kWarps) {
+            const bool on = r < rows;
+            const int i = (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
+            const char* src = static_cast<const char*>(a.p.q) + (rq.first + (on ? i : 0)) * a.p.nb_q;
+            const float2* s = reinterpret_cast<const float2*>(src) + static_cast<int64_t>(h) * (D / 2);
+            // F16 pieces reach down to 2^-24 only: the row is scaled by a power of
+            // two to a largest value in [1, 2)
+            float big = 0.f, up = 1.f;
+            if (NP == 2) {
+                for (int c = lane; on && c < D / 2; c += 32) big = fmaxf(big, fmaxf(fabsf(s[c].x), fabsf(s[c].y)));
 #pragma unroll
-        for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] *= mul[e >> 1];
-        if (a.post != 0.f)
-#pragma unroll
-            for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][e] = a.post * tanhf(s[n][e]);
-        if (a.bias_near)
-#pragma unroll
-            for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = j0 + n * 8 + 2 * (lane & 3) + (e & 1);
-                    s[n][e] = fmaf(slope[e >> 1], static_cast<float>(j - p[e >> 1]), s[n][e]);
-                }
-        if (j0 < all_lo || j0 + kKeys > all_hi)
-#pragma unroll
-            for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int q = e >> 1, j = j0 + n * 8 + 2 * (lane & 3) + (e & 1);
-                    if (j > last[q] || (a.p.window > 0 && p[q] - j >= a.p.window)) s[n][e] = -INFINITY;
-                }
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-        // the maximum moves only when a score passes it by kSlack (a weight is 2^kSlack at most)
-        if (__any_sync(0xffffffffu, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 1));
-                top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 2));
-                top[q] = fmaxf(top[q], m[q]);
-                const float c = top[q] == -INFINITY ? 1.f : exp2f(m[q] - top[q]);
-                m[q] = top[q];
-                l[q] *= c;
-#pragma unroll
-                for (int n = 0; n < D / 8; ++n) {
-                    o[n][2 * q] *= c;
-                    o[n][2 * q + 1] *= c;
-                }
+                for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+                if (big > 0.f && big <= FLT_MAX) up = ldexpf(1.f, min(ilogbf(big), 126));
             }
-        }
-        const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};  // no key yet: 0
-        uint32_t pf[kKeys / 16][NP][4];
-#pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float* x = &s[2 * k + (e >> 1)][2 * (e & 1)];
-                x[0] = exp2_fast(x[0] - base[e & 1]);
-                x[1] = exp2_fast(x[1] - base[e & 1]);
-                l[e & 1] += x[0] + x[1];
+            if (lane == 0) row_scale[r] = up;
+            const float down = 1.f / up;
+            for (int c = lane; c < D / 2; c += 32) {
+                const float2 x = on ? s[c] : make_float2(0.f, 0.f);
                 uint32_t piece[NP];
-                split_pair<T, NP>(x[0], x[1], piece);
+                split_pair<T, NP>(x.x * down, x.y * down, piece);
 #pragma unroll
-                for (int i = 0; i < NP; ++i) pf[k][i][e] = piece[i];
+                for (int k = 0; k < NP; ++k) *reinterpret_cast<uint32_t*>(qs + k * L::kQ + r * kS + 2 * c) = piece[k];
             }
-        // The matrix unit cuts its sums off instead of rounding them, which adds up
-        // over a long axis: every tile's sum starts at 0 and is added by a rounded
-        // addition.
-#pragma unroll
-        for (int n = 0; n < D / 16; ++n) {
-            float t[2][4] = {};
-#pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k) {
-                uint32_t vf[4];
-                ldsm4_t(vf, smem_addr(vt + (k * 16 + (lane & 15)) * kS + n * 16 + (lane >> 4) * 8));
-#pragma unroll
-                for (int i = NP - 1; i >= 0; --i) {
-                    mma16816<T>(t[0], pf[k][i], vf[0], vf[1]);
-                    mma16816<T>(t[1], pf[k][i], vf[2], vf[3]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[2 * n][e] += t[0][e], o[2 * n + 1][e] += t[1][e];
         }
         __syncthreads();
-    }
 
-    // the rows' output, or the item's partial
-    const bool whole = w.s0 == w.t0 && w.s1 == w.t1;
-    float* part = g.parts + (static_cast<size_t>(me) * 2 + (w.s0 == w.t0)) * part_floats(kRows, D);
+        // this thread's two rows
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, slope[2], mul[2];
+        int p[2], last[2], row[2];  // position, last key it sees, row of the tile
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        l[q] += __shfl_xor_sync(0xffffffffu, l[q], 1);
-        l[q] += __shfl_xor_sync(0xffffffffu, l[q], 2);
-        if (row[q] >= rows) continue;
-        const bool none = l[q] == 0.f;  // no key, or only scores of -inf
-        const float inv = whole ? 1.f / l[q] : 1.f;
-        const int i = (r0 + row[q]) / G, h = kvh * G + (r0 + row[q]) - i * G;
+        for (int e = 0; e < 2; ++e) {
+            row[e] = warp * 16 + (lane >> 2) + 8 * e;
+            const int i = (r0 + row[e]) / G;
+            p[e] = rq.pos0() + i;
+            last[e] = min(p[e], w.hi - 1);
+            slope[e] = head_slope(a, kvh * G + (r0 + row[e]) - i * G);
+            mul[e] = a.pre * row_scale[row[e]];
+        }
+        // keys [all_lo, all_hi) are seen by every row of the tile
+        const int p0 = rq.pos0() + r0 / G, p1 = rq.pos0() + (r0 + rows - 1) / G;
+        const int all_hi = min(p0 + 1, w.hi), all_lo = a.p.window > 0 && p1 >= a.p.window ? p1 - a.p.window + 1 : 0;
+        float o[D / 8][4];
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-            const int col = n * 8 + 2 * (lane & 3);
-            const float2 x = none ? make_float2(0.f, 0.f) : make_float2(o[n][2 * q] * inv, o[n][2 * q + 1] * inv);
-            if (whole)
-                store_out(a, rq.first + i, h, col, x.x, x.y);
-            else
-                *reinterpret_cast<float2*>(part + static_cast<size_t>(row[q]) * D + col) = x;
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+
+        int stage = 0;
+        for (int j0 = lo; j0 < hi; j0 += kKeys, stage ^= 1) {
+            if (j0 + kKeys < hi) {
+                load(j0 + kKeys, stage ^ 1);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            __syncthreads();
+            const uint16_t* kt = ks + stage * L::kK;
+            const uint16_t* vt = vs + stage * L::kK;
+
+            float s[kKeys / 8][4];
+#pragma unroll
+            for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                uint32_t qf[NP][4];
+#pragma unroll
+                for (int i = 0; i < NP; ++i)
+                    ldsm4(qf[i], smem_addr(qs + i * L::kQ + (warp * 16 + (lane & 15)) * kS + k * 16 + (lane >> 4) * 8));
+#pragma unroll
+                for (int n = 0; n < kKeys / 16; ++n) {
+                    uint32_t kf[4];
+                    ldsm4(kf, smem_addr(kt + (n * 16 + (lane & 7) + (lane >> 4) * 8) * kS + k * 16 + ((lane >> 3) & 1) * 8));
+#pragma unroll
+                    for (int i = NP - 1; i >= 0; --i) {
+                        mma16816<T>(s[2 * n], qf[i], kf[0], kf[1]);
+                        mma16816<T>(s[2 * n + 1], qf[i], kf[2], kf[3]);
+                    }
+                }
+            }
+
+            // scores in units of log 2, hidden keys at -inf
+#pragma unroll
+            for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] *= mul[e >> 1];
+            if (a.post != 0.f)
+#pragma unroll
+                for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][e] = a.post * tanhf(s[n][e]);
+            if (a.bias_near)
+#pragma unroll
+                for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = j0 + n * 8 + 2 * (lane & 3) + (e & 1);
+                        s[n][e] = fmaf(slope[e >> 1], static_cast<float>(j - p[e >> 1]), s[n][e]);
+                    }
+            if (j0 < all_lo || j0 + kKeys > all_hi)
+#pragma unroll
+                for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int q = e >> 1, j = j0 + n * 8 + 2 * (lane & 3) + (e & 1);
+                        if (j > last[q] || (a.p.window > 0 && p[q] - j >= a.p.window)) s[n][e] = -INFINITY;
+                    }
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+            // the maximum moves only when a score passes it by kSlack (a weight is 2^kSlack at most)
+            if (__any_sync(0xffffffffu, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 1));
+                    top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 2));
+                    top[q] = fmaxf(top[q], m[q]);
+                    const float c = top[q] == -INFINITY ? 1.f : exp2f(m[q] - top[q]);
+                    m[q] = top[q];
+                    l[q] *= c;
+#pragma unroll
+                    for (int n = 0; n < D / 8; ++n) {
+                        o[n][2 * q] *= c;
+                        o[n][2 * q + 1] *= c;
+                    }
+                }
+            }
+            const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};  // no key yet: 0
+            uint32_t pf[kKeys / 16][NP][4];
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float* x = &s[2 * k + (e >> 1)][2 * (e & 1)];
+                    x[0] = exp2_fast(x[0] - base[e & 1]);
+                    x[1] = exp2_fast(x[1] - base[e & 1]);
+                    l[e & 1] += x[0] + x[1];
+                    uint32_t piece[NP];
+                    split_pair<T, NP>(x[0], x[1], piece);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) pf[k][i][e] = piece[i];
+                }
+            // The matrix unit cuts its sums off instead of rounding them, which adds up
+            // over a long axis: every tile's sum starts at 0 and is added by a rounded
+            // addition.
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) {
+                float t[2][4] = {};
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; ++k) {
+                    uint32_t vf[4];
+                    ldsm4_t(vf, smem_addr(vt + (k * 16 + (lane & 15)) * kS + n * 16 + (lane >> 4) * 8));
+#pragma unroll
+                    for (int i = NP - 1; i >= 0; --i) {
+                        mma16816<T>(t[0], pf[k][i], vf[0], vf[1]);
+                        mma16816<T>(t[1], pf[k][i], vf[2], vf[3]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[2 * n][e] += t[0][e], o[2 * n + 1][e] += t[1][e];
+            }
+            __syncthreads();
         }
-        if (!whole && (lane & 3) == 0) {
-            part[kRows * D + row[q]] = m[q];
-            part[kRows * D + kRows + row[q]] = l[q];
+
+        // the rows' output, or the item's partial
+        const bool whole = w.s0 == w.t0 && w.s1 == w.t1;
+        float* part = g.parts + (static_cast<size_t>(me) * 2 + (w.s0 == w.t0)) * part_floats(kRows, D);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            l[q] += __shfl_xor_sync(0xffffffffu, l[q], 1);
+            l[q] += __shfl_xor_sync(0xffffffffu, l[q], 2);
+            if (row[q] >= rows) continue;
+            const bool none = l[q] == 0.f;  // no key, or only scores of -inf
+            const float inv = whole ? 1.f / l[q] : 1.f;
+            const int i = (r0 + row[q]) / G, h = kvh * G + (r0 + row[q]) - i * G;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+                const int col = n * 8 + 2 * (lane & 3);
+                const float2 x = none ? make_float2(0.f, 0.f) : make_float2(o[n][2 * q] * inv, o[n][2 * q + 1] * inv);
+                if (whole)
+                    store_out(a, rq.first + i, h, col, x.x, x.y);
+                else
+                    *reinterpret_cast<float2*>(part + static_cast<size_t>(row[q]) * D + col) = x;
+            }
+            if (!whole && (lane & 3) == 0) {
+                part[kRows * D + row[q]] = m[q];
+                part[kRows * D + kRows + row[q]] = l[q];
+            }
         }
-    }
-    if (tid == 0 && w.s0 == w.t0 && w.s1 < w.t1) g.heads[me] = run.head(w, first_item, me);
-    first_item = false;
-    __syncthreads();  // before the next item's queries
+        if (tid == 0 && w.s0 == w.t0 && w.s1 < w.t1) g.heads[me] = run.head(w, first_item, me);
+        first_item = false;
+        __syncthreads();  // before the next item's queries
     } while (w.next<kRows, kKeys>(a));
 }
 

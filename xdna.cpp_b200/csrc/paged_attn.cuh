@@ -69,7 +69,7 @@ __device__ __forceinline__ int my_rows(const AttnArgs& a, const Request& r) {
 // Keys a table row has room for; there are none behind it.
 __device__ __forceinline__ int table_keys(const AttnArgs& a) {
     const int64_t n = a.p.table_width << a.log_bs;
-    return n < 0x7fffffff ? static_cast<int>(n) : 0x7fffffff;
+    return n < 0x7fffff00 ? static_cast<int>(n) : 0x7fffff00;  // the caches hold fewer than 2^31
 }
 // Keys that some row of tokens [i0, i1] of the request sees: [lo, hi).
 __device__ __forceinline__ void key_range(const AttnArgs& a, const Request& r, int i0, int i1, int& lo, int& hi) {

@@ -256,111 +256,111 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
     if (run.units) {
         Walk w = run.first;
         if (warp >= kLoadWarp) {
-        if constexpr (L::kQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegs));
-        if (warp < kMmaWarp) {
-            // ---------------------------------------------------------------- loads
-            const bool values = uniform(warp) == kLoadWarp + 1;  // one warp for K, one for V
-            const CUtensorMap* map = values ? &c.v : &c.k;
-            uint64_t *full = values ? bars.vfull : bars.kfull, *empty = values ? bars.vempty : bars.kempty;
-            const uint32_t ring = values ? vs : ks;
-            const int boxes = kKeys / c.box_tokens;  // per half; lane i looks up the block of box i
-            uint32_t n = 0;                          // tiles so far
-            bool ok = true;
-            do {
-                const int s0 = uniform(w.s0), s1 = uniform(w.s1), kvh = uniform(w.kvh);
-                for (int t = s0; t < s1 && ok; ++t, ++n) {
-                    const int j = t * kKeys + lane * c.box_tokens;
-                    const bool on = lane < boxes && j < w.hi;
-                    const int id = on ? key_block(a, w.b, j >> a.log_bs) : 0;
-                    const int block = id < 0 ? static_cast<int>(a.kv.num_blocks) : id;  // behind the last: zeros
-                    const int count = __popc(__ballot_sync(0xffffffffu, on));
-                    const uint32_t stage = n % L::kStages;
-                    if (n >= L::kStages) ok = bar_wait(&empty[stage], ((n / L::kStages) & 1) ^ 1, dead);
-                    if (!ok) break;
-                    if (elect_one()) bar_expect(&full[stage], count * L::kHalves * c.box_tokens * 128);
-                    __syncwarp();
-                    for (int x = 0; x < count; ++x) {
-                        const int from = __shfl_sync(0xffffffffu, block, x), token = (t * kKeys + x * c.box_tokens) & (a.kv.block_size - 1);
-                        if (elect_one())
+            if constexpr (L::kQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegs));
+            if (warp < kMmaWarp) {
+                // ---------------------------------------------------------------- loads
+                const bool values = uniform(warp) == kLoadWarp + 1;  // one warp for K, one for V
+                const CUtensorMap* map = values ? &c.v : &c.k;
+                uint64_t *full = values ? bars.vfull : bars.kfull, *empty = values ? bars.vempty : bars.kempty;
+                const uint32_t ring = values ? vs : ks;
+                const int boxes = kKeys / c.box_tokens;  // per half; lane i looks up the block of box i
+                uint32_t n = 0;                          // tiles so far
+                bool ok = true;
+                do {
+                    const int s0 = uniform(w.s0), s1 = uniform(w.s1), kvh = uniform(w.kvh);
+                    for (int t = s0; t < s1 && ok; ++t, ++n) {
+                        const int j = t * kKeys + lane * c.box_tokens;
+                        const bool on = lane < boxes && j < w.hi;
+                        const int id = on ? key_block(a, w.b, j >> a.log_bs) : 0;
+                        const int block = id < 0 ? static_cast<int>(a.kv.num_blocks) : id;  // behind the last: zeros
+                        const int count = __popc(__ballot_sync(0xffffffffu, on));
+                        const uint32_t stage = n % L::kStages;
+                        if (n >= L::kStages) ok = bar_wait(&empty[stage], ((n / L::kStages) & 1) ^ 1, dead);
+                        if (!ok) break;
+                        if (elect_one()) bar_expect(&full[stage], count * L::kHalves * c.box_tokens * 128);
+                        __syncwarp();
+                        for (int x = 0; x < count; ++x) {
+                            const int from = __shfl_sync(0xffffffffu, block, x), token = (t * kKeys + x * c.box_tokens) & (a.kv.block_size - 1);
+                            if (elect_one())
 #pragma unroll
-                            for (int h = 0; h < L::kHalves; ++h)
-                                tma_box(ring + stage * L::kTile + h * 128 * 128 + x * c.box_tokens * 128, map, &full[stage], h * 64,
-                                        token, kvh, from);
+                                for (int h = 0; h < L::kHalves; ++h)
+                                    tma_box(ring + stage * L::kTile + h * 128 * 128 + x * c.box_tokens * 128, map, &full[stage], h * 64,
+                                            token, kvh, from);
+                            __syncwarp();
+                        }
+                    }
+                } while (ok && w.next<R, kKeys>(a));
+                if (!ok)  // copies in flight land before the CTA ends
+                    for (uint32_t i = n < L::kStages ? 0 : n - L::kStages; i < n; ++i)
+                        bar_wait(&full[i % L::kStages], (i / L::kStages) & 1, nullptr);
+            } else if (warp < kMmaWarp + L::kQ) {
+                // ----------------------------------------------------- matrix instructions
+                constexpr uint32_t kIdescS = instruction<T>(kKeys, false), kIdescO = instruction<T>(D, true);
+                const int q = uniform(warp) - kMmaWarp;
+                const uint32_t s_at = uniform(tmem) + L::kS + q * L::kPitch, o_at = uniform(tmem) + L::kO + q * L::kPitch;
+                const uint64_t q_op = operand(qs + q * L::kTile, 16), k_op = operand(ks, 16), v_op = operand(vs, 128 * 128);
+                uint32_t i = 0, nq = 0, np = 0;  // key tiles, phases of qfull and pfull
+                bool ok = true;
+                do {
+                    int lo, hi;
+                    query_tiles(a, w, w.tile * R + q * 128, lo, hi);
+                    lo = uniform(lo), hi = uniform(hi);
+                    const int s0 = uniform(w.s0), s1 = uniform(w.s1);
+                    // step t: O of tile t - 1, then S of tile t.  What S needs is waited for
+                    // before the weights, so that it follows at once.
+                    for (int t = s0; t <= s1 && ok; ++t, ++i) {
+                        const uint32_t k_stage = i % L::kStages, v_stage = (i + L::kStages - 1) % L::kStages;
+                        const bool value = t > lo && t <= hi && t > s0, score = t >= lo && t < hi && t < s1;
+                        if (t > s0) ok = bar_wait(&bars.vfull[v_stage], ((i - 1) / L::kStages) & 1, dead);
+                        if (ok && t < s1) ok = bar_wait(&bars.kfull[k_stage], (i / L::kStages) & 1, dead);
+                        if (ok && score && t == lo) ok = bar_wait(&bars.qfull[q], nq++ & 1, dead);
+                        const uint64_t v = v_op + (v_stage * L::kTile >> 4), k_at = k_op + (k_stage * L::kTile >> 4);
+                        // 16 keys k: their weights lie in half k / 4 of S's columns
+                        auto weighted = [&](int k, bool add) {
+                            mma_ts(o_at, s_at + (k >> 2) * 64 + (k & 3) * 8, v + (k * 2048 >> 4), kIdescO, add);
+                        };
+                        if (ok && value) ok = bar_wait(&bars.pfull[q][0], np & 1, dead);
+                        tc_after();
+                        if (ok && value && elect_one()) {
+                            weighted(0, t - 1 > lo);
+                            weighted(1, true);
+                            weighted(4, true);
+                            weighted(5, true);
+                        }
+                        __syncwarp();
+                        if (ok && value) ok = bar_wait(&bars.pfull[q][1], np++ & 1, dead);
+                        tc_after();
+                        if (ok && elect_one()) {
+                            if (value) {
+                                weighted(2, true);
+                                weighted(3, true);
+                                weighted(6, true);
+                                weighted(7, true);
+                                if (t == hi) tc_commit(&bars.ofull[q]);
+                            } else if (t > s0) {
+                                bar_arrive(&bars.vempty[v_stage]);
+                            }
+                            if (score) {
+#pragma unroll
+                                for (int k = 0; k < D / 16; ++k) {
+                                    const uint32_t off = ((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4;
+                                    mma_ss(s_at, q_op + off, k_at + off, kIdescS, k > 0);
+                                }
+                                tc_commit(&bars.sfull[q]);
+                            } else if (t < s1) {
+                                bar_arrive(&bars.kempty[k_stage]);
+                            }
+                        }
                         __syncwarp();
                     }
-                }
-            } while (ok && w.next<R, kKeys>(a));
-            if (!ok)  // copies in flight land before the CTA ends
-                for (uint32_t i = n < L::kStages ? 0 : n - L::kStages; i < n; ++i)
-                    bar_wait(&full[i % L::kStages], (i / L::kStages) & 1, nullptr);
-        } else if (warp < kMmaWarp + L::kQ) {
-            // ----------------------------------------------------- matrix instructions
-            constexpr uint32_t kIdescS = instruction<T>(kKeys, false), kIdescO = instruction<T>(D, true);
-            const int q = uniform(warp) - kMmaWarp;
-            const uint32_t s_at = uniform(tmem) + L::kS + q * L::kPitch, o_at = uniform(tmem) + L::kO + q * L::kPitch;
-            const uint64_t q_op = operand(qs + q * L::kTile, 16), k_op = operand(ks, 16), v_op = operand(vs, 128 * 128);
-            uint32_t i = 0, nq = 0, np = 0;  // key tiles, phases of qfull and pfull
-            bool ok = true;
-            do {
-                int lo, hi;
-                query_tiles(a, w, w.tile * R + q * 128, lo, hi);
-                lo = uniform(lo), hi = uniform(hi);
-                const int s0 = uniform(w.s0), s1 = uniform(w.s1);
-                // step t: O of tile t - 1, then S of tile t.  What S needs is waited for
-                // before the weights, so that it follows at once.
-                for (int t = s0; t <= s1 && ok; ++t, ++i) {
-                    const uint32_t k_stage = i % L::kStages, v_stage = (i + L::kStages - 1) % L::kStages;
-                    const bool value = t > lo && t <= hi && t > s0, score = t >= lo && t < hi && t < s1;
-                    if (t > s0) ok = bar_wait(&bars.vfull[v_stage], ((i - 1) / L::kStages) & 1, dead);
-                    if (ok && t < s1) ok = bar_wait(&bars.kfull[k_stage], (i / L::kStages) & 1, dead);
-                    if (ok && score && t == lo) ok = bar_wait(&bars.qfull[q], nq++ & 1, dead);
-                    const uint64_t v = v_op + (v_stage * L::kTile >> 4), k_at = k_op + (k_stage * L::kTile >> 4);
-                    // 16 keys k: their weights lie in half k / 4 of S's columns
-                    auto weighted = [&](int k, bool add) {
-                        mma_ts(o_at, s_at + (k >> 2) * 64 + (k & 3) * 8, v + (k * 2048 >> 4), kIdescO, add);
-                    };
-                    if (ok && value) ok = bar_wait(&bars.pfull[q][0], np & 1, dead);
-                    tc_after();
-                    if (ok && value && elect_one()) {
-                        weighted(0, t - 1 > lo);
-                        weighted(1, true);
-                        weighted(4, true);
-                        weighted(5, true);
-                    }
+                    --i;  // the last step has no tile of its own
+                } while (ok && w.next<R, kKeys>(a));
+                if (!ok) {  // matrix instructions in flight end before TMEM is freed
+                    if (elect_one()) tc_commit(&bars.drain[q]);
                     __syncwarp();
-                    if (ok && value) ok = bar_wait(&bars.pfull[q][1], np++ & 1, dead);
-                    tc_after();
-                    if (ok && elect_one()) {
-                        if (value) {
-                            weighted(2, true);
-                            weighted(3, true);
-                            weighted(6, true);
-                            weighted(7, true);
-                            if (t == hi) tc_commit(&bars.ofull[q]);
-                        } else if (t > s0) {
-                            bar_arrive(&bars.vempty[v_stage]);
-                        }
-                        if (score) {
-#pragma unroll
-                            for (int k = 0; k < D / 16; ++k) {
-                                const uint32_t off = ((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4;
-                                mma_ss(s_at, q_op + off, k_at + off, kIdescS, k > 0);
-                            }
-                            tc_commit(&bars.sfull[q]);
-                        } else if (t < s1) {
-                            bar_arrive(&bars.kempty[k_stage]);
-                        }
-                    }
-                    __syncwarp();
+                    bar_wait(&bars.drain[q], 0, nullptr);
                 }
-                --i;  // the last step has no tile of its own
-            } while (ok && w.next<R, kKeys>(a));
-            if (!ok) {  // matrix instructions in flight end before TMEM is freed
-                if (elect_one()) tc_commit(&bars.drain[q]);
-                __syncwarp();
-                bar_wait(&bars.drain[q], 0, nullptr);
             }
-        }
         } else {
             // ------------------------------------------------------------------ softmax
             if constexpr (L::kQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));

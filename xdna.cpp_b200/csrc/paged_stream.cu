@@ -205,393 +205,393 @@ __global__ void __launch_bounds__(Ring<D>::kThreads, 1) attn_stream_kernel(const
         at.b = item / a.kv.kv_heads / g.tiles;
         at.enter<R, kKeys>(a);
     } else {
-    // units of all requests, summed up over the threads
-    const int per = (B + kThreads - 1) / kThreads;
-    {
-        long long mine = 0;
-        for (int b = min(tid * per, B); b < min(tid * per + per, B); ++b) {
-            const Work w = request_work<kKeys>(a, read_request(a, b), R);
-            mine += static_cast<long long>(w.units) * w.tiles * a.kv.kv_heads;
-        }
-        long long inc = mine;
+        // units of all requests, summed up over the threads
+        const int per = (B + kThreads - 1) / kThreads;
+        {
+            long long mine = 0;
+            for (int b = min(tid * per, B); b < min(tid * per + per, B); ++b) {
+                const Work w = request_work<kKeys>(a, read_request(a, b), R);
+                mine += static_cast<long long>(w.units) * w.tiles * a.kv.kv_heads;
+            }
+            long long inc = mine;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const long long o = __shfl_up_sync(0xffffffffu, inc, d);
-            if (lane >= d) inc += o;
+            for (int d = 1; d < 32; d <<= 1) {
+                const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+                if (lane >= d) inc += o;
+            }
+            if (lane == 31) warp_units[warp] = inc;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) inc += warp_units[w];
+            before[tid + 1] = inc;
+            if (tid == 0) before[0] = 0;
+            __syncthreads();
         }
-        if (lane == 31) warp_units[warp] = inc;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) inc += warp_units[w];
-        before[tid + 1] = inc;
-        if (tid == 0) before[0] = 0;
-        __syncthreads();
-    }
-    all = before[kThreads];
-    streams = min(static_cast<long long>(g.streams), max(1LL, all / kMinUnits));
-    // neighbouring streams lie on different SMs: a short run of units uses all of them
-    me = static_cast<long long>(own) * gridDim.x + blockIdx.x;
-    if (lane == 0 && !loads && me < g.streams) g.heads[me].parts = 0;
-    if (me >= streams || all == 0) return;
-    const long long u0 = all * me / streams, u1 = all * (me + 1) / streams;
-    left = static_cast<int>(u1 - u0);
+        all = before[kThreads];
+        streams = min(static_cast<long long>(g.streams), max(1LL, all / kMinUnits));
+        // neighbouring streams lie on different SMs: a short run of units uses all of them
+        me = static_cast<long long>(own) * gridDim.x + blockIdx.x;
+        if (lane == 0 && !loads && me < g.streams) g.heads[me].parts = 0;
+        if (me >= streams || all == 0) return;
+        const long long u0 = all * me / streams, u1 = all * (me + 1) / streams;
+        left = static_cast<int>(u1 - u0);
 
-    // the first unit
-    {
-        int lo = 0, hi = kThreads;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (before[mid] <= u0) lo = mid; else hi = mid;
-        }
-        long long u = before[lo];
-        at.b = lo * per;
-        at.enter<R, kKeys>(a);
-        for (;;) {
-            const long long n = static_cast<long long>(at.w.units) * at.w.tiles * a.kv.kv_heads;
-            if (u0 < u + n) break;
-            u += n;
-            ++at.b;
+        // the first unit
+        {
+            int lo = 0, hi = kThreads;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (before[mid] <= u0) lo = mid; else hi = mid;
+            }
+            long long u = before[lo];
+            at.b = lo * per;
             at.enter<R, kKeys>(a);
+            for (;;) {
+                const long long n = static_cast<long long>(at.w.units) * at.w.tiles * a.kv.kv_heads;
+                if (u0 < u + n) break;
+                u += n;
+                ++at.b;
+                at.enter<R, kKeys>(a);
+            }
+            const long long item = (u0 - u) / at.w.units;
+            at.unit = static_cast<int>(u0 - u - item * at.w.units);
+            at.kvh = static_cast<int>(item / at.w.tiles);
+            at.tile = static_cast<int>(item - static_cast<long long>(at.kvh) * at.w.tiles);
+            item0 = u0 - at.unit;
         }
-        const long long item = (u0 - u) / at.w.units;
-        at.unit = static_cast<int>(u0 - u - item * at.w.units);
-        at.kvh = static_cast<int>(item / at.w.tiles);
-        at.tile = static_cast<int>(item - static_cast<long long>(at.kvh) * at.w.tiles);
-        item0 = u0 - at.unit;
-    }
     }
     const uint32_t ring = smem_addr(smem) + own * L::kWarpBytes;
     uint32_t done = 0;  // units loaded, or worked off, by this warp
     for (; !kJoin || at.tile < at.w.tiles; at.tile += g.tiles) {
-    if constexpr (kJoin) {
-        const int n = at.w.units, i = own * kCluster + static_cast<int>(blockIdx.x) % kCluster;
-        constexpr int kAll = kCluster * L::kWarps;
-        at.unit = static_cast<int>(static_cast<long long>(n) * i / kAll);
-        left = static_cast<int>(static_cast<long long>(n) * (i + 1) / kAll) - at.unit;
-    }
-    bool fresh = true;  // no unit of the item worked off yet
-
-    // ------------------------------------------------------------------- loads
-    if (loads) {
-        const int boxes = kKeys / c.box_tokens;  // lane i < boxes loads box i of a unit
-        // the table entry of a box's block, not looked at before the unit is loaded
-        auto block_of = [&](const Cursor& f) {
-            const int j = f.w.lo + f.unit * kKeys + lane * c.box_tokens, page = j >> a.log_bs;
-            return lane < boxes && j < f.w.hi ? __ldg(a.p.block_table + static_cast<int64_t>(f.b) * a.p.table_width + page)
-                                              : 0;
-        };
-        Cursor fetch = at;
-        int id = block_of(fetch);
-        bool ok = true;
-        for (int todo = left; todo > 0; ++done) {
-            const int j = fetch.w.lo + fetch.unit * kKeys + lane * c.box_tokens, kvh = fetch.kvh;
-            const bool on = lane < boxes && j < fetch.w.hi;
-            // a block outside the cache: behind the last one, zeros
-            const int block = id >= 0 && id < a.kv.num_blocks ? id : static_cast<int>(a.kv.num_blocks);
-            if (--todo > 0) {
-                fetch.next<R, kKeys>(a);
-                id = block_of(fetch);
-            }
-            const uint32_t stage = done % L::kStages;
-            if (done >= L::kStages) ok = bar_wait(&empty[own][stage], ((done / L::kStages) & 1) ^ 1, dead);
-            if (!ok) break;
-            uint64_t* bar = &full[own][stage];
-            const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, on)) * c.box_tokens * 128 * 2 * L::kHalves;
-            if (lane == 0) bar_expect(bar, bytes);
-            __syncwarp();
-            if (on) {
-                const uint32_t to = ring + stage * L::kStage + lane * c.box_tokens * 128;
-#pragma unroll
-                for (int h = 0; h < L::kHalves; ++h)
-                    tma_box(to + h * L::kBlock, &c.k, bar, h * 64, j & (a.kv.block_size - 1), kvh, block);
-#pragma unroll
-                for (int h = 0; h < L::kHalves; ++h)
-                    tma_box(to + (L::kHalves + h) * L::kBlock, &c.v, bar, h * 64, j & (a.kv.block_size - 1), kvh, block);
-            }
-            __syncwarp();
+        if constexpr (kJoin) {
+            const int n = at.w.units, i = own * kCluster + static_cast<int>(blockIdx.x) % kCluster;
+            constexpr int kAll = kCluster * L::kWarps;
+            at.unit = static_cast<int>(static_cast<long long>(n) * i / kAll);
+            left = static_cast<int>(static_cast<long long>(n) * (i + 1) / kAll) - at.unit;
         }
-        if (!ok)  // copies in flight land before the CTA ends
-            for (uint32_t i = done < L::kStages ? 0 : done - L::kStages; i < done; ++i)
-                bar_wait(&full[own][i % L::kStages], (i / L::kStages) & 1, nullptr);
-        if constexpr (!kJoin) return;
-    }
+        bool fresh = true;  // no unit of the item worked off yet
 
-    // Addresses of this lane's matrix rows: 16-byte column x of row r lies at
-    // column x ^ (r & 7) of it.
-    uint32_t k_at[4], v_at[4];
+        // ------------------------------------------------------------------- loads
+        if (loads) {
+            const int boxes = kKeys / c.box_tokens;  // lane i < boxes loads box i of a unit
+            // the table entry of a box's block, not looked at before the unit is loaded
+            auto block_of = [&](const Cursor& f) {
+                const int j = f.w.lo + f.unit * kKeys + lane * c.box_tokens, page = j >> a.log_bs;
+                return lane < boxes && j < f.w.hi ? __ldg(a.p.block_table + static_cast<int64_t>(f.b) * a.p.table_width + page)
+                                                  : 0;
+            };
+            Cursor fetch = at;
+            int id = block_of(fetch);
+            bool ok = true;
+            for (int todo = left; todo > 0; ++done) {
+                const int j = fetch.w.lo + fetch.unit * kKeys + lane * c.box_tokens, kvh = fetch.kvh;
+                const bool on = lane < boxes && j < fetch.w.hi;
+                // a block outside the cache: behind the last one, zeros
+                const int block = id >= 0 && id < a.kv.num_blocks ? id : static_cast<int>(a.kv.num_blocks);
+                if (--todo > 0) {
+                    fetch.next<R, kKeys>(a);
+                    id = block_of(fetch);
+                }
+                const uint32_t stage = done % L::kStages;
+                if (done >= L::kStages) ok = bar_wait(&empty[own][stage], ((done / L::kStages) & 1) ^ 1, dead);
+                if (!ok) break;
+                uint64_t* bar = &full[own][stage];
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, on)) * c.box_tokens * 128 * 2 * L::kHalves;
+                if (lane == 0) bar_expect(bar, bytes);
+                __syncwarp();
+                if (on) {
+                    const uint32_t to = ring + stage * L::kStage + lane * c.box_tokens * 128;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        k_at[i] = (lane & 15) * 128 + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4);
-        v_at[i] = ((lane & 7) + ((lane >> 4) & 1) * 8) * 128 + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
-    }
-    uint32_t qf[NP][NT][kSteps][2];
-    float o[NT][kSteps][4], m[NT][2], l[NT][2], mul[NT][2], slope[NT][2];
-    int pos[NT][2];
-    int rows = 0, all_lo = 0, all_hi = 0;  // keys [all_lo, all_hi) are seen by every row
+                    for (int h = 0; h < L::kHalves; ++h)
+                        tma_box(to + h * L::kBlock, &c.k, bar, h * 64, j & (a.kv.block_size - 1), kvh, block);
+#pragma unroll
+                    for (int h = 0; h < L::kHalves; ++h)
+                        tma_box(to + (L::kHalves + h) * L::kBlock, &c.v, bar, h * 64, j & (a.kv.block_size - 1), kvh, block);
+                }
+                __syncwarp();
+            }
+            if (!ok)  // copies in flight land before the CTA ends
+                for (uint32_t i = done < L::kStages ? 0 : done - L::kStages; i < done; ++i)
+                    bar_wait(&full[own][i % L::kStages], (i / L::kStages) & 1, nullptr);
+            if constexpr (!kJoin) return;
+        }
 
-    bool begun_here = at.unit == 0, ok = true;
-    int todo = loads ? 0 : left;  // units to work off
-    while (todo > 0) {
-        if (fresh) {  // a new item: its queries, and nothing seen yet
-            fresh = false;
-            const int G = a.group, r0 = at.tile * R;
-            rows = min(R, at.w.rows - r0);
+        // Addresses of this lane's matrix rows: 16-byte column x of row r lies at
+        // column x ^ (r & 7) of it.
+        uint32_t k_at[4], v_at[4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int r = nt * 8 + (lane >> 2);
-                const bool on = r < rows;
-                const int i = (r0 + r) / G, h = at.kvh * G + (r0 + r) - i * G;
-                const char* src = static_cast<const char*>(a.p.q) + (at.rq.first + (on ? i : 0)) * a.p.nb_q;
-                float up = 1.f;
-                if constexpr (NP == 1) {
-                    const uint32_t* s = reinterpret_cast<const uint32_t*>(src) + static_cast<int64_t>(h) * (D / 2) + (lane & 3);
+        for (int i = 0; i < 4; ++i) {
+            k_at[i] = (lane & 15) * 128 + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4);
+            v_at[i] = ((lane & 7) + ((lane >> 4) & 1) * 8) * 128 + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
+        }
+        uint32_t qf[NP][NT][kSteps][2];
+        float o[NT][kSteps][4], m[NT][2], l[NT][2], mul[NT][2], slope[NT][2];
+        int pos[NT][2];
+        int rows = 0, all_lo = 0, all_hi = 0;  // keys [all_lo, all_hi) are seen by every row
+
+        bool begun_here = at.unit == 0, ok = true;
+        int todo = loads ? 0 : left;  // units to work off
+        while (todo > 0) {
+            if (fresh) {  // a new item: its queries, and nothing seen yet
+                fresh = false;
+                const int G = a.group, r0 = at.tile * R;
+                rows = min(R, at.w.rows - r0);
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        qf[0][nt][k][0] = on ? __ldg(s + k * 8) : 0u;
-                        qf[0][nt][k][1] = on ? __ldg(s + k * 8 + 4) : 0u;
+                for (int nt = 0; nt < NT; ++nt) {
+                    const int r = nt * 8 + (lane >> 2);
+                    const bool on = r < rows;
+                    const int i = (r0 + r) / G, h = at.kvh * G + (r0 + r) - i * G;
+                    const char* src = static_cast<const char*>(a.p.q) + (at.rq.first + (on ? i : 0)) * a.p.nb_q;
+                    float up = 1.f;
+                    if constexpr (NP == 1) {
+                        const uint32_t* s = reinterpret_cast<const uint32_t*>(src) + static_cast<int64_t>(h) * (D / 2) + (lane & 3);
+#pragma unroll
+                        for (int k = 0; k < kSteps; ++k) {
+                            qf[0][nt][k][0] = on ? __ldg(s + k * 8) : 0u;
+                            qf[0][nt][k][1] = on ? __ldg(s + k * 8 + 4) : 0u;
+                        }
+                    } else {
+                        const float2* s = reinterpret_cast<const float2*>(src) + static_cast<int64_t>(h) * (D / 2) + (lane & 3);
+                        float2 x[kSteps][2];
+                        float big = 0.f;
+#pragma unroll
+                        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                x[k][e] = on ? __ldg(s + k * 8 + e * 4) : make_float2(0.f, 0.f);
+                                big = fmaxf(big, fmaxf(fabsf(x[k][e].x), fabsf(x[k][e].y)));
+                            }
+                        up = row_power<NP>(big);
+                        const float down = 1.f / up;
+#pragma unroll
+                        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                uint32_t piece[NP];
+                                split_pair<T, NP>(x[k][e].x * down, x[k][e].y * down, piece);
+#pragma unroll
+                                for (int c = 0; c < NP; ++c) qf[c][nt][k][e] = piece[c];
+                            }
                     }
-                } else {
-                    const float2* s = reinterpret_cast<const float2*>(src) + static_cast<int64_t>(h) * (D / 2) + (lane & 3);
-                    float2 x[kSteps][2];
-                    float big = 0.f;
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k)
+                    for (int e = 0; e < 2; ++e) {  // this lane's columns of S^T
+                        const int col = 2 * (lane & 3) + e, rr = r0 + nt * 8 + col, it = rr / G;
+                        mul[nt][e] = a.pre * __shfl_sync(0xffffffffu, up, col * 4);
+                        slope[nt][e] = head_slope(a, at.kvh * G + rr - it * G);
+                        pos[nt][e] = at.rq.pos0() + it;
+                        m[nt][e] = -INFINITY;
+                        l[nt][e] = 0.f;
+                    }
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            x[k][e] = on ? __ldg(s + k * 8 + e * 4) : make_float2(0.f, 0.f);
-                            big = fmaxf(big, fmaxf(fabsf(x[k][e].x), fabsf(x[k][e].y)));
-                        }
-                    up = row_power<NP>(big);
-                    const float down = 1.f / up;
+                    for (int n = 0; n < kSteps; ++n)
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            uint32_t piece[NP];
-                            split_pair<T, NP>(x[k][e].x * down, x[k][e].y * down, piece);
-#pragma unroll
-                            for (int c = 0; c < NP; ++c) qf[c][nt][k][e] = piece[c];
-                        }
+                        for (int e = 0; e < 4; ++e) o[nt][n][e] = 0.f;
                 }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {  // this lane's columns of S^T
-                    const int col = 2 * (lane & 3) + e, rr = r0 + nt * 8 + col, it = rr / G;
-                    mul[nt][e] = a.pre * __shfl_sync(0xffffffffu, up, col * 4);
-                    slope[nt][e] = head_slope(a, at.kvh * G + rr - it * G);
-                    pos[nt][e] = at.rq.pos0() + it;
-                    m[nt][e] = -INFINITY;
-                    l[nt][e] = 0.f;
+                const int p0 = at.rq.pos0() + r0 / G, p1 = at.rq.pos0() + (r0 + rows - 1) / G;
+                all_hi = min(p0 + 1, at.w.hi);
+                all_lo = a.p.window > 0 && p1 >= a.p.window ? p1 - a.p.window + 1 : 0;
+            }
+            const uint32_t stage = done % L::kStages, kt = ring + stage * L::kStage, vt = kt + L::kHalves * L::kBlock;
+            ok = bar_wait(&full[own][stage], (done / L::kStages) & 1, dead);
+            if (!ok) break;
+            ++done;
+            const int j0 = at.w.lo + at.unit * kKeys, exist = at.w.hi - j0;
+            if (exist < kKeys) {  // values of keys that do not exist: a weight of 0 would not hide a NaN
+                for (int x = lane; x < (kKeys - max(exist, 0)) * 8 * L::kHalves; x += 32) {
+                    const int r = max(exist, 0) + x / (8 * L::kHalves), col = x % (8 * L::kHalves);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (col >> 3) * L::kBlock + r * 128 +
+                                                                                 (col & 7) * 16),
+                                 "r"(0)
+                                 : "memory");
                 }
-#pragma unroll
-                for (int n = 0; n < kSteps; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[nt][n][e] = 0.f;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into the stage
+                __syncwarp();
             }
-            const int p0 = at.rq.pos0() + r0 / G, p1 = at.rq.pos0() + (r0 + rows - 1) / G;
-            all_hi = min(p0 + 1, at.w.hi);
-            all_lo = a.p.window > 0 && p1 >= a.p.window ? p1 - a.p.window + 1 : 0;
-        }
-        const uint32_t stage = done % L::kStages, kt = ring + stage * L::kStage, vt = kt + L::kHalves * L::kBlock;
-        ok = bar_wait(&full[own][stage], (done / L::kStages) & 1, dead);
-        if (!ok) break;
-        ++done;
-        const int j0 = at.w.lo + at.unit * kKeys, exist = at.w.hi - j0;
-        if (exist < kKeys) {  // values of keys that do not exist: a weight of 0 would not hide a NaN
-            for (int x = lane; x < (kKeys - max(exist, 0)) * 8 * L::kHalves; x += 32) {
-                const int r = max(exist, 0) + x / (8 * L::kHalves), col = x % (8 * L::kHalves);
-                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (col >> 3) * L::kBlock + r * 128 +
-                                                                             (col & 7) * 16),
-                             "r"(0)
-                             : "memory");
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into the stage
-            __syncwarp();
-        }
 
-        // scores: two chains of matrix instructions per 16 keys, joined by an addition
-        float s[kKeys / 16][NT][4];
+            // scores: two chains of matrix instructions per 16 keys, joined by an addition
+            float s[kKeys / 16][NT][4];
 #pragma unroll
-        for (int kb = 0; kb < kKeys / 16; ++kb) {
-            float t[NT][2][4] = {};
+            for (int kb = 0; kb < kKeys / 16; ++kb) {
+                float t[NT][2][4] = {};
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                uint32_t kf[4];
-                ldsm4(kf, kt + (k >> 2) * L::kBlock + kb * 2048 + k_at[k & 3]);
+                for (int k = 0; k < kSteps; ++k) {
+                    uint32_t kf[4];
+                    ldsm4(kf, kt + (k >> 2) * L::kBlock + kb * 2048 + k_at[k & 3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = NP - 1; i >= 0; --i) mma16816<T>(t[nt][k & 1], kf, qf[i][nt][k][0], qf[i][nt][k][1]);
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = NP - 1; i >= 0; --i) mma16816<T>(t[nt][k & 1], kf, qf[i][nt][k][0], qf[i][nt][k][1]);
+                    for (int e = 0; e < 4; ++e) s[kb][nt][e] = t[nt][0][e] + t[nt][1][e];
+            }
+            const bool whole = j0 >= all_lo && j0 + kKeys <= all_hi;
+            bool higher = false;
+#pragma unroll
+            for (int kb = 0; kb < kKeys / 16; ++kb)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int q = e & 1, j = j0 + kb * 16 + (lane >> 2) + 8 * (e >> 1);
+                        float x = s[kb][nt][e] * mul[nt][q];
+                        if (a.post != 0.f) x = a.post * tanhf(x);
+                        if (a.bias_near) x = fmaf(slope[nt][q], static_cast<float>(j - pos[nt][q]), x);
+                        if (!whole && (j > min(pos[nt][q], at.w.hi - 1) || (a.p.window > 0 && pos[nt][q] - j >= a.p.window)))
+                            x = -INFINITY;
+                        s[kb][nt][e] = x;
+                        higher |= x > m[nt][q] + kSlack;
+                    }
+            if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        float top = m[nt][q];
+#pragma unroll
+                        for (int kb = 0; kb < kKeys / 16; ++kb) top = fmaxf(top, fmaxf(s[kb][nt][q], s[kb][nt][2 + q]));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const float f = top == -INFINITY ? 1.f : exp2f(m[nt][q] - top);
+                        m[nt][q] = top;
+                        l[nt][q] *= f;
+#pragma unroll
+                        for (int n = 0; n < kSteps; ++n) o[nt][n][q] *= f, o[nt][n][2 + q] *= f;
+                    }
+            }
+            uint32_t pf[kKeys / 16][NP][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float base[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0], m[nt][1] == -INFINITY ? 0.f : m[nt][1]};
+#pragma unroll
+                for (int kb = 0; kb < kKeys / 16; ++kb) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[kb][nt][e] = exp2f(s[kb][nt][e] - base[e & 1]);
+                        l[nt][e & 1] += s[kb][nt][e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {  // keys 0-7, then 8-15
+                        uint32_t piece[NP];
+                        split_pair<T, NP>(s[kb][nt][2 * e], s[kb][nt][2 * e + 1], piece);
+#pragma unroll
+                        for (int i = 0; i < NP; ++i) pf[kb][i][nt][e] = transpose8x8(piece[i]);
+                    }
+                }
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int n = 0; n < kSteps; ++n) {
+                // the matrix unit cuts its sums off: with F32 queries every unit's sum starts
+                // at 0 and is added by a rounded addition, or a long axis would show it
+                float t[NT][4] = {};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[kb][nt][e] = t[nt][0][e] + t[nt][1][e];
-        }
-        const bool whole = j0 >= all_lo && j0 + kKeys <= all_hi;
-        bool higher = false;
+                for (int kb = 0; kb < kKeys / 16; ++kb) {
+                    uint32_t vf[4];
+                    ldsm4_t(vf, vt + (n >> 2) * L::kBlock + kb * 2048 + v_at[n & 3]);
 #pragma unroll
-        for (int kb = 0; kb < kKeys / 16; ++kb)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int q = e & 1, j = j0 + kb * 16 + (lane >> 2) + 8 * (e >> 1);
-                    float x = s[kb][nt][e] * mul[nt][q];
-                    if (a.post != 0.f) x = a.post * tanhf(x);
-                    if (a.bias_near) x = fmaf(slope[nt][q], static_cast<float>(j - pos[nt][q]), x);
-                    if (!whole && (j > min(pos[nt][q], at.w.hi - 1) || (a.p.window > 0 && pos[nt][q] - j >= a.p.window)))
-                        x = -INFINITY;
-                    s[kb][nt][e] = x;
-                    higher |= x > m[nt][q] + kSlack;
+                        for (int i = NP - 1; i >= 0; --i)
+                            mma16816<T>(NP > 1 ? t[nt] : o[nt][n], vf, pf[kb][i][nt][0], pf[kb][i][nt][1]);
                 }
-        if (__any_sync(0xffffffffu, higher)) {
+                if (NP > 1)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[nt][n][e] += t[nt][e];
+            }
+            __syncwarp();  // every lane has read the stage
+            if (lane == 0) bar_arrive(&empty[own][stage]);
+            --todo;
+            const bool ends = at.unit + 1 == at.w.units;
+            if constexpr (kJoin) {
+                if (todo > 0) ++at.unit;
+                continue;
+            }
+            if (!ends && todo > 0) {
+                ++at.unit;
+                continue;
+            }
+
+            // the item ends here, or goes on in the next stream
+            const bool whole_item = ends && begun_here;
+            const int part = begun_here ? 1 : 0;
+            float* to = g.parts + (static_cast<size_t>(me) * 2 + part) * part_floats(R, D);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    float top = m[nt][q];
+                    float sum = l[nt][q];
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                    const int r = nt * 8 + 2 * (lane & 3) + q;
+                    if (r >= rows) continue;
+                    if (whole_item) {
+                        const int rr = at.tile * R + r, i = rr / a.group, h = at.kvh * a.group + rr - i * a.group;
+                        const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-                    for (int kb = 0; kb < kKeys / 16; ++kb) top = fmaxf(top, fmaxf(s[kb][nt][q], s[kb][nt][2 + q]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float f = top == -INFINITY ? 1.f : exp2f(m[nt][q] - top);
-                    m[nt][q] = top;
-                    l[nt][q] *= f;
+                        for (int n = 0; n < kSteps; ++n) {
+                            store_one(a, at.rq.first + i, h, n * 16 + (lane >> 2), sum == 0.f ? 0.f : o[nt][n][q] * inv);
+                            store_one(a, at.rq.first + i, h, n * 16 + 8 + (lane >> 2),
+                                      sum == 0.f ? 0.f : o[nt][n][2 + q] * inv);
+                        }
+                    } else {
 #pragma unroll
-                    for (int n = 0; n < kSteps; ++n) o[nt][n][q] *= f, o[nt][n][2 + q] *= f;
+                        for (int n = 0; n < kSteps; ++n) {
+                            to[r * D + n * 16 + (lane >> 2)] = o[nt][n][q];
+                            to[r * D + n * 16 + 8 + (lane >> 2)] = o[nt][n][2 + q];
+                        }
+                        if ((lane >> 2) == 0) {
+                            to[R * D + r] = m[nt][q];
+                            to[R * D + R + r] = sum;
+                        }
+                    }
                 }
-        }
-        uint32_t pf[kKeys / 16][NP][NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const float base[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0], m[nt][1] == -INFINITY ? 0.f : m[nt][1]};
-#pragma unroll
-            for (int kb = 0; kb < kKeys / 16; ++kb) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[kb][nt][e] = exp2f(s[kb][nt][e] - base[e & 1]);
-                    l[nt][e & 1] += s[kb][nt][e];
-                }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {  // keys 0-7, then 8-15
-                    uint32_t piece[NP];
-                    split_pair<T, NP>(s[kb][nt][2 * e], s[kb][nt][2 * e + 1], piece);
-#pragma unroll
-                    for (int i = 0; i < NP; ++i) pf[kb][i][nt][e] = transpose8x8(piece[i]);
-                }
+            if (begun_here && !ends && lane == 0) {
+                const long long w1 = stream_of(item0 + at.w.units - 1, all, streams);
+                g.heads[me] = SplitHead{at.b, at.kvh, at.tile, static_cast<int>(w1 - me + 1)};
+            }
+            if (todo > 0) {
+                item0 += at.w.units;
+                at.next<R, kKeys>(a);
+                fresh = begun_here = true;
             }
         }
+        if constexpr (!kJoin) {
+            break;
+        } else {
+            // this warp's sums to the start of its ring (all of it has been read)
+            __syncwarp();
+            float* to = reinterpret_cast<float*>(smem + own * L::kWarpBytes);
+            const bool any = at.w.units > 0 && !fresh;
+            const int r0 = at.tile * R;
+            rows = min(R, at.w.rows - r0);
+            if (!loads)
 #pragma unroll
-        for (int n = 0; n < kSteps; ++n) {
-            // the matrix unit cuts its sums off: with F32 queries every unit's sum starts
-            // at 0 and is added by a rounded addition, or a long axis would show it
-            float t[NT][4] = {};
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int kb = 0; kb < kKeys / 16; ++kb) {
-                uint32_t vf[4];
-                ldsm4_t(vf, vt + (n >> 2) * L::kBlock + kb * 2048 + v_at[n & 3]);
+                for (int q = 0; q < 2; ++q) {
+                    const int r = nt * 8 + 2 * (lane & 3) + q;
+                    float sum = any ? l[nt][q] : 0.f;
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                    if (any)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int i = NP - 1; i >= 0; --i)
-                        mma16816<T>(NP > 1 ? t[nt] : o[nt][n], vf, pf[kb][i][nt][0], pf[kb][i][nt][1]);
-            }
-            if (NP > 1)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[nt][n][e] += t[nt][e];
-        }
-        __syncwarp();  // every lane has read the stage
-        if (lane == 0) bar_arrive(&empty[own][stage]);
-        --todo;
-        const bool ends = at.unit + 1 == at.w.units;
-        if constexpr (kJoin) {
-            if (todo > 0) ++at.unit;
-            continue;
-        }
-        if (!ends && todo > 0) {
-            ++at.unit;
-            continue;
-        }
-
-        // the item ends here, or goes on in the next stream
-        const bool whole_item = ends && begun_here;
-        const int part = begun_here ? 1 : 0;
-        float* to = g.parts + (static_cast<size_t>(me) * 2 + part) * part_floats(R, D);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                float sum = l[nt][q];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-                const int r = nt * 8 + 2 * (lane & 3) + q;
-                if (r >= rows) continue;
-                if (whole_item) {
-                    const int rr = at.tile * R + r, i = rr / a.group, h = at.kvh * a.group + rr - i * a.group;
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-                    for (int n = 0; n < kSteps; ++n) {
-                        store_one(a, at.rq.first + i, h, n * 16 + (lane >> 2), sum == 0.f ? 0.f : o[nt][n][q] * inv);
-                        store_one(a, at.rq.first + i, h, n * 16 + 8 + (lane >> 2),
-                                  sum == 0.f ? 0.f : o[nt][n][2 + q] * inv);
-                    }
-                } else {
-#pragma unroll
-                    for (int n = 0; n < kSteps; ++n) {
-                        to[r * D + n * 16 + (lane >> 2)] = o[nt][n][q];
-                        to[r * D + n * 16 + 8 + (lane >> 2)] = o[nt][n][2 + q];
-                    }
+                        for (int n = 0; n < kSteps; ++n) {
+                            to[r * D + n * 16 + (lane >> 2)] = o[nt][n][q];
+                            to[r * D + n * 16 + 8 + (lane >> 2)] = o[nt][n][2 + q];
+                        }
                     if ((lane >> 2) == 0) {
-                        to[R * D + r] = m[nt][q];
+                        to[R * D + r] = any ? m[nt][q] : -INFINITY;
                         to[R * D + R + r] = sum;
                     }
                 }
-            }
-        if (begun_here && !ends && lane == 0) {
-            const long long w1 = stream_of(item0 + at.w.units - 1, all, streams);
-            g.heads[me] = SplitHead{at.b, at.kvh, at.tile, static_cast<int>(w1 - me + 1)};
+            cluster_join<D, R, kThreads, L::kWarps, L::kWarpBytes>(a, at.rq, at.kvh, at.tile, rows, smem);
         }
-        if (todo > 0) {
-            item0 += at.w.units;
-            at.next<R, kKeys>(a);
-            fresh = begun_here = true;
-        }
-    }
-    if constexpr (!kJoin) {
-        break;
-    } else {
-        // this warp's sums to the start of its ring (all of it has been read)
-        __syncwarp();
-        float* to = reinterpret_cast<float*>(smem + own * L::kWarpBytes);
-        const bool any = at.w.units > 0 && !fresh;
-        const int r0 = at.tile * R;
-        rows = min(R, at.w.rows - r0);
-        if (!loads)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int r = nt * 8 + 2 * (lane & 3) + q;
-                float sum = any ? l[nt][q] : 0.f;
-                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-                if (any)
-#pragma unroll
-                    for (int n = 0; n < kSteps; ++n) {
-                        to[r * D + n * 16 + (lane >> 2)] = o[nt][n][q];
-                        to[r * D + n * 16 + 8 + (lane >> 2)] = o[nt][n][2 + q];
-                    }
-                if ((lane >> 2) == 0) {
-                    to[R * D + r] = any ? m[nt][q] : -INFINITY;
-                    to[R * D + R + r] = sum;
-                }
-            }
-        cluster_join<D, R, kThreads, L::kWarps, L::kWarpBytes>(a, at.rq, at.kvh, at.tile, rows, smem);
-    }
     }
 }
 
