@@ -13,8 +13,9 @@
 //                            than the matrix unit)
 //   one warp each            TMA loads of K and of V, page by page, into rings
 // While one query tile is in its softmax the matrix unit works on the other
-// one: their warps take turns in the exponentials.  O is rescaled only when a row's maximum grows by more than 8 (weights
-// stay below 2^8), which a vote of the warp finds out.  The weights are rounded
+// one: their warps take turns in the exponentials.  O is rescaled only when a row's
+// maximum grows by more than 8 (weights stay below 2^8), which a vote of the warp
+// finds out.  The weights are rounded
 // to 16 bits (the cache's type) because the matrix unit takes both factors in
 // one type; scores, sums and O are F32.
 //
@@ -36,9 +37,12 @@
 // exponential unit 54 %, issue 49 %.  A key tile of a query tile is one chain: S, the
 // maximum, its exchange between the halves of a row, the exponentials, O and the
 // next S (about 4000 clocks, of which the matrix unit has 1024 for each query tile),
-// and two query tiles fill TMEM.  Tried and slower: 64-key tiles with two buffers
-// of S (923 us in bursts), a whole row per thread (1044 against 1013 us), a share of
-// the exponentials by a polynomial (every share), turns by an mbarrier (1115 us).
+// and two query tiles fill TMEM.  Heads of 256 have one query tile; its S has two
+// buffers instead, so that S of the next tile is formed during the softmax (509 new
+// tokens of 16 heads beside 11 requests of one token, all launches: 143 -> 135 us).
+// Tried and slower: 64-key tiles with two buffers of S for heads of 128 (923 us in
+// bursts), a whole row per thread (1044 against 1013 us), a share of the exponentials
+// by a polynomial (every share), turns by an mbarrier (1115 us).
 #include <algorithm>
 
 #include "paged_split.cuh"
@@ -68,6 +72,10 @@ struct Shape {
     static_assert(kQ == 1 || 512 * kSoftmaxRegs + 128 * kOtherRegs <= 640 * kLaunchRegs, "registers of the launch");
     static constexpr int kSmem = (kQ + 2 * kStages) * kTile + 1024;  // 1024: alignment
     static constexpr int kS = 0, kO = 256, kPitch = 128;             // TMEM columns of q's S and O: + 128 q
+    // One query tile leaves room for two buffers of S (columns 0 and 128), used in turn.
+    static constexpr bool kTwo = kQ == 1;
+    static __device__ __forceinline__ uint32_t buffer(uint32_t n) { return kTwo ? n & 1 : 0; }
+    static __device__ __forceinline__ uint32_t phase(uint32_t n) { return kTwo ? n >> 1 & 1 : n & 1; }
 };
 
 struct ChunkArgs {
@@ -79,7 +87,8 @@ struct ChunkArgs {
 // ------------------------------------------------------------------- barriers
 struct Bars {
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-    uint64_t qfull[2], sfull[2], pfull[2][2], ofull[2], drain[2];  // pfull: keys 0-31 and 64-95, then the others
+    // of each query tile; of each buffer of S; pfull: keys 0-31 and 64-95, then the others
+    uint64_t qfull[2], sfull[2][2], pfull[2][2][2], ofull[2][2], drain[2];
 };
 
 // ------------------------------------------------------------ matrix unit, TMEM
@@ -227,10 +236,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
         }
         for (int i = 0; i < 2; ++i) {
             bar_init(&bars.qfull[i], 256);
-            bar_init(&bars.sfull[i], 1);
-            bar_init(&bars.pfull[i][0], 8);
-            bar_init(&bars.pfull[i][1], 8);
-            bar_init(&bars.ofull[i], 1);
+            for (int j = 0; j < 2; ++j) {
+                bar_init(&bars.sfull[i][j], 1);
+                bar_init(&bars.pfull[i][j][0], 8);
+                bar_init(&bars.pfull[i][j][1], 8);
+                bar_init(&bars.ofull[i][j], 1);
+            }
             bar_init(&bars.drain[i], 1);
         }
         dead_word = 0;
@@ -299,27 +310,48 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                 const int q = uniform(warp) - kMmaWarp;
                 const uint32_t s_at = uniform(tmem) + L::kS + q * L::kPitch, o_at = uniform(tmem) + L::kO + q * L::kPitch;
                 const uint64_t q_op = operand(qs + q * L::kTile, 16), k_op = operand(ks, 16), v_op = operand(vs, 128 * 128);
-                uint32_t i = 0, nq = 0, np = 0;  // key tiles, phases of qfull and pfull
+                uint32_t i = 0, nq = 0, ns = 0, np = 0;  // key tiles; phases of qfull; tiles of S, and of P, so far
                 bool ok = true;
                 do {
                     int lo, hi;
                     query_tiles(a, w, w.tile * R + q * 128, lo, hi);
                     lo = uniform(lo), hi = uniform(hi);
                     const int s0 = uniform(w.s0), s1 = uniform(w.s1);
-                    // step t: O of tile t - 1, then S of tile t.  What S needs is waited for
-                    // before the weights, so that it follows at once.
+                    // step t: with one buffer of S, O of tile t - 1, then S of tile t; what S
+                    // needs is waited for before the weights, so that it follows at once.
+                    // With two, S of tile t first (the weights in its buffer, of tile t - 2,
+                    // have been taken by the instructions before it).
                     for (int t = s0; t <= s1 && ok; ++t, ++i) {
                         const uint32_t k_stage = i % L::kStages, v_stage = (i + L::kStages - 1) % L::kStages;
                         const bool value = t > lo && t <= hi && t > s0, score = t >= lo && t < hi && t < s1;
-                        if (t > s0) ok = bar_wait(&bars.vfull[v_stage], ((i - 1) / L::kStages) & 1, dead);
-                        if (ok && t < s1) ok = bar_wait(&bars.kfull[k_stage], (i / L::kStages) & 1, dead);
-                        if (ok && score && t == lo) ok = bar_wait(&bars.qfull[q], nq++ & 1, dead);
                         const uint64_t v = v_op + (v_stage * L::kTile >> 4), k_at = k_op + (k_stage * L::kTile >> 4);
+                        auto scores = [&] {
+                            if (score) {
+#pragma unroll
+                                for (int k = 0; k < D / 16; ++k) {
+                                    const uint32_t off = ((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4;
+                                    mma_ss(s_at + L::buffer(ns) * 128, q_op + off, k_at + off, kIdescS, k > 0);
+                                }
+                                tc_commit(&bars.sfull[q][L::buffer(ns)]);
+                            } else if (t < s1) {
+                                bar_arrive(&bars.kempty[k_stage]);
+                            }
+                        };
                         // 16 keys k: their weights lie in half k / 4 of S's columns
                         auto weighted = [&](int k, bool add) {
-                            mma_ts(o_at, s_at + (k >> 2) * 64 + (k & 3) * 8, v + (k * 2048 >> 4), kIdescO, add);
+                            mma_ts(o_at, s_at + L::buffer(np) * 128 + (k >> 2) * 64 + (k & 3) * 8, v + (k * 2048 >> 4),
+                                   kIdescO, add);
                         };
-                        if (ok && value) ok = bar_wait(&bars.pfull[q][0], np & 1, dead);
+                        if (!L::kTwo && t > s0) ok = bar_wait(&bars.vfull[v_stage], ((i - 1) / L::kStages) & 1, dead);
+                        if (ok && t < s1) ok = bar_wait(&bars.kfull[k_stage], (i / L::kStages) & 1, dead);
+                        if (ok && score && t == lo) ok = bar_wait(&bars.qfull[q], nq++ & 1, dead);
+                        if (L::kTwo) {
+                            tc_after();
+                            if (ok && elect_one()) scores();
+                            __syncwarp();
+                            if (ok && t > s0) ok = bar_wait(&bars.vfull[v_stage], ((i - 1) / L::kStages) & 1, dead);
+                        }
+                        if (ok && value) ok = bar_wait(&bars.pfull[q][L::buffer(np)][0], L::phase(np), dead);
                         tc_after();
                         if (ok && value && elect_one()) {
                             weighted(0, t - 1 > lo);
@@ -328,7 +360,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             weighted(5, true);
                         }
                         __syncwarp();
-                        if (ok && value) ok = bar_wait(&bars.pfull[q][1], np++ & 1, dead);
+                        if (ok && value) ok = bar_wait(&bars.pfull[q][L::buffer(np)][1], L::phase(np), dead);
                         tc_after();
                         if (ok && elect_one()) {
                             if (value) {
@@ -336,22 +368,15 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                                 weighted(3, true);
                                 weighted(6, true);
                                 weighted(7, true);
-                                if (t == hi) tc_commit(&bars.ofull[q]);
+                                if (L::kTwo) tc_commit(&bars.vempty[v_stage]);
+                                if (L::kTwo || t == hi) tc_commit(&bars.ofull[q][L::buffer(np)]);
                             } else if (t > s0) {
                                 bar_arrive(&bars.vempty[v_stage]);
                             }
-                            if (score) {
-#pragma unroll
-                                for (int k = 0; k < D / 16; ++k) {
-                                    const uint32_t off = ((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4;
-                                    mma_ss(s_at, q_op + off, k_at + off, kIdescS, k > 0);
-                                }
-                                tc_commit(&bars.sfull[q]);
-                            } else if (t < s1) {
-                                bar_arrive(&bars.kempty[k_stage]);
-                            }
+                            if (!L::kTwo) scores();
                         }
                         __syncwarp();
+                        ns += score, np += value;
                     }
                     --i;  // the last step has no tile of its own
                 } while (ok && w.next<R, kKeys>(a));
@@ -367,10 +392,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
             // Warps 8 q + 4 h + i: rows 32 i .. of query tile q, half h of the columns
             const int q = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
             const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-            const uint32_t s_at = tmem + lanes + L::kS + q * L::kPitch + half * 64;
+            const uint32_t s_base = tmem + lanes + L::kS + q * L::kPitch + half * 64;
             const uint32_t o_at = tmem + lanes + L::kO + q * L::kPitch + half * (D / 2);
             const uint32_t q_at = qs + q * L::kTile + row * 128;
-            uint32_t ns = 0, no = 0, nx = 0;  // phases of sfull and ofull, exchanges
+            uint32_t ns = 0, no = 0, nx = 0;  // key tiles of this query tile, items, exchanges so far
             uint32_t n = 0;                   // key tiles before the item's
             int mine = 0, theirs = 0;         // key tiles of this and of the other query tile before the item's
             bool first_item = true;
@@ -417,14 +442,19 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                         const int p1 = w.rq.pos0() + (min(r0 + 128, w.rows) - 1) / a.group;
                         const int all_hi = min(p0 + 1, w.hi);
                         const int all_lo = a.p.window > 0 && p1 >= a.p.window ? p1 - a.p.window + 1 : 0;
-                        for (int t = lo; t < hi; ++t) {
-                            bar_wait(&bars.sfull[q], ns++ & 1, dead);
+                        for (int t = lo; t < hi; ++t, ++ns) {
+                            bar_wait(&bars.sfull[q][L::buffer(ns)], L::phase(ns), dead);
+                            // O of the tile two before was ordered ahead of S; its phase is passed on every
+                            // tile, so that the one waited for below is never mistaken for it
+                            if (L::kTwo && ns >= 2) bar_wait(&bars.ofull[q][L::buffer(ns)], L::phase(ns - 2), dead);
                             tc_after();
-                            // S is there, and so is O of the tile before: K and that tile's V are free
+                            const uint32_t s_at = s_base + L::buffer(ns) * 128;
+                            // S is there: K is free.  With one buffer of S, so are O of the tile
+                            // before and that tile's V.
                             if (row == 0 && half == 0) {
                                 const uint32_t x = n + t - w.s0;
                                 bar_arrive(&bars.kempty[x % L::kStages]);
-                                if (t > lo) bar_arrive(&bars.vempty[(x - 1) % L::kStages]);
+                                if (!L::kTwo && t > lo) bar_arrive(&bars.vempty[(x - 1) % L::kStages]);
                             }
                             const int j0 = t * kKeys + half * 64;
                             const bool cut = t * kKeys < all_lo || (t + 1) * kKeys > all_hi;
@@ -482,6 +512,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                                 const float f = m == -INFINITY ? 1.f : exp2_fast(was - m);
                                 l *= f;
                                 if (t > lo) {
+                                    if (L::kTwo) {  // once O has the tile before
+                                        bar_wait(&bars.ofull[q][L::buffer(ns - 1)], L::phase(ns - 1), dead);
+                                        tc_after();
+                                    }
 #pragma unroll 1
                                     for (int i = 0; i < D / 32; ++i) {
                                         float o[16];
@@ -539,7 +573,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                                 tm_wait_st();
                                 tc_before();
                                 __syncwarp();
-                                if (lane == 0) bar_arrive(&bars.pfull[q][part]);
+                                if (lane == 0) bar_arrive(&bars.pfull[q][L::buffer(ns)][part]);
                             };
                             hand_over(0);
                             tm_wait16(s0);
@@ -553,9 +587,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             l += both.x + both.y;
                         }
                         l += other_half(l);
-                        bar_wait(&bars.ofull[q], no++ & 1, dead);
+                        if (L::kTwo)
+                            bar_wait(&bars.ofull[q][L::buffer(ns - 1)], L::phase(ns - 1), dead);
+                        else
+                            bar_wait(&bars.ofull[q][0], no++ & 1, dead);
                         tc_after();
-                        if (row == 0 && half == 0) bar_arrive(&bars.vempty[(n + hi - 1 - w.s0) % L::kStages]);
+                        if (!L::kTwo && row == 0 && half == 0)
+                            bar_arrive(&bars.vempty[(n + hi - 1 - w.s0) % L::kStages]);
                     }
                     // half of O to the output, or to the item's partial
                     const bool whole = w.s0 == w.t0 && w.s1 == w.t1;
