@@ -340,6 +340,14 @@ def test_paged_attention_long(cuda, G, lens, bs, q_type, cache_type):
     check_attention(G, lens, 16, 2, 128, q_type, cache_type, bs, seed=bs, max_kv=100000)  # another work split
 
 
+# few tall items with many parts: one item, two, and more than their bound from the token count
+@pytest.mark.parametrize("lens", [[(5000, 20)], [(6000, 40)], [(2100, 40), (1900, 35), (2500, 45)]], ids=str)
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("q_type,cache_type", TYPES)
+def test_paged_attention_few_long_items(cuda, G, lens, D, q_type, cache_type):
+    check_attention(G, lens, 8, 1, D, q_type, cache_type, 32)
+
+
 @pytest.mark.parametrize("lens", [[(200, 1), (90, 1)], [(200, 100), (90, 1)]], ids=str)
 @pytest.mark.parametrize("kw", [dict(layout="token"), dict(layout="both"), dict(fused=True), dict(out_type="other"),
                                 dict(max_new=0, max_kv=0), dict(max_new=100000, max_kv=1000000)], ids=str)

@@ -39,7 +39,7 @@
 // next S (about 4000 clocks, of which the matrix unit has 1024 for each query tile),
 // and two query tiles fill TMEM.  Heads of 256 have one query tile; its S has two
 // buffers instead, so that S of the next tile is formed during the softmax (509 new
-// tokens of 16 heads beside 11 requests of one token, all launches: 143 -> 135 us).
+// tokens of 16 heads beside 11 requests of one token, all launches: 143 -> 135 us; 131 us now).
 // Tried and slower: 64-key tiles with two buffers of S for heads of 128 (923 us in
 // bursts), a whole row per thread (1044 against 1013 us), a share of the exponentials
 // by a polynomial (every share), turns by an mbarrier (1115 us).

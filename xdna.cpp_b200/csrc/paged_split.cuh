@@ -47,21 +47,18 @@ __device__ __forceinline__ long long stream_of(long long u, long long all, long 
 
 constexpr int kCombineWarps = 8;
 
-// Joins the item that stream blockIdx.x began.  Block y takes the rows y, y +
+// Joins the item that stream `me` began.  Block y takes the rows y, y +
 // gridDim.y, ...; kSpread: all warps share the parts of one row at a time (few
 // items, many parts), else every warp takes rows of its own.
 template <int D, int R, bool kSpread>
-__global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const __grid_constant__ SplitArgs g) {
-    __shared__ float shared_o[kSpread ? kCombineWarps : 1][D];
-    __shared__ float shared_l[kCombineWarps];
-    grid_wait();
+__device__ __forceinline__ void combine_item(const SplitArgs& g, int me, const SplitHead& head,
+                                             float (&shared_o)[kSpread ? kCombineWarps : 1][D],
+                                             float (&shared_l)[kCombineWarps]) {
     const AttnArgs& a = g.a;
-    const SplitHead head = g.heads[blockIdx.x];
-    if (!head.parts) return;
     const Request rq = read_request(a, head.b);
     const int rows = min(R, rq.count * a.group - head.tile * R), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t slot = part_floats(R, D);
-    const float* mine = g.parts + 2 * static_cast<size_t>(blockIdx.x) * slot;
+    const float* mine = g.parts + 2 * static_cast<size_t>(me) * slot;
     auto part = [&](int p) { return mine + (2 * static_cast<size_t>(p) + (p == 0)) * slot; };
     const int step = kSpread ? gridDim.y : gridDim.y * kCombineWarps;
     for (int r = kSpread ? blockIdx.y : blockIdx.y + gridDim.y * warp; r < rows; r += step) {
@@ -127,17 +124,49 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const __gri
     }
 }
 
+// Joins the items of stream blockIdx.x; kScan: of the blockIdx.x-th stream that has
+// one to join, and of every gridDim.x-th after it.
+template <int D, int R, bool kSpread, bool kScan>
+__global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const __grid_constant__ SplitArgs g) {
+    __shared__ float shared_o[kSpread ? kCombineWarps : 1][D];
+    __shared__ float shared_l[kCombineWarps];
+    grid_wait();
+    if (!kScan) {
+        const SplitHead head = g.heads[blockIdx.x];
+        if (head.parts) combine_item<D, R, kSpread>(g, blockIdx.x, head, shared_o, shared_l);
+        return;
+    }
+    const int lane = threadIdx.x & 31;
+    unsigned seen = 0;
+    for (int from = 0; from < g.streams; from += 32) {  // alike in all warps
+        const bool any = from + lane < g.streams && g.heads[from + lane].parts;
+        for (unsigned left = __ballot_sync(0xffffffffu, any); left; left &= left - 1)
+            if (seen++ % gridDim.x == blockIdx.x) {
+                const int me = from + __ffs(left) - 1;
+                combine_item<D, R, kSpread>(g, me, g.heads[me], shared_o, shared_l);
+            }
+    }
+}
+
 // Launches combine_kernel after a kernel whose items are about `items` (as the
-// hints have it).  Few items have many parts each and leave most blocks nothing to
+// hints have it).  Few items have many parts each and leave most streams nothing to
 // do: then a row is a CTA's (up to 32 rows an item) or a warp's, else a warp takes 4.
+// Very few tall items: a row is a CTA's, and the CTAs look for the items, since a
+// grid over all streams would be empty blocks for the most part (33 tokens of 8 heads
+// over 19.9 K keys, 2 items: 40.8 -> 27.2 us with the attention kernel; 8 items, of
+// 19 parts: 40.0 with a row a warp against 43.1).
 template <int D, int R>
 cudaError_t combine_launch(const SplitArgs& g, int64_t items, cudaStream_t stream) {
+    const dim3 threads(32 * kCombineWarps);
     const bool few = g.streams >= 4 * items;
     if (few && R <= 32)
-        return launch_pdl(combine_kernel<D, R, true>, dim3(g.streams, R), dim3(32 * kCombineWarps), 0, stream, 1, g);
+        return launch_pdl(combine_kernel<D, R, true, false>, dim3(g.streams, R), threads, 0, stream, 1, g);
+    if (R > 32 && g.streams >= 32 * items)
+        return launch_pdl(combine_kernel<D, R, true, true>, dim3(static_cast<unsigned>(std::max<int64_t>(items, 1)), R),
+                          threads, 0, stream, 1, g);
     const int rows = few ? kCombineWarps : 4 * kCombineWarps;  // of a block
-    return launch_pdl(combine_kernel<D, R, false>, dim3(g.streams, (R + rows - 1) / rows), dim3(32 * kCombineWarps), 0,
-                      stream, 1, g);
+    return launch_pdl(combine_kernel<D, R, false, false>, dim3(g.streams, (R + rows - 1) / rows), threads, 0, stream, 1,
+                      g);
 }
 #endif
 
