@@ -345,8 +345,9 @@ int b200_qk_norm_rope(const struct b200_qk_norm_rope_args *p, const struct b200_
  * Query head h reads KV head h / (heads / kv_heads).  Rows of q that belong to
  * no request leave their row of out as it is.  q and out are F32 or of the
  * cache's type.  Scores, softmax and sums are held in F32; with 16-bit q the
- * softmax weights are rounded to the cache's type for the product with V, with
- * F32 q both products carry F32's precision.
+ * softmax weights are rounded to the cache's type for the product with V (F16:
+ * in steps of 2^-31 of the row's largest at the finest), with F32 q both
+ * products carry F32's precision (F16: weights in steps of 2^-42 at the finest).
  * Keys behind kv_lens[b] may hold anything, NaN included; the values of keys
  * in front of it are finite (a request's own non-finite values may reach rows
  * of that request that do not see them). */

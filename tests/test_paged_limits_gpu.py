@@ -1,0 +1,68 @@
+"""The paged KV cache operators at the ends of their ranges: softmax weights and queries far below a row's largest, the
+largest caps, request counts next to a shared-memory limit, calls on several streams.  Bounds as in paged_helpers."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from paged_helpers import HALF, U, Cache, attention_ref, ints, run_attention
+from test_paged_gpu import BF16, F16, F32, TYPES, gen, near, no_wait_ran_out, normal  # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def one_request(G, g, n, KH, D, bs, cache_type, keys=None, values=None):
+    """A cache with one request of n keys: (cache, block table, keys, values)."""
+    ids = torch.randperm(-(-n // bs), generator=torch.Generator().manual_seed(n)).tolist()
+    c = Cache(G, len(ids), KH, bs, D, cache_type)
+    c.put(ids, normal(g, n, KH, D) if keys is None else keys, normal(g, n, KH, D) if values is None else values)
+    return c, ints([ids]), *c.get(ids, n)
+
+
+def attend(G, q, c, table, n, scale, **opts):
+    out = torch.full_like(q, 7.0)
+    run_attention(G, q, out, c, ints([0, q.shape[0]]), ints([n]), table, scale, **opts)
+    torch.cuda.synchronize()
+    return out
+
+
+# new tokens of one request, and the hint that chooses between its forms: joined in a cluster, joined from partials
+# (of the stream kernel), and the kernels of many rows
+FORMS = [(1, None), (1, 100000), (3, 100000), (90, None)]
+
+
+@pytest.mark.parametrize("new,max_kv", FORMS)
+@pytest.mark.parametrize("q_type,cache_type,nats", [(F32, F16, 17), (F32, F16, 22), (F32, BF16, 22), (F16, F16, 17),
+                                                    (BF16, BF16, 22)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_paged_attention_tail_far_below_the_largest_key(cuda, G, D, q_type, cache_type, nats, new, max_kv):
+    """One key in 32 (its value is 0) lies `nats` above all others, so that the output is made of weights of e^-nats.
+
+    A weight is rounded relative to itself down to the smallest normal number of its pieces, and by an absolute amount
+    below it, in units of the weight of the running maximum: F16 weights are held times 2^7 and end at 2^-24 (off by
+    2^-25 / 2^7); of F32 queries the second piece is held times 2^11 more (off by 2^-25 / 2^18); BF16 pieces end where
+    F32 does.  The row's sum is at least that of the weights relative to its largest."""
+    g = gen(nats + D)
+    n, scale = 2100, 0.125
+    keys = normal(g, n, 2, D)
+    keys[..., 0] = -8.0 * nats / 4.0
+    keys[::32] = 0.0
+    values = 1000.0 * (1.0 + 0.3 * normal(g, n, 2, D))
+    values[::32] = 0.0
+    c, table, k, v = one_request(G, g, n, 2, D, 16, cache_type, keys, values)
+    q = 0.25 * math.sqrt(64 / D) * normal(g, new, 6, D)
+    q[..., 0] = 4.0
+    q = q.to(q_type)
+    out = attend(G, q, c, table, n, scale, max_kv=max_kv)
+    ref, bound = attention_ref(q, k, v, n - new, scale, weight_half=0.0 if q_type == F32 else HALF[cache_type])
+    floor = {(F32, F16): 2.0 ** -43, (F16, F16): 2.0 ** -32}.get((q_type, cache_type), 0.0)
+    top = n // 32 - new // 32  # keys whose weight is 1 that every row sees: a lower bound of its sum
+    bound = bound + floor * v.double().abs().sum(0).repeat_interleave(3, 0)[None] / top
+    assert (bound < 0.02 * ref.abs()).all()  # what is asked for can fail
+    near(out, ref, bound, f"{nats} nats below")

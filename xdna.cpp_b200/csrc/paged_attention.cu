@@ -29,7 +29,7 @@ namespace xb {
 namespace {
 
 constexpr int kMinTiles = 2;   // key tiles per CTA below which fewer CTAs run
-constexpr float kSlack = 8.f;  // log2 of the largest weight
+constexpr float kSlack = 8.f;  // log2 of the largest weight (before kWeightLog2)
 
 template <int D, int NP>
 struct Tile {
@@ -54,6 +54,8 @@ __global__ void __launch_bounds__(Tile<D, NP>::kThreads, Tile<D, NP>::kCtas)
     attn_tile_kernel(const __grid_constant__ SplitArgs g) {
     using L = Tile<D, NP>;
     constexpr int kKeys = L::kKeys, kS = L::kStride, kThreads = L::kThreads, kRows = L::kRows;
+    constexpr int kSums = weight_sums(NP);
+    constexpr float kUp = 1 << Half16<T>::kWeightLog2;
     extern __shared__ __align__(16) uint16_t smem[];
     __shared__ RunUnits<kThreads> units;
     const AttnArgs& a = g.a;
@@ -231,11 +233,11 @@ __global__ void __launch_bounds__(Tile<D, NP>::kThreads, Tile<D, NP>::kCtas)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float* x = &s[2 * k + (e >> 1)][2 * (e & 1)];
-                    x[0] = exp2_fast(x[0] - base[e & 1]);
-                    x[1] = exp2_fast(x[1] - base[e & 1]);
+                    x[0] = exp2_fast(x[0] - base[e & 1]) * kUp;
+                    x[1] = exp2_fast(x[1] - base[e & 1]) * kUp;
                     l[e & 1] += x[0] + x[1];
                     uint32_t piece[NP];
-                    split_pair<T, NP>(x[0], x[1], piece);
+                    split_pair<T, NP>(x[0], x[1], piece, Half16<T>::kLow);
 #pragma unroll
                     for (int i = 0; i < NP; ++i) pf[k][i][e] = piece[i];
                 }
@@ -244,19 +246,23 @@ __global__ void __launch_bounds__(Tile<D, NP>::kThreads, Tile<D, NP>::kCtas)
             // addition.
 #pragma unroll
             for (int n = 0; n < D / 16; ++n) {
-                float t[2][4] = {};
+                float t[kSums][2][4] = {};
 #pragma unroll
                 for (int k = 0; k < kKeys / 16; ++k) {
                     uint32_t vf[4];
                     ldsm4_t(vf, smem_addr(vt + (k * 16 + (lane & 15)) * kS + n * 16 + (lane >> 4) * 8));
 #pragma unroll
                     for (int i = NP - 1; i >= 0; --i) {
-                        mma16816<T>(t[0], pf[k][i], vf[0], vf[1]);
-                        mma16816<T>(t[1], pf[k][i], vf[2], vf[3]);
+                        mma16816<T>(t[i % kSums][0], pf[k][i], vf[0], vf[1]);
+                        mma16816<T>(t[i % kSums][1], pf[k][i], vf[2], vf[3]);
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[2 * n][e] += t[0][e], o[2 * n + 1][e] += t[1][e];
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[2 * n + h][e] +=
+                            kSums == 2 ? fmaf(t[kSums - 1][h][e], 1.f / Half16<T>::kLow, t[0][h][e]) : t[0][h][e];
             }
             __syncthreads();
         }

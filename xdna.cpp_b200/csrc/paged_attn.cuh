@@ -124,11 +124,20 @@ __device__ __forceinline__ void store_one(const AttnArgs& a, int64_t row, int he
 }
 
 // 16-bit types: packing, and the pieces whose sum is an F32 value.
+//
+// A softmax weight is 2^8 at most (the running maximum moves when a score passes
+// it by 8), and most of a long row's are small.  F16 ends at 2^-24, below which a
+// weight would be lost for V while the sum of weights still counts it (32 keys in
+// 33 at 17 nats below the 33rd: all of their share of the output); so weights are
+// formed times 2^kWeightLog2, up to 2^15, and o and l carry the same factor until
+// they are divided.
 template <typename T>
 struct Half16;
 template <>
 struct Half16<__half> {
-    static constexpr int kPieces = 2;  // of an F32 value below 2: 11 + 11 bits
+    static constexpr int kPieces = 2;  // of an F32 value: 11 + 11 bits
+    static constexpr int kWeightLog2 = 7;
+    static constexpr float kLow = 2048.f;  // what the second piece of a weight is held times
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         const __half2 h = __floats2half2_rn(x, y);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -140,6 +149,8 @@ struct Half16<__half> {
 template <>
 struct Half16<__nv_bfloat16> {
     static constexpr int kPieces = 3;  // 8 + 8 + 8 bits
+    static constexpr int kWeightLog2 = 0;  // F32's range
+    static constexpr float kLow = 1.f;
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -148,20 +159,24 @@ struct Half16<__nv_bfloat16> {
         return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
     }
 };
-// Splits the pair (x, y) into NP 16-bit pairs, highest first; the sum of the
-// pieces is off by at most 2^-22 (F16, |x| < 2) or 2^-24 (BF16) of x.
+// Splits the pair (x, y) into NP 16-bit pairs, highest first, those behind the
+// first held times `low` each.  The sum of the pieces is off by at most 2^-24
+// (BF16), or 2^-22 of x or 2^-25 / low (F16; the smallest step is 2^-24).
 template <typename T, int NP>
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[NP]) {
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[NP], float low = 1.f) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         out[i] = Half16<T>::pack(x, y);
         if (i + 1 < NP) {
             const float2 h = Half16<T>::unpack(out[i]);
-            x -= h.x;
-            y -= h.y;
+            x = (x - h.x) * low;
+            y = (y - h.y) * low;
         }
     }
 }
+// Two pieces of a weight have a sum of products each: second[...] / kLow joins the
+// first's (with one or three pieces there is one sum).
+constexpr int weight_sums(int pieces) { return pieces == 2 ? 2 : 1; }
 // F16 pieces reach down to 2^-24 only, so a row of F32 queries is divided by a
 // power of two that leaves its largest value in [1, 2) (BF16 pieces have F32's
 // range).  `big` is a lane's largest value of the row; 4 lanes hold a row.

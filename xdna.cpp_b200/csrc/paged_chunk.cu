@@ -16,8 +16,8 @@
 // one: their warps take turns in the exponentials.  O is rescaled only when a row's
 // maximum grows by more than 8 (weights stay below 2^8), which a vote of the warp
 // finds out.  The weights are rounded
-// to 16 bits (the cache's type) because the matrix unit takes both factors in
-// one type; scores, sums and O are F32.
+// to 16 bits (the cache's type; F16 times 2^7, see Half16) because the matrix unit
+// takes both factors in one type; scores, sums and O are F32.
 //
 // The work of all items, counted in key tiles, is dealt out in equal contiguous
 // runs to one CTA per SM; items that end up cut are joined by combine_kernel.
@@ -54,7 +54,7 @@ namespace {
 
 constexpr int kKeys = 128;
 constexpr int kMinTiles = 2;   // key tiles per CTA below which fewer CTAs run
-constexpr float kSlack = 8.f;  // log2 of the largest weight
+constexpr float kSlack = 8.f;  // log2 of the largest weight (before kWeightLog2)
 constexpr int kTurnClocks = 4000;  // longest wait for a turn (a courtesy: nothing depends on it)
 
 template <int D>
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                                                  : "memory");
                                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                             }
-                            const float off = m == -INFINITY ? 0.f : -m;
+                            const float off = m == -INFINITY ? 0.f : Half16<T>::kWeightLog2 - m;
                             // The two query tiles' warps on a scheduler take turns in the exponentials,
                             // so that the matrix unit has the other one's work meanwhile (left alone
                             // they run in step, and the matrix unit waits for both).

@@ -35,7 +35,7 @@ namespace xb {
 namespace {
 
 constexpr int kMinUnits = 1;     // units per stream below which fewer streams run
-constexpr float kSlack = 8.f;    // log2 of the largest weight
+constexpr float kSlack = 8.f;    // log2 of the largest weight (before kWeightLog2)
 constexpr int kCluster = 8;      // CTAs that share an item of the joining form
 // Keys up to which the joining form is taken: it uses 8 SMs an item.  2, 8 KV
 // heads: 6.9, 6.9 us at 1024 keys, 12.5, 12.8 us at 8192, against 10.7, 11.9 us and
@@ -464,18 +464,22 @@ __global__ void __launch_bounds__(Ring<D>::kThreads, 1) attn_stream_kernel(const
             uint32_t pf[kKeys / 16][NP][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float base[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0], m[nt][1] == -INFINITY ? 0.f : m[nt][1]};
+                // 16-bit queries: the weights' factor goes into the exponent, whose rounding
+                // is far below that of the weights; F32 queries: an exact product
+                constexpr float kUp = NP > 1 ? 1 << Half16<T>::kWeightLog2 : 1, kOff = NP > 1 ? 0 : Half16<T>::kWeightLog2;
+                const float base[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0] - kOff,
+                                       m[nt][1] == -INFINITY ? 0.f : m[nt][1] - kOff};
 #pragma unroll
                 for (int kb = 0; kb < kKeys / 16; ++kb) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        s[kb][nt][e] = exp2f(s[kb][nt][e] - base[e & 1]);
+                        s[kb][nt][e] = exp2f(s[kb][nt][e] - base[e & 1]) * kUp;
                         l[nt][e & 1] += s[kb][nt][e];
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {  // keys 0-7, then 8-15
                         uint32_t piece[NP];
-                        split_pair<T, NP>(s[kb][nt][2 * e], s[kb][nt][2 * e + 1], piece);
+                        split_pair<T, NP>(s[kb][nt][2 * e], s[kb][nt][2 * e + 1], piece, Half16<T>::kLow);
 #pragma unroll
                         for (int i = 0; i < NP; ++i) pf[kb][i][nt][e] = transpose8x8(piece[i]);
                     }
@@ -485,7 +489,8 @@ __global__ void __launch_bounds__(Ring<D>::kThreads, 1) attn_stream_kernel(const
             for (int n = 0; n < kSteps; ++n) {
                 // the matrix unit cuts its sums off: with F32 queries every unit's sum starts
                 // at 0 and is added by a rounded addition, or a long axis would show it
-                float t[NT][4] = {};
+                constexpr int kSums = weight_sums(NP);
+                float t[kSums][NT][4] = {};
 #pragma unroll
                 for (int kb = 0; kb < kKeys / 16; ++kb) {
                     uint32_t vf[4];
@@ -494,13 +499,14 @@ __global__ void __launch_bounds__(Ring<D>::kThreads, 1) attn_stream_kernel(const
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = NP - 1; i >= 0; --i)
-                            mma16816<T>(NP > 1 ? t[nt] : o[nt][n], vf, pf[kb][i][nt][0], pf[kb][i][nt][1]);
+                            mma16816<T>(NP > 1 ? t[i % kSums][nt] : o[nt][n], vf, pf[kb][i][nt][0], pf[kb][i][nt][1]);
                 }
                 if (NP > 1)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[nt][n][e] += t[nt][e];
+                        for (int e = 0; e < 4; ++e)
+                            o[nt][n][e] += kSums == 2 ? fmaf(t[kSums - 1][nt][e], 1.f / Half16<T>::kLow, t[0][nt][e]) : t[0][nt][e];
             }
             __syncwarp();  // every lane has read the stage
             if (lane == 0) bar_arrive(&empty[own][stage]);
