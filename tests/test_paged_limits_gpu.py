@@ -66,3 +66,20 @@ def test_paged_attention_tail_far_below_the_largest_key(cuda, G, D, q_type, cach
     bound = bound + floor * v.double().abs().sum(0).repeat_interleave(3, 0)[None] / top
     assert (bound < 0.02 * ref.abs()).all()  # what is asked for can fail
     near(out, ref, bound, f"{nats} nats below")
+
+
+@pytest.mark.parametrize("new,max_kv", FORMS)
+@pytest.mark.parametrize("cache_type", [F16, BF16])
+@pytest.mark.parametrize("size", [2.0 ** -126, 2.0 ** -128, 1e-39, 1e-44])
+def test_paged_attention_subnormal_queries(cuda, G, size, cache_type, new, max_kv):
+    """F32 queries around and below the smallest normal number, zeros among them: scores of 0 but for a rounding, so
+    the output is the mean of the values seen."""
+    g = gen(21)
+    n = 130
+    c, table, k, v = one_request(G, g, n, 2, 64, 16, cache_type)
+    q = torch.sign(normal(g, new, 6, 64)) * size
+    q[..., ::3] = 0.0
+    assert ((q != 0) & (q.abs() <= 2.0 ** -126)).any()
+    out = attend(G, q, c, table, n, 0.125, max_kv=max_kv)
+    ref, bound = attention_ref(q, k, v, n - new, 0.125)
+    near(out, ref, bound, f"size {size}")

@@ -101,14 +101,12 @@ __global__ void __launch_bounds__(Tile<D, NP>::kThreads, Tile<D, NP>::kCtas)
             const int i = (r0 + r) / G, h = kvh * G + (r0 + r) - i * G;
             const char* src = static_cast<const char*>(a.p.q) + (rq.first + (on ? i : 0)) * a.p.nb_q;
             const float2* s = reinterpret_cast<const float2*>(src) + static_cast<int64_t>(h) * (D / 2);
-            // F16 pieces reach down to 2^-24 only: the row is scaled by a power of
-            // two to a largest value in [1, 2)
             float big = 0.f, up = 1.f;
             if (NP == 2) {
                 for (int c = lane; on && c < D / 2; c += 32) big = fmaxf(big, fmaxf(fabsf(s[c].x), fabsf(s[c].y)));
 #pragma unroll
                 for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-                if (big > 0.f && big <= FLT_MAX) up = ldexpf(1.f, min(ilogbf(big), 126));
+                up = row_power(big);
             }
             if (lane == 0) row_scale[r] = up;
             const float down = 1.f / up;

@@ -177,15 +177,12 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[NP]
 // Two pieces of a weight have a sum of products each: second[...] / kLow joins the
 // first's (with one or three pieces there is one sum).
 constexpr int weight_sums(int pieces) { return pieces == 2 ? 2 : 1; }
-// F16 pieces reach down to 2^-24 only, so a row of F32 queries is divided by a
-// power of two that leaves its largest value in [1, 2) (BF16 pieces have F32's
-// range).  `big` is a lane's largest value of the row; 4 lanes hold a row.
-template <int NP>
+// F16 pieces reach down to 2^-24 only, so a row of F32 queries whose largest value
+// is `big` is divided by a power of two that leaves it in [1, 2) (BF16 pieces have
+// F32's range).  The power and its reciprocal are normal numbers: a row of
+// subnormal queries ends below 1.
 __device__ __forceinline__ float row_power(float big) {
-    if (NP != 2) return 1.f;
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    return big > 0.f && big <= FLT_MAX ? ldexpf(1.f, min(ilogbf(big), 126)) : 1.f;
+    return big > 0.f && big <= FLT_MAX ? ldexpf(1.f, max(min(ilogbf(big), 126), -126)) : 1.f;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place

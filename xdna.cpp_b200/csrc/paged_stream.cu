@@ -360,7 +360,11 @@ __global__ void __launch_bounds__(Ring<D>::kThreads, 1) attn_stream_kernel(const
                                 x[k][e] = on ? __ldg(s + k * 8 + e * 4) : make_float2(0.f, 0.f);
                                 big = fmaxf(big, fmaxf(fabsf(x[k][e].x), fabsf(x[k][e].y)));
                             }
-                        up = row_power<NP>(big);
+                        if (NP == 2) {  // 4 lanes hold a row
+                            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                            up = row_power(big);
+                        }
                         const float down = 1.f / up;
 #pragma unroll
                         for (int k = 0; k < kSteps; ++k)
