@@ -83,3 +83,21 @@ def test_paged_attention_subnormal_queries(cuda, G, size, cache_type, new, max_k
     out = attend(G, q, c, table, n, 0.125, max_kv=max_kv)
     ref, bound = attention_ref(q, k, v, n - new, 0.125)
     near(out, ref, bound, f"size {size}")
+
+
+@pytest.mark.parametrize("new,max_kv", FORMS)
+@pytest.mark.parametrize("cache_type", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_paged_attention_small_queries_beside_a_large_one(cuda, G, D, cache_type, new, max_kv):
+    """F32 queries of about 2^-15 of the row's largest value, where keys are about 10^4 and the largest value's key is
+    0: the scores are made of the small ones, which carry their 22 bits all the same."""
+    g = gen(22 + D)
+    n = 300
+    keys = 20000.0 * normal(g, n, 2, D).clamp(-3, 3)
+    keys[..., 5] = 0.0
+    c, table, k, v = one_request(G, g, n, 2, D, 32, cache_type, keys)
+    q = 2.0 ** -15 * math.sqrt(64 / D) * normal(g, new, 6, D)
+    q[..., 5] = 1.0
+    out = attend(G, q, c, table, n, 0.5, max_kv=max_kv)
+    ref, bound = attention_ref(q, k, v, n - new, 0.5)
+    near(out, ref, bound, "small queries")

@@ -178,11 +178,14 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&out)[NP]
 // first's (with one or three pieces there is one sum).
 constexpr int weight_sums(int pieces) { return pieces == 2 ? 2 : 1; }
 // F16 pieces reach down to 2^-24 only, so a row of F32 queries whose largest value
-// is `big` is divided by a power of two that leaves it in [1, 2) (BF16 pieces have
-// F32's range).  The power and its reciprocal are normal numbers: a row of
-// subnormal queries ends below 1.
+// is `big` is divided by a power of two that leaves it in [2^14, 2^15): values down
+// to 2^-17 of it keep their 22 bits, and smaller ones are off by 2^-39 of it, which
+// keys of 65504 do not show.  (In [1, 2) that was 2^-25, and a query of 2^-15 of the
+// largest beside keys of 10^4 had scores off by 10^-3.)  BF16 pieces have F32's
+// range.  The power and its reciprocal are normal numbers: a row of subnormal
+// queries ends below 2^14.
 __device__ __forceinline__ float row_power(float big) {
-    return big > 0.f && big <= FLT_MAX ? ldexpf(1.f, max(min(ilogbf(big), 126), -126)) : 1.f;
+    return big > 0.f && big <= FLT_MAX ? ldexpf(1.f, max(ilogbf(big) - 14, -126)) : 1.f;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place
