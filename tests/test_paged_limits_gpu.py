@@ -101,3 +101,31 @@ def test_paged_attention_small_queries_beside_a_large_one(cuda, G, D, cache_type
     out = attend(G, q, c, table, n, 0.5, max_kv=max_kv)
     ref, bound = attention_ref(q, k, v, n - new, 0.5)
     near(out, ref, bound, "small queries")
+
+
+PLAN_IN_A_FRESH_PROCESS = """
+import sys
+import ggml_b200 as G
+from test_paged_gpu import Plan, lens_of, plan_ref
+B = int(sys.argv[1])
+for most_new, most in ((1, 2000), (1, 1 << 30), (9, 1 << 30)):  # a CTA, 8 CTAs, 16 CTAs
+    cached, new = lens_of(B, 40, most_new, B)
+    while sum(new) > most:
+        new = [x if i % 4 == 0 else 0 for i, x in enumerate(new)]
+    p = Plan(G, cached, new, 16, 4, sum(new), sum(new), seed=2)
+    ref = plan_ref(cached, new, p.rows, p.free_list, 0, 16, sum(new))
+    p.run(G)
+    assert p.status.item() == 0 and p.got() == ref, (B, most_new)
+print("same plans")
+"""
+
+
+@pytest.mark.parametrize("B", [6079, 6144])
+def test_kv_plan_first_call_next_to_the_shared_memory_limit(cuda, G, B):
+    """Request counts whose sums fit 48 KB of shared memory alone, but not beside what a kernel declares, as the first
+    call of a process."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    path = os.pathsep.join([here, os.path.join(here, os.pardir, "xdna.cpp_b200")])
+    got = subprocess.run([sys.executable, "-c", PLAN_IN_A_FRESH_PROCESS, str(B)], capture_output=True, text=True,
+                         env={**os.environ, "PYTHONPATH": path}, timeout=300)
+    assert got.returncode == 0 and "same plans" in got.stdout, got.stderr[-2000:]

@@ -208,26 +208,32 @@ __global__ void __launch_bounds__(kThreads) kv_plan_kernel(const __grid_constant
     }
 }
 
-}  // namespace
-
-cudaError_t kv_plan_launch(const struct b200_kv_plan_args& p, cudaStream_t stream) {
+template <int kCtas, int kEach>
+cudaError_t launch_ctas(const struct b200_kv_plan_args& p, cudaStream_t stream) {
+    constexpr auto kernel = kv_plan_kernel<kCtas, kEach>;
     int log_bs = 4;
     while ((1 << log_bs) < p.block_size) ++log_bs;
-    const size_t smem = 2 * static_cast<size_t>(p.n_seqs) * sizeof(int);
-    const int ctas = p.max_tokens <= kOneCtaTokens ? 1 : p.max_tokens <= kShortTokens ? kCluster : kWide;
-    void (*kernel)(const struct b200_kv_plan_args, int) = ctas == 1          ? kv_plan_kernel<1, 1>
-                                                          : ctas == kCluster ? kv_plan_kernel<kCluster, 1>
-                                                                             : kv_plan_kernel<kWide, 4>;
-    if (ctas == kWide) {
+    if (kCtas == kWide) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
     }
-    if (smem > 48 * 1024) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // Without the attribute a kernel has 48 KB, of which its static shared memory is
+    // part.  It is set to the most any call needs: calls at once need one limit.
+    constexpr int kEachSeq = 2 * sizeof(int), kAlways = 32 * 1024;
+    const size_t smem = static_cast<size_t>(p.n_seqs) * kEachSeq;
+    if (smem > kAlways) {
+        const cudaError_t e = allow_smem<kernel>(kMaxSeqs * kEachSeq);
         if (e != cudaSuccess) return e;
     }
-    return launch_pdl(kernel, dim3(ctas), dim3(kThreads), smem, stream, ctas, p, log_bs);
+    return launch_pdl(kernel, dim3(kCtas), dim3(kThreads), smem, stream, kCtas, p, log_bs);
+}
+
+}  // namespace
+
+cudaError_t kv_plan_launch(const struct b200_kv_plan_args& p, cudaStream_t stream) {
+    if (p.max_tokens <= kOneCtaTokens) return launch_ctas<1, 1>(p, stream);
+    if (p.max_tokens <= kShortTokens) return launch_ctas<kCluster, 1>(p, stream);
+    return launch_ctas<kWide, 4>(p, stream);
 }
 
 }  // namespace xb

@@ -15,6 +15,7 @@ namespace xb {
 // Streaming multiprocessors of the current device (0 without one).
 int sm_count();
 
+constexpr int kMaxSeqs = 16384;  // requests of a plan
 cudaError_t kv_plan_launch(const struct b200_kv_plan_args& p, cudaStream_t stream);
 
 cudaError_t qk_norm_rope_launch(const struct b200_qk_norm_rope_args& p, const struct b200_kv_cache& kv,

@@ -63,7 +63,7 @@ bool check_rows(const char* what, const char* name, const void* ptr, int64_t& nb
 
 bool check_plan(const struct b200_kv_plan_args& p) {
     const char* what = "b200_kv_plan";
-    REFUSE_IF(p.n_seqs < 0 || p.n_seqs > 16384, "%s: n_seqs %d is not in 0 .. 16384", what, p.n_seqs);
+    REFUSE_IF(p.n_seqs < 0 || p.n_seqs > kMaxSeqs, "%s: n_seqs %d is not in 0 .. %d", what, p.n_seqs, kMaxSeqs);
     REFUSE_IF(!block_size_ok(p.block_size), "%s: block_size %d is not 16, 32, 64, 128 or 256", what, p.block_size);
     REFUSE_IF(p.table_width < 0 || p.table_width > kMaxInt || p.n_free < 0 || p.n_free > kMaxInt || p.max_tokens < 0 ||
                   p.max_tokens > kMaxInt,
