@@ -375,7 +375,8 @@ size_t b200_paged_attention_workspace(const struct b200_paged_attention_args *p,
 int b200_paged_attention(const struct b200_paged_attention_args *p, const struct b200_kv_cache *kv, void *stream);
 /* Status of the attention kernels' bounded waits on the current CUDA device:
  * *status = 1 if a wait inside a kernel ran out (2 s) since the last call, whose
- * output is then not valid, else 0; the word is cleared.  Synchronises. */
+ * output is then not valid, else 0; the word is cleared.  Waits for all streams of
+ * the device first; not for use while a stream is being captured. */
 int b200_paged_attention_error(int *status);
 
 #ifdef __cplusplus

@@ -129,3 +129,24 @@ def test_kv_plan_first_call_next_to_the_shared_memory_limit(cuda, G, B):
     got = subprocess.run([sys.executable, "-c", PLAN_IN_A_FRESH_PROCESS, str(B)], capture_output=True, text=True,
                          env={**os.environ, "PYTHONPATH": path}, timeout=300)
     assert got.returncode == 0 and "same plans" in got.stdout, got.stderr[-2000:]
+
+
+def test_paged_attention_error_waits_for_every_stream(cuda, G):
+    """The status is that of all calls made before it, also of those still in work on a stream that the legacy stream
+    does not wait for."""
+    side, status = torch.cuda.Stream(), C.c_int(-1)
+    g = gen(23)
+    c, table, _, _ = one_request(G, g, 40, 2, 64, 16, F16)
+    q = normal(g, 1, 4, 64)
+    out, cu, kv = torch.empty_like(q), ints([0, 1]), ints([40])
+    args, _workspace = run_attention(G, q, out, c, cu, kv, table, 0.125)
+    G.check(G.lib().b200_paged_attention_error(C.byref(status)), "warm-up: what is loaded at its first use")
+    ran = torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)  # about 0.2 s
+        G.check(G.lib().b200_paged_attention(C.byref(args), C.byref(c.rec), side.cuda_stream), "paged_attention")
+        ran.record()
+    assert not ran.query()
+    G.check(G.lib().b200_paged_attention_error(C.byref(status)), "paged_attention_error")
+    assert ran.query() and status.value == 0

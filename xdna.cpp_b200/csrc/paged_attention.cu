@@ -405,8 +405,12 @@ cudaError_t paged_attention_launch(const struct b200_paged_attention_args& p, co
 }
 
 cudaError_t paged_error_status(int* out) {
+    // all streams: the copy that reads a word waits for the legacy stream alone
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) return e;
     int stream = 0, chunk = 0;
-    const cudaError_t e = stream_error(&stream), f = chunk_error(&chunk);
+    e = stream_error(&stream);
+    const cudaError_t f = chunk_error(&chunk);
     *out = stream || chunk;
     return e != cudaSuccess ? e : f;
 }

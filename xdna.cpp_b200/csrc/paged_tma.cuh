@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda.h>
 
+#include <mutex>
+
 #include "paged_attn.cuh"
 
 namespace xb {
@@ -11,14 +13,18 @@ namespace {
 constexpr unsigned long long kWaitNs = 2000000000ull;  // of %globaltimer
 
 // Set when a wait in one of this file's kernels has run out.
-__device__ int g_wait_error;
+__device__ int g_wait_error, g_wait_taken;
 
+__global__ void take_error_kernel() { g_wait_taken = atomicExch(&g_wait_error, 0); }
+
+// Reads and clears the word in one step, so that none is lost that a kernel of
+// another thread sets meanwhile.  The caller has waited for the device.
 inline cudaError_t take_wait_error(int* out) {
-    int v = 0, zero = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&v, g_wait_error, sizeof(int));
-    if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(g_wait_error, &zero, sizeof(int));
-    *out = v;
-    return e;
+    static std::mutex one;  // at a time: g_wait_taken is shared
+    std::lock_guard<std::mutex> lock(one);
+    take_error_kernel<<<1, 1>>>();
+    const cudaError_t e = cudaGetLastError();
+    return e != cudaSuccess ? e : cudaMemcpyFromSymbol(out, g_wait_taken, sizeof(int));
 }
 
 __device__ __forceinline__ void bar_init(uint64_t* b, int count) {
