@@ -150,3 +150,30 @@ def test_paged_attention_error_waits_for_every_stream(cuda, G):
     assert not ran.query()
     G.check(G.lib().b200_paged_attention_error(C.byref(status)), "paged_attention_error")
     assert ran.query() and status.value == 0
+
+
+@pytest.mark.parametrize("new,max_kv", FORMS)
+@pytest.mark.parametrize("q_type,cache_type", TYPES)
+@pytest.mark.parametrize("cap", [50.0, 64.0, 65.0, 1e3, 1e4, 1e6])
+def test_paged_attention_large_caps(cuda, G, cap, q_type, cache_type, new, max_kv):
+    """A cap far above the scores changes them by less and less: no term of the error grows with the cap.
+
+    tanh's argument and value, and their products, are off by a few roundings of the score itself (8 U counted); up to
+    a cap of 64 the kernel of many rows takes tanh from an exponential instead, off by 2^-21 of the cap."""
+    g = gen(24)
+    n = 260
+    c, table, k, v = one_request(G, g, n, 2, 64, 16, cache_type)
+    q = (3 * normal(g, new, 6, 64)).to(q_type)
+    out = attend(G, q, c, table, n, 0.125, max_kv=max_kv, cap=cap)
+    half = 0.0 if q_type == F32 else HALF[cache_type]
+    ref, _ = attention_ref(q, k, v, n - new, 0.125, cap=cap)
+    _, bound = attention_ref(q, k, v, n - new, 0.125, weight_half=half)  # all but the cap's own error
+    kk, vv = (x.double().repeat_interleave(3, 1) for x in (k, v))
+    s = torch.einsum("nhd,khd->hnk", q.double(), kk) * 0.125
+    seen = torch.arange(n, device="cuda")[None, :] <= torch.arange(n - new, n, device="cuda")[:, None]
+    w = torch.softmax((cap * torch.tanh(s / cap)).masked_fill(~seen, -math.inf), -1)
+    off = 8 * U * s.abs().amax() + (2.0 ** -21 * cap if cap <= 64 and new == 90 and q_type != F32 else 0.0)
+    # a score off by d: a weight and the row's sum off by d each; the bound's own weights are those without the cap
+    most = torch.einsum("hnk,khd->nhd", w, vv.abs())
+    plain = torch.einsum("hnk,khd->nhd", torch.softmax(s.masked_fill(~seen, -math.inf), -1), vv.abs())
+    near(out, ref, bound * (most / plain).clamp(min=1) + 2 * off * most, f"cap {cap}")
