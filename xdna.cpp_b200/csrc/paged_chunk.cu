@@ -315,9 +315,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                         }
                     }
                 } while (ok && w.next<R, kKeys>(a));
-                if (!ok)  // copies in flight land before the CTA ends
-                    for (uint32_t i = n < L::kStages ? 0 : n - L::kStages; i < n; ++i)
-                        bar_wait(&full[i % L::kStages], (i / L::kStages) & 1, nullptr);
+                // Copies in flight land before the CTA ends, also where the warps that they
+                // are for have given up.
+                for (uint32_t i = n < L::kStages ? 0 : n - L::kStages; i < n; ++i)
+                    bar_wait(&full[i % L::kStages], (i / L::kStages) & 1, nullptr);
             } else if (warp < kMmaWarp + L::kQ) {
                 // ----------------------------------------------------- matrix instructions
                 constexpr uint32_t kIdescS = instruction<T>(kKeys, false), kIdescO = instruction<T>(D, true);
@@ -394,11 +395,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                     }
                     --i;  // the last step has no tile of its own
                 } while (ok && w.next<R, kKeys>(a));
-                if (!ok) {  // matrix instructions in flight end before TMEM is freed
-                    if (elect_one()) tc_commit(&bars.drain[q]);
-                    __syncwarp();
-                    bar_wait(&bars.drain[q], 0, nullptr);
-                }
+                // matrix instructions in flight end before TMEM is freed, whoever has given up
+                if (elect_one()) tc_commit(&bars.drain[q]);
+                __syncwarp();
+                bar_wait(&bars.drain[q], 0, nullptr);
             }
         } else {
             // ------------------------------------------------------------------ softmax

@@ -309,9 +309,10 @@ __global__ void __launch_bounds__(Ring<D>::kThreads, 1) attn_stream_kernel(const
                 }
                 __syncwarp();
             }
-            if (!ok)  // copies in flight land before the CTA ends
-                for (uint32_t i = done < L::kStages ? 0 : done - L::kStages; i < done; ++i)
-                    bar_wait(&full[own][i % L::kStages], (i / L::kStages) & 1, nullptr);
+            // Copies in flight land before the CTA ends, also where the warp that they are
+            // for has given up.
+            for (uint32_t i = done < L::kStages ? 0 : done - L::kStages; i < done; ++i)
+                bar_wait(&full[own][i % L::kStages], (i / L::kStages) & 1, nullptr);
             if constexpr (!kJoin) return;
         }
 
