@@ -353,7 +353,7 @@ int b200_qk_norm_rope(const struct b200_qk_norm_rope_args *p, const struct b200_
  * of that request that do not see them). */
 struct b200_paged_attention_args {
     int64_t n_tokens;        /* rows of q and out */
-    int32_t n_seqs, heads;
+    int32_t n_seqs, heads;   /* n_seqs <= 2^24 */
     int32_t q_type, out_type;
     const void *q;           /* [n_tokens][heads][head_dim], 16-byte aligned */
     void *out;

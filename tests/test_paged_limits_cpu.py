@@ -1,0 +1,16 @@
+"""Refusals of the paged KV cache operators at the ends of their ranges, without a GPU."""
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+
+from test_paged_cpu import attn, cache, refused
+
+
+@pytest.mark.parametrize("n_seqs", [2 ** 24 + 1, 2 ** 31 - 1])
+def test_attention_refuses_more_requests_than_it_counts(G, n_seqs):
+    """The threads' shares of the requests are counted in 32 bits: near 2^31 the last ones would pass them."""
+    L, p, c = G.lib(), attn(G, n_seqs=n_seqs), cache(G)
+    refused(G, L.b200_paged_attention(C.byref(p), C.byref(c), None), "n_seqs")
+    assert L.b200_paged_attention_workspace(C.byref(p), C.byref(c)) == 0

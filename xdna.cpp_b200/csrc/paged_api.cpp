@@ -13,6 +13,9 @@ namespace xb {
 namespace {
 
 constexpr int64_t kMaxInt = 0x7fffffff;
+// Requests of an attention call: every CTA reads all of their lengths, and the
+// threads' shares of them are counted in 32 bits.
+constexpr int kMaxAttnSeqs = 1 << 24;
 
 size_t type_size(int type) {
     return type == GGML_TYPE_F32 ? 4 : type == GGML_TYPE_F16 || type == GGML_TYPE_BF16 ? 2 : 0;
@@ -106,6 +109,7 @@ bool check_attention(struct b200_paged_attention_args& p, struct b200_kv_cache& 
                   p.n_tokens > kMaxInt / p.heads,
               "%s: n_tokens %ld, n_seqs %d, heads %d over kv_heads %d", what, long(p.n_tokens), p.n_seqs, p.heads,
               kv.kv_heads);
+    REFUSE_IF(p.n_seqs > kMaxAttnSeqs, "%s: n_seqs %d is not in 0 .. 2^24", what, p.n_seqs);
     REFUSE_IF(p.table_width < 0 || p.table_width > kMaxInt, "%s: table_width %ld", what, long(p.table_width));
     REFUSE_IF(p.max_new < 0 || p.max_kv < 0 || p.window < 0, "%s: max_new %d, max_kv %d or window %d is negative", what,
               p.max_new, p.max_kv, p.window);
