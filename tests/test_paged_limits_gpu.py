@@ -177,3 +177,17 @@ def test_paged_attention_large_caps(cuda, G, cap, q_type, cache_type, new, max_k
     most = torch.einsum("hnk,khd->nhd", w, vv.abs())
     plain = torch.einsum("hnk,khd->nhd", torch.softmax(s.masked_fill(~seen, -math.inf), -1), vv.abs())
     near(out, ref, bound * (most / plain).clamp(min=1) + 2 * off * most, f"cap {cap}")
+
+
+def test_paged_decode_goes_on_after_a_refused_step(cuda, G):
+    """A step that the cache has no room for leaves the length as it was: a shorter one still fits."""
+    import decode_harness as D
+
+    tiny = dict(hidden=256, layers=1, heads=4, kv_heads=2, head_dim=64, inter=512, vocab=992, theta=1.0e6, eps=1.0e-6)
+    att = D.DeviceAttention(cuda, tiny, 32)
+    att.begin(20)
+    with pytest.raises(RuntimeError, match="32 tokens"):
+        att.begin(13)
+    att.begin(12)
+    torch.cuda.synchronize()
+    assert att.status.item() == 0 and att.cached.item() == 32

@@ -163,13 +163,13 @@ class DeviceAttention:
 
     def begin(self, n: int) -> None:
         """Positions and cache slots of n new tokens; lengths and table move on, on the device."""
-        self.length += n
-        if self.length > self.table.shape[1] * self.bs:
+        if self.length + n > self.table.shape[1] * self.bs:
             raise RuntimeError(f"the KV cache holds {self.table.shape[1] * self.bs} tokens")
         if n not in self.steps:
             self.steps[n] = self._step(n)
         self.step = self.steps[n]
         G.check(G.lib().b200_kv_plan(C.byref(self.step["plan"]), self._stream()), "kv_plan")
+        self.length += n
 
     def attend(self, layer: int, q, k, v):
         s, L, cache = self.step, G.lib(), C.byref(self.caches[layer])
