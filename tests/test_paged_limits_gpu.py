@@ -12,7 +12,8 @@ import pytest
 import torch
 
 from paged_helpers import HALF, U, Cache, attention_ref, ints, run_attention
-from test_paged_gpu import BF16, F16, F32, TYPES, gen, near, no_wait_ran_out, normal  # noqa: F401 (a fixture)
+from test_paged_gpu import (BF16, F16, F32, TYPES, check_attention, gen, near, no_wait_ran_out,  # noqa: F401 (a fixture)
+                            normal)
 
 pytestmark = pytest.mark.gpu
 
@@ -191,3 +192,89 @@ def test_paged_decode_goes_on_after_a_refused_step(cuda, G):
     att.begin(12)
     torch.cuda.synchronize()
     assert att.status.item() == 0 and att.cached.item() == 32
+
+
+@pytest.mark.parametrize("new,max_kv", FORMS)
+@pytest.mark.parametrize("cache_type", [F16, BF16])
+@pytest.mark.parametrize("power", [20, 60, 100, -20, -60, -100])
+def test_paged_attention_queries_of_any_power(cuda, G, power, cache_type, new, max_kv):
+    """F32 queries times a power of two, with the scale divided by it, are the same scores: the normal bound holds, at
+    10^30 and at 10^-30 too."""
+    g = gen(25)
+    n = 130
+    c, table, k, v = one_request(G, g, n, 2, 64, 16, cache_type)
+    q = 1.5 * normal(g, new, 6, 64)
+    out = attend(G, q * 2.0 ** power, c, table, n, 0.125 * 2.0 ** -power, max_kv=max_kv)
+    ref, bound = attention_ref(q, k, v, n - new, 0.125)
+    near(out, ref, bound, f"2^{power}")
+
+
+@pytest.mark.parametrize("lens", [[(4000, 1)], [(20000, 1), (300, 1)], [(3000, 400), (900, 1), (5000, 1)], [(2000, 700)]],
+                         ids=str)
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("q_type,cache_type", TYPES)
+def test_paged_attention_repeats_itself(cuda, G, lens, D, q_type, cache_type):
+    """The same call gives the same bits, whatever else the GPU does beside it."""
+    g = gen(26)
+    pages = [-(-n // 16) for n, _ in lens]
+    table = torch.full((len(lens), max(pages)), -1, dtype=torch.int32)
+    cu, at = [0], 0
+    for b, (_, m) in enumerate(lens):
+        table[b, : pages[b]] = torch.arange(at, at + pages[b])
+        at += pages[b]
+        cu.append(cu[-1] + m)
+    c = Cache(G, at, 4, 16, D, cache_type)
+    c.k.copy_(normal(g, *c.k.shape))
+    c.v.copy_(normal(g, *c.v.shape))
+    q = (1.5 * normal(g, cu[-1], 16, D)).to(q_type)
+    outs, table, cu, kv = [torch.empty_like(q) for _ in range(4)], table.cuda(), ints(cu), ints([n for n, _ in lens])
+    hints, side, x = dict(max_new=max(m for _, m in lens), max_kv=max(n for n, _ in lens)), torch.cuda.Stream(), None
+    for i, out in enumerate(outs):
+        if i % 2:
+            with torch.cuda.stream(side):
+                x = torch.randn(2048, 2048, device="cuda") @ torch.randn(2048, 2048, device="cuda")
+        run_attention(G, q, out, c, cu, kv, table, 0.09, **hints)
+        torch.cuda.synchronize()
+    assert all(torch.equal(outs[0], o) for o in outs[1:]) and x is not None
+
+
+@pytest.mark.parametrize("q_type,cache_type", TYPES)
+@pytest.mark.parametrize("new", [1, 12, 200])
+def test_paged_attention_two_calls_at_once(cuda, G, new, q_type, cache_type):
+    """Two calls on two streams, each with a workspace of its own, in work at the same time."""
+    g = gen(27)
+    n, sides = 3000, [torch.cuda.Stream(), torch.cuda.Stream()]
+    c, table, k, v = one_request(G, g, n, 2, 128, 16, cache_type)
+    calls = []
+    for side in sides:
+        q = normal(g, new, 16, 128).to(q_type)
+        out, cu, kv = torch.zeros_like(q), ints([0, new]), ints([n])
+        calls.append((q, out, cu, kv, run_attention(G, q, out, c, cu, kv, table, 0.09, max_kv=100000, call=False)))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for side, (_, _, _, _, (args, _)) in zip(sides, calls):
+            G.check(G.lib().b200_paged_attention(C.byref(args), C.byref(c.rec), side.cuda_stream), "paged_attention")
+    torch.cuda.synchronize()
+    for q, out, *_ in calls:
+        ref, bound = attention_ref(q, k, v, n - new, 0.09, weight_half=0.0 if q_type == F32 else HALF[cache_type])
+        near(out, ref, bound, "two streams")
+
+
+@pytest.mark.parametrize("q_type,cache_type", TYPES)
+@pytest.mark.parametrize("H,KH", [(300, 1), (40, 40)])
+def test_paged_attention_many_heads(cuda, G, H, KH, q_type, cache_type):
+    check_attention(G, [(100, 1), (33, 2), (257, 20)], H, KH, 64, q_type, cache_type, 32, seed=H)
+
+
+@pytest.mark.parametrize("new,max_kv", FORMS)
+@pytest.mark.parametrize("q_type,cache_type", TYPES)
+def test_paged_attention_window_behind_the_table_row(cuda, G, q_type, cache_type, new, max_kv):
+    """Keys behind a table row do not exist: rows whose window lies behind it all see none and are 0."""
+    g = gen(28)
+    c, _, _, _ = one_request(G, g, 32, 2, 64, 16, cache_type)
+    q = normal(g, new, 6, 64).to(q_type)
+    for table in (ints([[1, 0]]), torch.empty((1, 0), dtype=torch.int32, device="cuda")):
+        out = torch.full_like(q, 7.0)
+        run_attention(G, q, out, c, ints([0, new]), ints([400]), table, 0.125, window=10, max_kv=max_kv)
+        torch.cuda.synchronize()
+        assert (out == 0).all()
