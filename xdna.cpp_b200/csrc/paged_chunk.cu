@@ -67,7 +67,9 @@ struct Shape {
     static constexpr int kTile = kHalves * 128 * 128;  // bytes of 128 rows
     // 8 softmax warps and a matrix warp per query tile, a loading warp; made up to
     // whole groups of 4 warps, so that with two query tiles the softmax warps can
-    // take registers from the others
+    // take registers from the others.  The compiler works to the launch's 96 all the
+    // same: 148 bytes of a thread are spilled at heads of 64 to 128 (288 with a cap or
+    // bias), none to speak of at 256 (168 registers).
     static constexpr int kThreads = kQ * 256 + 128;
     static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 64;
     static_assert(kQ == 1 || 512 * kSoftmaxRegs + 128 * kOtherRegs <= 640 * kLaunchRegs, "registers of the launch");
@@ -479,8 +481,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) attn_chunk_kernel(const
                             const bool cut = t * kKeys < all_lo || (t + 1) * kKeys > all_hi;
                             const float pre = kGeneral ? 1.f : a.pre;
                             const int k0 = first - j0, k1 = last - j0;
-                            // Columns of S, 16 worked on and 16 on their way (so few registers that 16
-                            // softmax warps fit).  First pass: the maximum of half the row, in eight
+                            // Columns of S, 16 worked on and 16 on their way (16 softmax warps leave no
+                            // registers for more).  First pass: the maximum of half the row, in eight
                             // chains.  Scores that the cap, the bias or a hidden key change go back
                             // for the second pass.
                             float s0[16], s1[16], tops[8];

@@ -8,8 +8,8 @@
 // are dealt out as one equal contiguous run to each of 4 streams per SM, whatever
 // the lengths.  A stream is a warp that works and a warp that loads for it: TMA
 // boxes, page by page, into a ring of 48 KB (with warps that issue their own loads
-// one token over 1001 keys took 7.9 us, now 6.5).  No stream waits for another one.  An item that ends in another
-// stream than it began in leaves a partial (m, l, o) in the workspace for each
+// one token over 1001 keys took 0.9 us more).  No stream waits for another one.  An
+// item that ends in another stream than it began in leaves a partial (m, l, o) in the workspace for each
 // stream; combine_kernel joins them in stream order, so results do not depend on
 // timing.  Where there are few items with few keys, a cluster takes each instead
 // and joins its sums in shared memory (kJoin).
@@ -20,7 +20,8 @@
 // rate of the fifth-generation tensor cores would not help: a unit's products take
 // about a fifth of the time its bytes take.
 // The running maximum is moved only when a score passes it by 8 (a weight then
-// is at most 2^8), which a vote finds out; moving it takes the shuffles.
+// is at most 2^8; what F16 makes of small ones: Half16), which a vote finds out;
+// moving it takes the shuffles.
 //
 // Measured on a B200: one request of 130001 BF16 keys, 64 query and 8 KV heads of
 // 128: 93 us, 5.7 TB/s of K and V; 64 requests of up to 8193 F16 keys with F32
@@ -34,7 +35,6 @@
 namespace xb {
 namespace {
 
-constexpr int kMinUnits = 1;     // units per stream below which fewer streams run
 constexpr float kSlack = 8.f;    // log2 of the largest weight (before kWeightLog2)
 constexpr int kCluster = 8;      // CTAs that share an item of the joining form
 // Keys up to which the joining form is taken: it uses 8 SMs an item.  2, 8 KV
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(Ring<D>::kThreads, 1) attn_stream_kernel(const
             __syncthreads();
         }
         all = before[kThreads];
-        streams = min(static_cast<long long>(g.streams), max(1LL, all / kMinUnits));
+        streams = min(static_cast<long long>(g.streams), max(1LL, all));
         // neighbouring streams lie on different SMs: a short run of units uses all of them
         me = static_cast<long long>(own) * gridDim.x + blockIdx.x;
         if (lane == 0 && !loads && me < g.streams) g.heads[me].parts = 0;
@@ -652,14 +652,15 @@ cudaError_t launch_rows(const AttnArgs& a, cudaStream_t stream) {
     if (items.join) return launch_form<T, D, NP, NT, true>(c, static_cast<int>(items.count) * kCluster, stream);
     // no more streams than the hints give work for
     const int64_t units = std::min<int64_t>(items.count, 1 << 30) * std::max<int64_t>(1, (int64_t(a.p.max_kv) + L::kKeys - 1) / L::kKeys);
-    g.streams = static_cast<int>(std::min<int64_t>(sms * L::kWarps, std::max<int64_t>(1, units / kMinUnits)));
+    g.streams = static_cast<int>(std::min<int64_t>(sms * L::kWarps, std::max<int64_t>(1, units)));
     const cudaError_t e = launch_form<T, D, NP, NT, false>(c, std::min(sms, g.streams), stream);
     if (e != cudaSuccess) return e;
     return combine_launch<D, 8 * NT>(g, items.count, stream);
 }
 
 // Rows of an item: as few 8-column blocks as the hints ask for, as many as the
-// registers hold beside q's NP pieces and o (255 a thread; more would spill).
+// registers hold beside q's NP pieces and o (255 a thread: four blocks of heads of 96
+// spill 124 bytes, two with F32 queries up to 32, the others none).
 constexpr int most_blocks(int D, bool f32) { return D > 128 ? 1 : f32 || D > 96 ? 2 : 4; }
 int row_blocks(const AttnArgs& a) {
     const int64_t rows = static_cast<int64_t>(a.p.max_new) * a.group;
