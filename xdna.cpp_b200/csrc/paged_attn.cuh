@@ -127,8 +127,8 @@ __device__ __forceinline__ void store_one(const AttnArgs& a, int64_t row, int he
 //
 // A softmax weight is 2^8 at most (the running maximum moves when a score passes
 // it by 8), and most of a long row's are small.  F16 ends at 2^-24, below which a
-// weight would be lost for V while the sum of weights still counts it (32 keys in
-// 33 at 17 nats below the 33rd: all of their share of the output); so weights are
+// weight would be lost for V while the sum of weights still counts it (31 keys in
+// 32 at 17 nats below the 32nd: all of their share of the output); so weights are
 // formed times 2^kWeightLog2, up to 2^15, and o and l carry the same factor until
 // they are divided.
 template <typename T>

@@ -22,8 +22,7 @@ __global__ void take_error_kernel() { g_wait_taken = atomicExch(&g_wait_error, 0
 inline cudaError_t take_wait_error(int* out) {
     static std::mutex one;  // at a time: g_wait_taken is shared
     std::lock_guard<std::mutex> lock(one);
-    take_error_kernel<<<1, 1>>>();
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = cudaLaunchKernel(take_error_kernel, dim3(1), dim3(1), nullptr, 0, nullptr);
     return e != cudaSuccess ? e : cudaMemcpyFromSymbol(out, g_wait_taken, sizeof(int));
 }
 
