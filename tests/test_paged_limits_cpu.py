@@ -14,3 +14,10 @@ def test_attention_refuses_more_requests_than_it_counts(G, n_seqs):
     L, p, c = G.lib(), attn(G, n_seqs=n_seqs), cache(G)
     refused(G, L.b200_paged_attention(C.byref(p), C.byref(c), None), "n_seqs")
     assert L.b200_paged_attention_workspace(C.byref(p), C.byref(c)) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(scale=0.1, logit_softcap=1e-39), dict(scale=-2e38), dict(scale=3e38)], ids=str)
+def test_attention_refuses_factors_past_f32(G, kw):
+    """The factor that takes q.k to tanh's argument, or to an exponent of 2: an infinite one would turn scores of 0 into
+    NaN."""
+    refused(G, G.lib().b200_paged_attention(C.byref(attn(G, **kw)), C.byref(cache(G)), None), "scale")

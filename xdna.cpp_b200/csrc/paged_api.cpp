@@ -116,6 +116,10 @@ bool check_attention(struct b200_paged_attention_args& p, struct b200_kv_cache& 
     REFUSE_IF(!std::isfinite(p.scale) || !(p.logit_softcap >= 0.f && std::isfinite(p.logit_softcap)) ||
                   !(p.max_bias >= 0.f && std::isfinite(p.max_bias)),
               "%s: scale %g, logit_softcap %g, max_bias %g", what, p.scale, p.logit_softcap, p.max_bias);
+    // the score's factor in units of log 2, and (with a cap) that of tanh's exponential
+    const float factor = p.logit_softcap != 0.f ? 4.f * (p.scale / p.logit_softcap) : 2.f * p.scale;
+    REFUSE_IF(!std::isfinite(factor), "%s: scale %g with logit_softcap %g passes F32's range", what, p.scale,
+              p.logit_softcap);
     if (p.n_tokens == 0 || p.n_seqs == 0) return true;
     REFUSE_IF(!p.cu_new || !p.kv_lens || (p.table_width && !p.block_table), "%s: null pointer", what);
     const int64_t row = int64_t(p.heads) * kv.head_dim;
