@@ -5,7 +5,7 @@ import ctypes as C
 
 import pytest
 
-from test_paged_cpu import attn, cache, refused
+from test_paged_cpu import attn, cache, refused, rope
 
 
 @pytest.mark.parametrize("n_seqs", [2 ** 24 + 1, 2 ** 31 - 1])
@@ -21,3 +21,9 @@ def test_attention_refuses_factors_past_f32(G, kw):
     """The factor that takes q.k to tanh's argument, or to an exponent of 2: an infinite one would turn scores of 0 into
     NaN."""
     refused(G, G.lib().b200_paged_attention(C.byref(attn(G, **kw)), C.byref(cache(G)), None), "scale")
+
+
+@pytest.mark.parametrize("kw", [dict(out_type=1), dict(n_tokens=2, nb_q=4096), dict(n_tokens=2, nb_q_out=4096)], ids=str)
+def test_rope_in_place_refuses_another_type_or_stride(G, kw):
+    """Rows written over rows that are still to be read."""
+    refused(G, G.lib().b200_qk_norm_rope(C.byref(rope(G, **kw)), C.byref(cache(G)), None), "q_out is q")

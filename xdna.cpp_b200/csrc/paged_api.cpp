@@ -94,10 +94,15 @@ bool check_rope(struct b200_qk_norm_rope_args& p, struct b200_kv_cache& kv) {
     REFUSE_IF(!aligned16(p.q_norm) || !aligned16(p.k_norm), "%s: norm weights must be 16-byte aligned", what);
     if (p.n_tokens == 0) return true;
     REFUSE_IF(!p.positions || !p.slots, "%s: null pointer", what);
-    return check_rows(what, "q", p.q, p.nb_q, int64_t(p.heads) * kv.head_dim * in) &&
-           check_rows(what, "k", p.k, p.nb_k, int64_t(kv.kv_heads) * kv.head_dim * in) &&
-           check_rows(what, "v", p.v, p.nb_v, int64_t(kv.kv_heads) * kv.head_dim * in) &&
-           check_rows(what, "q_out", p.q_out, p.nb_q_out, int64_t(p.heads) * kv.head_dim * out);
+    if (!check_rows(what, "q", p.q, p.nb_q, int64_t(p.heads) * kv.head_dim * in) ||
+        !check_rows(what, "k", p.k, p.nb_k, int64_t(kv.kv_heads) * kv.head_dim * in) ||
+        !check_rows(what, "v", p.v, p.nb_v, int64_t(kv.kv_heads) * kv.head_dim * in) ||
+        !check_rows(what, "q_out", p.q_out, p.nb_q_out, int64_t(p.heads) * kv.head_dim * out))
+        return false;
+    REFUSE_IF(p.q_out == p.q && (p.in_type != p.out_type || (p.n_tokens > 1 && p.nb_q != p.nb_q_out)),
+              "%s: q_out is q with another type (%d, %d) or stride (%ld, %ld)", what, p.in_type, p.out_type,
+              long(p.nb_q), long(p.nb_q_out));
+    return true;
 }
 
 bool check_attention(struct b200_paged_attention_args& p, struct b200_kv_cache& kv) {
